@@ -28,7 +28,11 @@ SOURCES = ["sdfx_core.hip", "raymarching.hip", "gridencoder.hip", "gridencoder_f
 ARCH = "gfx950"
 # -ffp-contract=off: the march / encode arithmetic must not gain FMAs the source does not spell
 # out (bit-exact ray counts and fp32 features against the CPU oracle).
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32. hipcc -O3 forms them from ordinary float code, and some of their forms have given
+# wrong results on MI355X now and then; the scalar instructions round the same way, so no result changes. (The host pass warns that
+# it does not know the feature: harmless.)
 FLAGS = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-fno-fast-math",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
          "-Wall", "-Wno-unused-function", "-Wno-pass-failed", "-I", INCLUDE]
 
 
@@ -41,6 +45,7 @@ def hipcc() -> str:
 
 def _deps_mtime(devtools: bool = False) -> float:
     hdrs = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".h")] + [os.path.join(INCLUDE, "sdfx.h")]
+    hdrs.append(os.path.abspath(__file__))       # (the flags)
     if devtools and os.path.isdir(DEVTOOLS_KERNELS):
         hdrs += [os.path.join(DEVTOOLS_KERNELS, f) for f in os.listdir(DEVTOOLS_KERNELS) if f.endswith(".h")]
     return max(os.path.getmtime(h) for h in hdrs)

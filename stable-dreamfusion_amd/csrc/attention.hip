@@ -182,7 +182,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_fwd(const _Float16* __restr
         const float m_new = fmaxf(m_run, mx * s.c);
         const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
         m_run = m_new;
-        f2 psum2 = {0.f, 0.f};                         // (pairs: v_pk_fma_f32 / v_pk_add_f32 — half the issue slots of the scalar forms)
+        f2 psum2 = {0.f, 0.f};                         // (two partial sums: shorter dependent chains)
         const f2 c2 = {s.c, s.c}, nm2 = {-m_new, -m_new};
         h8 pf[4];
 #pragma unroll

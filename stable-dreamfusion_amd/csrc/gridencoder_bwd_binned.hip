@@ -155,7 +155,7 @@ __device__ __forceinline__ float masked_shr(float v, uint32_t mask) {
     return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), 0x110 + N, 0xf, 0xf, true) & mask);
 }
 
-// one segmented-scan step on the two channels of a corner at once: two v_and_b32_dpp + one v_pk_add_f32
+// one segmented-scan step on the two channels of a corner at once: two v_and_b32_dpp + two v_add_f32
 __device__ __forceinline__ void fold_runs(const RunScan& r, float2_t& v) {
     { const float2_t u = {masked_shr<1>(v.x, r.take1), masked_shr<1>(v.y, r.take1)}; v = v + u; }
     { const float2_t u = {masked_shr<2>(v.x, r.take2), masked_shr<2>(v.y, r.take2)}; v = v + u; }
@@ -201,7 +201,7 @@ __device__ __forceinline__ void spill_add(unsigned long long* __restrict__ spill
 // Instruction issue bounds this kernel (round 2, PMC: 560 VALU + 276 SALU instructions per wave and level, 76 % of its time),
 // so it is written like the forward (gridencoder_fwd.hip): the grid's kind, interpolation and alignment are template
 // parameters, the level's constants sit in scalar registers, the 8 row indices share their hash / stride terms
-// (level_prepare), both channels of a corner travel as one float2 (v_pk_mul_f32, v_pk_add_f32, v_cvt_pk_f16_f32), the run
+// (level_prepare), both channels of a corner travel as one float2 (v_mul_f32, v_add_f32, v_cvt_pk_f16_f32), the run
 // folding is a workgroup-uniform template branch and nothing about a corner is decided by control flow.
 // the contributions of this lane's sample at one level: 8 table rows, 8 float2 values (folded over the lane run that ends here
 // when MERGE), and whether this lane emits them. Shared by K1 and by the spill kernel, which must reproduce K1's values bit for bit.
