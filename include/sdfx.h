@@ -578,6 +578,55 @@ int sdfx_add_bias_residual(const void* a, const void* b, const void* bias, uint3
 /* out[rows, n] = x[rows, :n] * gelu(x[rows, n:]) (exact erf GELU; the GEGLU of the UNet's feed-forward blocks), fp16, n % 8 == 0 */
 int sdfx_geglu(const void* x, uint64_t rows, uint32_t n, void* out, sdfx_stream_t stream);
 
+/* ---------------------------------------------------------------- attention with its gradient (extension) */
+
+/*
+ * Extension (no reference kernel) — o[B, Nq, H, D] (contiguous) = softmax(scale q k^T over the visible keys) v per (batch, head) and its gradient,
+ * which recomputes the probabilities from q, k and the saved log-sum-exp (csrc/attention_train.h). fp16, or bf16 with bf16 != 0; float32
+ * accumulation and statistics. H query heads share Hk key heads (H % Hk == 0): head h reads key head h / (H / Hk). D a multiple of 8 up to
+ * 256. q[b, h, n, :] is read at q + b strides[0] + n strides[1] + h strides[2] (elements, multiples of 8; unit channel stride; 16-byte
+ * aligned), k / v likewise over Nk keys. key_mask[B, Nk] bytes (may be NULL): 0 = no query sees the key, whatever its k and v hold.
+ * causal != 0: query i sees keys <= i + Nk - Nq. A row that sees no key: o = 0, lse = +inf, no gradient. scale > 0.
+ * forward: lse[B, H, Nq] (base-2 log-sum-exp of the scaled scores) and o_lo (what rounding o to 16 bits left, same type and layout) are what
+ *   the backward needs; both NULL without one.
+ * backward: dy[B, Nq, H, D] contiguous -> dq[B, Nq, H, D] (may be NULL), dk / dv[B, Nk, Hk, D] (NULL together).
+ * scratch: sdfx_attention_train_scratch_bytes(..., backward) bytes, 16-byte aligned, uninitialised (0: none needed). Results do not depend
+ * on the order in which workgroups run.
+ */
+uint64_t sdfx_attention_train_scratch_bytes(uint32_t B, uint32_t H, uint32_t Hk, uint32_t Nq, uint32_t Nk, uint32_t D, int backward);
+int sdfx_attention_train_forward(const void* q, const void* k, const void* v, const void* key_mask, uint32_t B, uint32_t H, uint32_t Hk, uint32_t Nq,
+                                 uint32_t Nk, uint32_t D, const uint64_t* q_strides, const uint64_t* k_strides, const uint64_t* v_strides, float scale,
+                                 int causal, int bf16, void* o, void* o_lo, float* lse, float* scratch, sdfx_stream_t stream);
+int sdfx_attention_train_backward(const void* q, const void* k, const void* v, const void* key_mask, const void* o, const void* o_lo, const float* lse,
+                                  const void* dy, uint32_t B, uint32_t H, uint32_t Hk, uint32_t Nq, uint32_t Nk, uint32_t D, const uint64_t* q_strides,
+                                  const uint64_t* k_strides, const uint64_t* v_strides, float scale, int causal, int bf16, void* dq, void* dk, void* dv,
+                                  float* scratch, sdfx_stream_t stream);
+
+/* ---------------------------------------------------------------- training a prior block: norm, GEGLU (extension) */
+
+/*
+ * Extension (no reference kernel) — the group norm above with every gradient, for blocks that train. dtype: 0 fp16, 1 bf16, 2 float32
+ * (x, pre, y, dy, dx, dpre); gamma / beta / dgamma / dbeta have that type, or float32 with params_f32 != 0. x[N, HW, C] is
+ * channels-last memory, C % 8 == 0, C <= 2560, G <= 64, C % G == 0; map pointers 16-byte aligned.
+ * forward: y = act(norm(x + pre) * gamma + beta); mean_rstd[N, G, 2] and, when saved8 is not NULL (C % 32 == 0), the 8-bit form of x:
+ *   N HW C code bytes, then N HW C / 32 scale bytes (block of 32 channels: step 2^(scale - 127), scale 255 = the block holds an
+ *   infinity or a NaN and decodes as NaN). pre[N, C] may be NULL.
+ * backward: x is the forward's x, or its saved8 with eight_bits != 0. dx / dpre / dgamma / dbeta may each be NULL. With the 8-bit input the
+ *   derivative is evaluated at the decoded x with the forward's statistics.
+ * scratch: sdfx_group_norm_train_scratch_bytes(N, HW, C, G) bytes, 8-byte aligned, uninitialised (0: the shape is not taken).
+ */
+uint64_t sdfx_group_norm_train_scratch_bytes(uint32_t N, uint32_t HW, uint32_t C, uint32_t G);
+int sdfx_group_norm_train_forward(const void* x, const void* pre, const void* gamma, const void* beta, uint32_t N, uint32_t HW, uint32_t C, uint32_t G,
+                                  float eps, int silu, int dtype, int params_f32, void* y, void* saved8, float* mean_rstd, float* scratch,
+                                  sdfx_stream_t stream);
+int sdfx_group_norm_train_backward(const void* x, int eight_bits, const void* pre, const void* dy, const void* gamma, const void* beta,
+                                   const float* mean_rstd, uint32_t N, uint32_t HW, uint32_t C, uint32_t G, int silu, int dtype, int params_f32, void* dx,
+                                   void* dpre, void* dgamma, void* dbeta, float* scratch, sdfx_stream_t stream);
+/* y[rows, n] = x[rows, :n] * gelu(x[rows, n:]) with its gradient; dtype as above, n % 8 == 0; saved8 (n % 32 == 0, may be NULL): the 8-bit
+ * form of x[rows, 2 n], laid out as above. backward: x, or saved8 with eight_bits != 0. */
+int sdfx_geglu_train_forward(const void* x, uint64_t rows, uint32_t n, int dtype, void* y, void* saved8, sdfx_stream_t stream);
+int sdfx_geglu_train_backward(const void* x, int eight_bits, const void* dy, uint64_t rows, uint32_t n, int dtype, void* dx, sdfx_stream_t stream);
+
 /* ---------------------------------------------------------------- frozen prior: 3 x 3 convolutions on the matrix cores (extension) */
 
 /*

@@ -6,6 +6,7 @@ nothing in the shipped path routes around the HIP kernels.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 
@@ -108,7 +109,16 @@ _SIGNATURES = {
     "sdfx_group_norm_backward": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _u32, _u32, _u32, _u32, _int, _ptr, _ptr, _ptr],
     "sdfx_add_bias_residual": [_ptr, _ptr, _ptr, _u32, _u32, _u32, _ptr, _ptr],
     "sdfx_geglu": [_ptr, _u64, _u32, _ptr, _ptr],
+    "sdfx_group_norm_train_scratch_bytes": [_u32, _u32, _u32, _u32],
+    "sdfx_group_norm_train_forward": [_ptr, _ptr, _ptr, _ptr, _u32, _u32, _u32, _u32, _f32, _int, _int, _int, _ptr, _ptr, _ptr, _ptr, _ptr],
+    "sdfx_group_norm_train_backward": [_ptr, _int, _ptr, _ptr, _ptr, _ptr, _ptr, _u32, _u32, _u32, _u32, _int, _int, _int, _ptr, _ptr, _ptr, _ptr,
+                                       _ptr, _ptr],
+    "sdfx_geglu_train_forward": [_ptr, _u64, _u32, _int, _ptr, _ptr, _ptr],
+    "sdfx_geglu_train_backward": [_ptr, _int, _ptr, _u64, _u32, _int, _ptr, _ptr],
     "sdfx_attention_forward": [_ptr, _ptr, _ptr, _u32, _u32, _u32, _u32, _u32, _ptr, _ptr, _ptr, _f32, _int, _ptr, _ptr],
+    "sdfx_attention_train_scratch_bytes": [_u32, _u32, _u32, _u32, _u32, _u32, _int],
+    "sdfx_attention_train_forward": [_ptr] * 4 + [_u32] * 6 + [_ptr] * 3 + [_f32, _int, _int] + [_ptr] * 5,
+    "sdfx_attention_train_backward": [_ptr] * 8 + [_u32] * 6 + [_ptr] * 3 + [_f32, _int, _int] + [_ptr] * 5,
     "sdfx_conv3x3_packed_ok": [_u32, _u32, _u32, _u32, _u32, _u32],
     "sdfx_conv3x3_packed_scratch_bytes": [_u32, _u32, _u32, _u32, _u32, _u32, _int],
     "sdfx_conv3x3_pack_weights": [_ptr, _u32, _u32, _ptr, _ptr],
@@ -134,6 +144,8 @@ _RESTYPES = {
     "sdfx_field_packed_words": _u32,
     "sdfx_field_backward_scratch_bytes": _u64,
     "sdfx_group_norm_scratch_bytes": _u64,
+    "sdfx_group_norm_train_scratch_bytes": _u64,
+    "sdfx_attention_train_scratch_bytes": _u64,
     "sdfx_conv3x3_scratch_bytes": _u64,
     "sdfx_linear_scratch_bytes": _u64,
     "sdfx_conv3x3_packed_scratch_bytes": _u64,
@@ -268,6 +280,11 @@ def check(rc: int) -> None:
 def stream() -> C.c_void_p:
     """hipStream_t of torch's current stream on the current device."""
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def on_device(t):
+    """A context in which the device of `t` is the current one (and stream() its current stream)."""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def ptr(t) -> C.c_void_p | None:

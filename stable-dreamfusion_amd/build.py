@@ -24,7 +24,7 @@ INCLUDE = os.path.normpath(os.path.join(HERE, "..", "include"))
 DEVTOOLS_KERNELS = os.path.normpath(os.path.join(HERE, "..", "tools", "devtools_kernels"))
 LIB = os.path.join(CSRC, "libsdfx_hip.so")
 DEV_LIB = os.path.join(CSRC, "libsdfx_hip_dev.so")
-SOURCES = ["sdfx_core.hip", "raymarching.hip", "gridencoder.hip", "gridencoder_fwd.hip", "gridencoder_bwd_binned.hip", "encoders.hip", "field.hip", "optim.hip", "shade.hip", "render.hip", "occupancy.hip", "infer.hip", "head.hip", "sds.hip", "dmtet.hip", "raster.hip", "groupnorm.hip", "conv.hip", "attention.hip"]
+SOURCES = ["sdfx_core.hip", "raymarching.hip", "gridencoder.hip", "gridencoder_fwd.hip", "gridencoder_bwd_binned.hip", "encoders.hip", "field.hip", "optim.hip", "shade.hip", "render.hip", "occupancy.hip", "infer.hip", "head.hip", "sds.hip", "dmtet.hip", "raster.hip", "groupnorm.hip", "groupnorm_train.hip", "geglu_train.hip", "conv.hip", "attention.hip", "attention_train.hip", "attention_train_dq.hip", "attention_train_dkdv.hip"]
 ARCH = "gfx950"
 # -ffp-contract=off: the march / encode arithmetic must not gain FMAs the source does not spell
 # out (bit-exact ray counts and fp32 features against the CPU oracle).

@@ -1,0 +1,254 @@
+// attention_train.h — what the attention kernels with a gradient share: shapes, matrix-core fragments, tiles in LDS.
+//   s = scale q k^T, p = softmax(s over the visible keys), o = p v;   delta = sum(do o), dp = do v^T, ds = p (dp - delta),
+//   dq = scale ds k, dk = scale ds^T q, dv = p^T do
+// (attention_train.hip: forward, joins, entry points; attention_train_dq.hip; attention_train_dkdv.hip)
+//
+// Every product runs transposed on v_mfma_f32_32x32x16 so that a lane owns one row of the softmax (forward, dq) or one key (dk / dv): the
+// D fragment of lane (x = lane & 31, hi = lane >> 5) holds, in element r, row (r & 3) + 8 (r >> 2) + 4 hi of column x. Packed to 16 bits
+// its elements 8 e .. 8 e + 7 are the B operand of K step e when the A operand takes its 16 rows in that same order, which two
+// ds_read_b64_tr_b16 of a row-major tile deliver: probabilities never pass through LDS and no tile is stored transposed.
+#pragma once
+
+#include "sdfx_common.h"
+
+namespace sdfx_attn {
+
+using namespace sdfx;
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef short s8 __attribute__((ext_vector_type(8)));
+typedef unsigned u2v __attribute__((ext_vector_type(2)));
+typedef unsigned u4v __attribute__((ext_vector_type(4)));   // (native vectors: arrays of HIP's uint4 struct end up in scratch)
+
+struct Shape {
+    uint32_t B, H, Hk, Nq, Nk, D;
+    uint32_t group, rows;                 // query heads per key head; rows of one key head: group * Nq, row R = (head in group) * Nq + query
+    uint64_t q_sb, q_sn, q_sh, k_sb, k_sn, k_sh, v_sb, v_sn, v_sh;   // element strides (the channel stride is 1)
+    const uint8_t* mask;                  // [B, Nk], 0 = the key is not seen; or null
+    int causal, off;                      // query i sees keys <= i + off (off = Nk - Nq)
+    float scale, c;                       // softmax scale; times log2(e)
+    uint32_t tiles_x;                     // workgroups along rows (forward, dq) or keys (dk / dv)
+    uint32_t splits, per_split;           // the other axis: workgroups, tiles for each
+};
+
+template <typename T> struct Half;
+template <> struct Half<_Float16> {
+    typedef h8 v8; typedef h4 v4; typedef h2 v2;
+    // Probabilities of a long flat row lie under fp16's normal range (2^-14), ds further down. The backward forms p * 2^15 and
+    // ds * (2^15 g), g from the largest |do| |v| (see grad_scale): both in range, the power of two taken out of the float32 sums.
+    static constexpr float kShift = 15.f;
+    static constexpr bool kScaled = true;
+};
+template <> struct Half<__bf16> {
+    typedef b8 v8; typedef b4 v4; typedef b2 v2;
+    static constexpr float kShift = 0.f;
+    static constexpr bool kScaled = false;
+};
+__device__ __forceinline__ f32x16 mma(h8 a, h8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mma(b8 a, b8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+
+__device__ __forceinline__ float max_halves(float x) {      // over lanes l and l ^ 32
+    const uint32_t u = __float_as_uint(x);
+    const u2v r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t a = r.x, b = r.y;
+    return fmaxf(__uint_as_float(a), __uint_as_float(b));
+}
+__device__ __forceinline__ float sum_halves(float x) {
+    const uint32_t u = __float_as_uint(x);
+    const u2v r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t a = r.x, b = r.y;
+    return __uint_as_float(a) + __uint_as_float(b);
+}
+__device__ __forceinline__ f32x16 zero16() {
+    f32x16 z;
+#pragma unroll
+    for (int r = 0; r < 16; r++) z[r] = 0.f;
+    return z;
+}
+// elements 8 e .. 8 e + 7 of a D fragment as the B operand of K step e
+template <typename T> __device__ __forceinline__ typename Half<T>::v8 operand(const f32x16& p, int e) {
+    typename Half<T>::v8 v;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const typename Half<T>::v2 h = __builtin_convertvector(f2{p[8 * e + 2 * j], p[8 * e + 2 * j + 1]}, typename Half<T>::v2);
+        v[2 * j] = h[0]; v[2 * j + 1] = h[1];
+    }
+    return v;
+}
+
+// ---- tiles of ROWS rows in LDS, row-major, an odd number of 16-byte chunks a row (16 rows of a ds_read_b128 start in 16 bank quads) ----
+template <int DP, int ROWS, int TH> struct Tile {
+    static constexpr int CH = DP / 8;
+    static constexpr uint32_t PITCH = (uint32_t)(CH | 1) * 16u;
+    static constexpr uint32_t BYTES = (uint32_t)ROWS * PITCH;
+    static constexpr int NCH = ROWS * CH;
+    static constexpr int PT = (NCH + TH - 1) / TH;           // chunks per thread
+};
+// Channel blocks are 32 wide: the transposed reads of the last block of a row whose width is no multiple of 32 run up to 32 channels past
+// it (their results are rows of the product that nothing stores): bytes to have behind the last tile.
+constexpr uint32_t kTileSlack = 64;
+
+// rows base .. base + ROWS - 1 (clamped to n - 1) into registers; channels from D on are zero
+template <typename L> __device__ __forceinline__ void request(u4v (&r)[L::PT], const void* p, uint64_t sn, uint32_t base, uint32_t n, uint32_t D, uint32_t tid, uint32_t th) {
+#pragma unroll
+    for (int i = 0; i < L::PT; i++) {
+        const uint32_t c = min(tid + (uint32_t)i * th, (uint32_t)L::NCH - 1u);        // (threads past the tile repeat its last chunk)
+        const uint32_t row = c / L::CH, ch = c - row * L::CH;
+        const uint32_t at = min(base + row, n - 1u);
+        r[i] = u4v{0u, 0u, 0u, 0u};
+        if (ch * 8u < D) r[i] = *reinterpret_cast<const u4v*>(static_cast<const uint16_t*>(p) + (size_t)at * sn + ch * 8u);
+    }
+}
+// ... and into LDS; rows whose bit of `live` is clear as zeros (a masked key's values may be anything: 0 * NaN must not reach a product)
+template <typename L> __device__ __forceinline__ void stash(uint8_t* tile, const u4v (&r)[L::PT], uint64_t live, uint32_t tid, uint32_t th) {
+#pragma unroll
+    for (int i = 0; i < L::PT; i++) {
+        const uint32_t c = tid + (uint32_t)i * th;
+        if (c < (uint32_t)L::NCH) {
+            const uint32_t row = c / L::CH, ch = c - row * L::CH;
+            const bool on = (live >> row) & 1u;
+            *reinterpret_cast<u4v*>(tile + row * L::PITCH + ch * 16u) = on ? r[i] : u4v{0u, 0u, 0u, 0u};
+        }
+    }
+}
+// A operand, rows of the tile: lane (x, hi) row 32 blk + x, channels 16 ks + 8 hi .. + 7
+template <typename T, typename L> __device__ __forceinline__ typename Half<T>::v8 row_operand(const uint8_t* tile, uint32_t blk, uint32_t ks, uint32_t x, uint32_t hi) {
+    return *reinterpret_cast<const typename Half<T>::v8*>(tile + (32u * blk + x) * L::PITCH + ks * 32u + hi * 16u);
+}
+// A operand, the tile transposed: lane (x, hi) channel 32 dt + x; its 8 elements are rows 16 e + 4 hi + {0..3, 8..11}
+typedef s4 __attribute__((address_space(3)))* lds_s4;
+template <typename T, typename L> __device__ __forceinline__ typename Half<T>::v8 col_operand(const uint8_t* tile, uint32_t e, uint32_t dt, uint32_t lane) {
+    const uint32_t l16 = lane & 15u, cb = (lane >> 4) & 1u, hi = lane >> 5;
+    const uint8_t* p = tile + (16u * e + 4u * hi + (l16 >> 2)) * L::PITCH + (32u * dt + 16u * cb + 4u * (l16 & 3u)) * 2u;
+    const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p));
+    const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + 8u * L::PITCH));
+    const s8 v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(typename Half<T>::v8, v);
+}
+// B operand straight from memory: lane (x, hi) row `p`, channels 16 ks + 8 hi .. + 7, zero from D on
+template <typename T, int KS> __device__ __forceinline__ void row_fragments(typename Half<T>::v8 (&f)[KS], const void* p, uint32_t D, uint32_t hi) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) {
+        const uint32_t c0 = 16u * ks + 8u * hi;
+        u4v w = u4v{0u, 0u, 0u, 0u};
+        if (c0 < D) w = *reinterpret_cast<const u4v*>(static_cast<const uint16_t*>(p) + c0);
+        f[ks] = __builtin_bit_cast(typename Half<T>::v8, w);
+    }
+}
+// four consecutive channels
+template <typename T> __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
+    const typename Half<T>::v2 x = __builtin_convertvector(f2{a, b}, typename Half<T>::v2), y = __builtin_convertvector(f2{c, d}, typename Half<T>::v2);
+    *reinterpret_cast<typename Half<T>::v4*>(p) = typename Half<T>::v4{x[0], x[1], y[0], y[1]};
+}
+
+// ---- the power of two the fp16 backward scales ds by -------------------------------------------------------------------------------
+// |dp - delta| <= 2 M, M = max |do row| max |v row| over the key head's rows (attention_train.hip: k_prep leaves the squares of
+// block maxima): g = 2^-k with 2 M g <= 1, so |2^15 p g (dp - delta)| <= 2^15 whatever the loss scale, and gradients down to 2^-29 of
+// that bound are normal numbers.
+__device__ __forceinline__ float grad_scale(const float* rows2, uint32_t nr, const float* v2, uint32_t nv, uint32_t lane) {
+    float a = 0.f, b = 0.f;
+    for (uint32_t i = lane; i < nr; i += 64) a = fmaxf(a, rows2[i]);
+    for (uint32_t i = lane; i < nv; i += 64) b = fmaxf(b, v2[i]);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) { a = fmaxf(a, __shfl_xor(a, o, 64)); b = fmaxf(b, __shfl_xor(b, o, 64)); }
+    const float m = sqrtf(a) * sqrtf(b);
+    if (!(m > 0.f) || m > 1e37f) return 1.f;
+    const uint32_t e = __float_as_uint(m) >> 23;
+    return __uint_as_float((252u - min(e, 251u)) << 23);
+}
+constexpr uint32_t kPrepRows = 64;         // rows per workgroup of k_prep = rows per entry of the maxima
+__host__ __device__ inline uint32_t prep_blocks(uint32_t n) { return (n + kPrepRows - 1) / kPrepRows; }
+
+// what the backward's kernels get beside the shape
+struct BwdArgs {
+    const void *q, *k, *v, *dy;
+    const float *lse, *delta, *rows2, *v2;
+    void *dq, *dk, *dv;                    // T [B, Nq, H, D], [B, Nk, Hk, D] (or null: not wanted)
+    float *part, *part2;                   // splits > 1: float32 [splits][B Hk][rows or Nk][D] of dq, or of dk and dv
+};
+constexpr int kWidths[] = {48, 64, 80, 128, 160, 256};      // channels a kernel is built for; a head takes the next of them
+
+// attention_train_dq.hip, attention_train_dkdv.hip: launch (shape's tiles_x / splits / per_split set for `waves` a workgroup)
+void launch_dq(const BwdArgs& a, const Shape& s, int bf16, int waves, hipStream_t st);
+void launch_dkdv(const BwdArgs& a, const Shape& s, int bf16, int waves, hipStream_t st);
+// rows of the tile each stages: keys (forward, dq) or queries (dk / dv)
+constexpr int key_tile(int dp) { return dp <= 128 ? 64 : 32; }
+constexpr int query_tile(int dp) { return dp <= 80 ? 64 : 32; }
+inline int padded(uint32_t D) {
+    for (int w : kWidths)
+        if (D <= (uint32_t)w) return w;
+    return 0;
+}
+
+#define SDFX_ATTN_WIDTH(fn, T, nw, ...)                                   \
+    do {                                                                  \
+        switch (padded(s.D)) {                                            \
+            case 48: fn<T, 48, nw>(__VA_ARGS__); break;                   \
+            case 64: fn<T, 64, nw>(__VA_ARGS__); break;                   \
+            case 80: fn<T, 80, nw>(__VA_ARGS__); break;                   \
+            case 128: fn<T, 128, nw>(__VA_ARGS__); break;                 \
+            case 160: fn<T, 160, nw>(__VA_ARGS__); break;                 \
+            default: fn<T, 256, nw>(__VA_ARGS__); break;                  \
+        }                                                                 \
+    } while (0)
+#define SDFX_ATTN_DISPATCH(fn, ...)                                       \
+    do {                                                                  \
+        if (bf16 && waves == 4) SDFX_ATTN_WIDTH(fn, __bf16, 4, __VA_ARGS__);        \
+        else if (bf16) SDFX_ATTN_WIDTH(fn, __bf16, 1, __VA_ARGS__);                 \
+        else if (waves == 4) SDFX_ATTN_WIDTH(fn, _Float16, 4, __VA_ARGS__);         \
+        else SDFX_ATTN_WIDTH(fn, _Float16, 1, __VA_ARGS__);                         \
+    } while (0)
+
+// the row a lane owns in the forward and in dq
+struct Row {
+    uint32_t R, head, qi;                  // row of the key head (clamped), query head, query
+    bool on;
+    int lim;                               // last key a causal row sees (may be negative)
+};
+__device__ __forceinline__ Row row_of(const Shape& s, uint32_t r, uint32_t hk) {
+    Row w;
+    w.on = r < s.rows;
+    w.R = min(r, s.rows - 1u);
+    const uint32_t g = w.R / s.Nq;
+    w.qi = w.R - g * s.Nq;
+    w.head = hk * s.group + g;
+    w.lim = s.causal ? (int)w.qi + s.off : 0x7fffffff;
+    return w;
+}
+// smallest and largest query among rows a .. b (rows of several heads: all queries)
+__device__ __forceinline__ void query_range(const Shape& s, uint32_t a, uint32_t b, uint32_t& lo, uint32_t& hi) {
+    const uint32_t ga = a / s.Nq, gb = b / s.Nq;
+    lo = ga == gb ? a - ga * s.Nq : 0u;
+    hi = ga == gb ? b - ga * s.Nq : s.Nq - 1u;
+}
+// Keys of a tile that exist and are not masked, one bit each (the same in every wave). The byte is loaded early, the ballot taken later.
+template <int KT> __device__ __forceinline__ uint8_t mask_byte(const Shape& s, uint32_t b, uint32_t tile, uint32_t lane) {
+    const uint32_t key = tile * KT + lane;
+    if (!s.mask) return 1;
+    return s.mask[(size_t)b * s.Nk + min(key, s.Nk - 1u)];
+}
+template <int KT> __device__ __forceinline__ uint64_t live_keys(const Shape& s, uint8_t byte, uint32_t tile, uint32_t lane) {
+    return __ballot(lane < (uint32_t)KT && tile * KT + lane < s.Nk && byte != 0);
+}
+template <int KT> constexpr uint64_t all_keys() { return KT == 64 ? ~0ull : ((1ull << (KT & 63)) - 1ull); }
+// -inf where the lane's row does not see the key: D element r of block st is key 32 st + (r & 3) + 8 (r >> 2) + 4 hi of the tile
+__device__ __forceinline__ void hide(f32x16& sc, uint64_t live, int lim, uint32_t tile0, int st, uint32_t hi) {
+    const uint32_t bits = (uint32_t)(live >> (32 * st)) >> (4 * hi);
+    const int last = lim - (int)(tile0 + 32u * st + 4u * hi);
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+        const int k = (r & 3) + 8 * (r >> 2);
+        if (!((bits >> k) & 1u) || k > last) sc[r] = -INFINITY;
+    }
+}
+
+}  // namespace sdfx_attn

@@ -1,0 +1,436 @@
+// attention_train.hip — softmax attention that keeps what its gradient needs: the forward (one pass over the keys with the running
+// maximum and sum), the small kernels around the gradient's two, the joins of split axes, and the entry points. See attention_train.h.
+#include "attention_train.h"
+
+using namespace sdfx_attn;
+
+namespace {
+
+// ---- forward ----------------------------------------------------------------------------------------------------------------------
+// A wave owns 32 rows (of the query heads that share a key head), a workgroup of NW waves shares the key / value tiles, double-buffered
+// in LDS with the loads of tile j + 1 in flight while tile j is used. splits > 1 (few rows, a long key axis): a workgroup takes a range of
+// the tiles and leaves its unnormalised output, maximum and sum for k_join_o.
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_fwd(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
+                                                   T* __restrict__ o, T* __restrict__ o_lo, float* __restrict__ lse, float* __restrict__ part,
+                                                   float* __restrict__ part_ml, Shape s) {
+    constexpr int KT = key_tile(DP), KS = DP / 16, DT = (DP + 31) / 32, NB = KT / 32;
+    typedef Tile<DP, KT, 64 * NW> L;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[4 * L::BYTES + kTileSlack];
+    uint8_t* const ldsK = lds;
+    uint8_t* const ldsV = lds + 2 * L::BYTES;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, x = lane & 31u, hi = lane >> 5;
+    const uint32_t per_bh = s.tiles_x * s.splits;
+    const uint32_t lid = xcd_contiguous(blockIdx.x, per_bh * s.B * s.Hk);
+    const uint32_t bh = lid / per_bh, rest = lid - bh * per_bh, split = rest / s.tiles_x, xt = rest - split * s.tiles_x;
+    const uint32_t b = bh / s.Hk, hk = bh - b * s.Hk;
+    const uint32_t r0 = xt * NW * 32u, w0 = r0 + wave * 32u;
+    const Row row = row_of(s, w0 + x, hk);
+    const T* kb = k + (size_t)b * s.k_sb + (size_t)hk * s.k_sh;
+    const T* vb = v + (size_t)b * s.v_sb + (size_t)hk * s.v_sh;
+
+    typename Half<T>::v8 qf[KS];
+    row_fragments<T, KS>(qf, q + (size_t)b * s.q_sb + (size_t)row.qi * s.q_sn + (size_t)row.head * s.q_sh, s.D, hi);
+
+    // keys this workgroup needs, and the causal bounds of this wave's rows
+    uint32_t kend = s.Nk;
+    int wave_lo = 0x7fffffff, wave_hi = 0x7fffffff;
+    if (s.causal) {
+        uint32_t lo, hi_q;
+        query_range(s, r0, min(r0 + NW * 32u, s.rows) - 1u, lo, hi_q);
+        kend = (uint32_t)max(0, min((int)s.Nk, (int)hi_q + s.off + 1));
+        query_range(s, min(w0, s.rows - 1u), min(w0 + 32u, s.rows) - 1u, lo, hi_q);
+        wave_lo = (int)lo + s.off; wave_hi = (int)hi_q + s.off;
+    }
+    const uint32_t t0 = split * s.per_split, t1 = min(t0 + s.per_split, (kend + KT - 1) / KT);
+
+    f32x16 acc[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++) acc[dt] = zero16();
+    float m_run = -1e30f, l_run = 0.f;
+    if (t0 < t1) {
+        u4v rk[L::PT], rv[L::PT];
+        request<L>(rk, kb, s.k_sn, t0 * KT, s.Nk, s.D, tid, 64 * NW);
+        request<L>(rv, vb, s.v_sn, t0 * KT, s.Nk, s.D, tid, 64 * NW);
+        uint64_t live = live_keys<KT>(s, mask_byte<KT>(s, b, t0, lane), t0, lane);
+        stash<L>(ldsK, rk, live, tid, 64 * NW);
+        stash<L>(ldsV, rv, live, tid, 64 * NW);
+        __syncthreads();
+        for (uint32_t j = t0; j < t1; j++) {
+            const uint32_t buf = (j - t0) & 1u;
+            uint8_t next_byte = 0;
+            if (j + 1 < t1) {
+                request<L>(rk, kb, s.k_sn, (j + 1) * KT, s.Nk, s.D, tid, 64 * NW);
+                request<L>(rv, vb, s.v_sn, (j + 1) * KT, s.Nk, s.D, tid, 64 * NW);
+                next_byte = mask_byte<KT>(s, b, j + 1, lane);
+            }
+            const uint8_t* kt = ldsK + buf * L::BYTES;
+            const uint8_t* vt = ldsV + buf * L::BYTES;
+            if (live != 0 && (int)(j * KT) <= wave_hi) {
+                f32x16 sc[NB];
+#pragma unroll
+                for (int st = 0; st < NB; st++) {
+                    sc[st] = zero16();
+#pragma unroll
+                    for (int ks = 0; ks < KS; ks++) sc[st] = mma(row_operand<T, L>(kt, st, ks, x, hi), qf[ks], sc[st]);
+                }
+                if (live != all_keys<KT>() || (int)(j * KT + KT - 1) > wave_lo) {
+#pragma unroll
+                    for (int st = 0; st < NB; st++) hide(sc[st], live, row.lim, j * KT, st, hi);
+                }
+                float mx = -INFINITY;
+#pragma unroll
+                for (int st = 0; st < NB; st++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) mx = fmaxf(mx, sc[st][r]);
+                mx = max_halves(mx);
+                const float m_new = fmaxf(m_run, mx * s.c);
+                const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+                m_run = m_new;
+                float sum0 = 0.f, sum1 = 0.f;
+                typename Half<T>::v8 pf[2 * NB];
+#pragma unroll
+                for (int st = 0; st < NB; st++) {
+#pragma unroll
+                    for (int r = 0; r < 16; r += 2) {
+                        sc[st][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[st][r], s.c, -m_new));
+                        sc[st][r + 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[st][r + 1], s.c, -m_new));
+                        sum0 += sc[st][r]; sum1 += sc[st][r + 1];
+                    }
+                    pf[2 * st] = operand<T>(sc[st], 0);          // (the probabilities' rounding: half a unit of each, as the inputs')
+                    pf[2 * st + 1] = operand<T>(sc[st], 1);
+                }
+                l_run = __builtin_fmaf(l_run, alpha, sum0 + sum1);
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) acc[dt][r] *= alpha;
+#pragma unroll
+                for (int e = 0; e < 2 * NB; e++)
+#pragma unroll
+                    for (int dt = 0; dt < DT; dt++) acc[dt] = mma(col_operand<T, L>(vt, e, dt, lane), pf[e], acc[dt]);
+            }
+            if (j + 1 < t1) {
+                live = live_keys<KT>(s, next_byte, j + 1, lane);
+                stash<L>(ldsK + (buf ^ 1u) * L::BYTES, rk, live, tid, 64 * NW);
+                stash<L>(ldsV + (buf ^ 1u) * L::BYTES, rv, live, tid, 64 * NW);
+            }
+            __syncthreads();
+        }
+    }
+    const float l = sum_halves(l_run);
+    if (!row.on) return;
+    const size_t at = (size_t)bh * s.rows + row.R;                 // = (b, head, query) of [B, H, Nq]
+    if (s.splits > 1) {
+        const size_t pa = (size_t)split * s.B * s.Hk * s.rows + at;
+        if (hi == 0) { part_ml[2 * pa] = m_run; part_ml[2 * pa + 1] = l; }
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const uint32_t c0 = 32u * dt + 8u * g + 4u * hi;
+                if (c0 < s.D) *reinterpret_cast<f4*>(part + pa * s.D + c0) = f4{acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]};
+            }
+        return;
+    }
+    // a row that sees nothing: zero, and a log-sum-exp of +inf, at which the backward's exp2(s - lse) is 0
+    const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+    if (lse && hi == 0) lse[at] = l > 0.f ? m_run + __builtin_amdgcn_logf(l) : (l == l ? INFINITY : l);
+    T* op = o + (((size_t)b * s.Nq + row.qi) * s.H + row.head) * s.D;
+    T* lp = o_lo ? o_lo + (((size_t)b * s.Nq + row.qi) * s.H + row.head) * s.D : nullptr;
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const uint32_t c0 = 32u * dt + 8u * g + 4u * hi;
+            if (c0 < s.D) {
+                float f[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) f[i] = acc[dt][4 * g + i] * inv;
+                store4(op + c0, f[0], f[1], f[2], f[3]);
+                if (lp) store4(lp + c0, f[0] - (float)(T)f[0], f[1] - (float)(T)f[1], f[2] - (float)(T)f[2], f[3] - (float)(T)f[3]);
+            }
+        }
+}
+
+// o of the splits of each row: thread per (row, 4 channels)
+template <typename T>
+__global__ __launch_bounds__(256) void k_join_o(const float* __restrict__ part, const float* __restrict__ ml, Shape s, T* __restrict__ o,
+                                               T* __restrict__ o_lo, float* __restrict__ lse) {
+    const uint32_t per = s.D / 4;
+    const uint64_t total = (uint64_t)s.B * s.H * s.Nq;
+    const uint64_t id = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    if (id >= total * per) return;
+    const uint64_t r = id / per;
+    const uint32_t c0 = (uint32_t)(id - r * per) * 4;
+    float m = -1e30f;
+    for (uint32_t i = 0; i < s.splits; i++) m = fmaxf(m, ml[2 * (i * total + r)]);
+    float l = 0.f;
+    f4 a = {0.f, 0.f, 0.f, 0.f};
+    for (uint32_t i = 0; i < s.splits; i++) {
+        const uint64_t at = i * total + r;
+        const float li = ml[2 * at + 1];
+        if (li == 0.f) continue;                      // nothing seen in this range
+        const float w = __builtin_amdgcn_exp2f(ml[2 * at] - m);
+        const f4 p = *reinterpret_cast<const f4*>(part + at * s.D + c0);
+        l = __builtin_fmaf(w, li, l);
+#pragma unroll
+        for (int j = 0; j < 4; j++) a[j] = __builtin_fmaf(w, p[j], a[j]);
+    }
+    const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+    const uint32_t bh = (uint32_t)(r / s.Nq), qi = (uint32_t)(r - (uint64_t)bh * s.Nq), b = bh / s.H, h = bh - b * s.H;
+    const size_t at = (((size_t)b * s.Nq + qi) * s.H + h) * s.D + c0;
+    if (lse && c0 == 0) lse[r] = l > 0.f ? m + __builtin_amdgcn_logf(l) : (l == l ? INFINITY : l);
+    a = a * inv;
+    store4(o + at, a[0], a[1], a[2], a[3]);
+    if (o_lo) store4(o_lo + at, a[0] - (float)(T)a[0], a[1] - (float)(T)a[1], a[2] - (float)(T)a[2], a[3] - (float)(T)a[3]);
+}
+
+// out[b, n, h, :] = sum over splits of part[split][b, h, n, :], in order (gridDim.y: a second pair)
+template <typename T>
+__global__ __launch_bounds__(256) void k_join_sum(const float* __restrict__ pa, const float* __restrict__ pb, uint32_t splits, uint32_t B, uint32_t H,
+                                                 uint32_t N, uint32_t D, T* __restrict__ oa, T* __restrict__ ob) {
+    const float* part = blockIdx.y ? pb : pa;
+    T* out = blockIdx.y ? ob : oa;
+    const uint32_t per = D / 4;
+    const uint64_t total = (uint64_t)B * H * N, id = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    if (id >= total * per) return;
+    const uint64_t r = id / per;
+    const uint32_t c0 = (uint32_t)(id - r * per) * 4;
+    f4 a = {0.f, 0.f, 0.f, 0.f};
+    for (uint32_t i = 0; i < splits; i++) a += *reinterpret_cast<const f4*>(part + (i * total + r) * D + c0);
+    const uint32_t bh = (uint32_t)(r / N), n = (uint32_t)(r - (uint64_t)bh * N), b = bh / H, h = bh - b * H;
+    store4(out + (((size_t)b * N + n) * H + h) * D + c0, a[0], a[1], a[2], a[3]);
+}
+
+// ---- ahead of the gradient's kernels ---------------------------------------------------------------------------------------------
+// delta[b, h, i] = sum over channels of dy (o + o_lo): o_lo is what rounding o to 16 bits left, without which ds = p (dp - delta) of a
+// peaked row loses the digits the subtraction cancels (bf16, scores with a deviation of 4: dq 5.8e-3 off instead of 2.4e-3). Also the
+// block maxima of |dy row|^2 and |v row|^2 that grad_scale reads (fp16). LR lanes a row.
+template <typename T, int LR>
+__global__ __launch_bounds__(256) void k_prep(const T* __restrict__ v, const T* __restrict__ o, const T* __restrict__ o_lo, const T* __restrict__ dy,
+                                             const float* __restrict__ lse, Shape s, float* __restrict__ delta, float* __restrict__ rows2, float* __restrict__ v2) {
+    __shared__ float red[256 / LR];
+    const uint32_t nr = prep_blocks(s.rows), nv = prep_blocks(s.Nk), bh_n = s.B * s.Hk;
+    const bool of_v = blockIdx.x >= bh_n * nr;
+    const uint32_t id = of_v ? blockIdx.x - bh_n * nr : blockIdx.x, per = of_v ? nv : nr;
+    const uint32_t bh = id / per, blk = id - bh * per, b = bh / s.Hk, hk = bh - b * s.Hk;
+    const uint32_t lr = threadIdx.x % LR, c0 = lr * 8u;
+    const uint32_t n = of_v ? s.Nk : s.rows, end = min((blk + 1) * kPrepRows, n);
+    float most = 0.f;
+    for (uint32_t r = blk * kPrepRows + threadIdx.x / LR; r < end; r += 256 / LR) {
+        float d = 0.f, q = 0.f;
+        size_t at = 0;
+        if (of_v) {
+            if ((!s.mask || s.mask[(size_t)b * s.Nk + r]) && c0 < s.D) {
+                const typename Half<T>::v8 a = *reinterpret_cast<const typename Half<T>::v8*>(v + (size_t)b * s.v_sb + (size_t)r * s.v_sn + (size_t)hk * s.v_sh + c0);
+#pragma unroll
+                for (int i = 0; i < 8; i++) q = __builtin_fmaf((float)a[i], (float)a[i], q);
+            }
+        } else {
+            const uint32_t g = r / s.Nq, qi = r - g * s.Nq;
+            at = (((size_t)b * s.Nq + qi) * s.H + hk * s.group + g) * s.D + c0;
+            if (c0 < s.D && lse[(size_t)bh * s.rows + r] != INFINITY) {          // (the dy of a row that sees nothing may be anything)
+                const typename Half<T>::v8 y = *reinterpret_cast<const typename Half<T>::v8*>(dy + at), a = *reinterpret_cast<const typename Half<T>::v8*>(o + at),
+                                           l = *reinterpret_cast<const typename Half<T>::v8*>(o_lo + at);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float f = (float)y[i];
+                    d = __builtin_fmaf(f, (float)a[i] + (float)l[i], d);
+                    q = __builtin_fmaf(f, f, q);
+                }
+            }
+        }
+#pragma unroll
+        for (int w = LR / 2; w >= 1; w >>= 1) { d += __shfl_xor(d, w, 64); q += __shfl_xor(q, w, 64); }
+        if (!of_v && lr == 0) delta[(size_t)bh * s.rows + r] = d;
+        most = fmaxf(most, q);
+    }
+    if (!Half<T>::kScaled) return;
+    if (lr == 0) red[threadIdx.x / LR] = most;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 1; i < 256 / LR; i++) most = fmaxf(most, red[i]);
+        (of_v ? v2 : rows2)[(size_t)bh * per + blk] = most;
+    }
+}
+
+// ---- launches -----------------------------------------------------------------------------------------------------------------------
+// Workgroups: 4 waves share a tile where that leaves every CU one or more; else one wave each. Then the other axis is split until
+// about two workgroups a CU run, two tiles each at least.
+constexpr uint32_t kCus = 256;
+void plan(Shape& s, uint32_t along, uint32_t other_tiles, int& waves) {
+    const uint64_t heads = (uint64_t)s.B * s.Hk;
+    waves = (uint64_t)div_up(along, 128) * heads >= kCus || along > 1024 ? 4 : 1;
+    s.tiles_x = div_up(along, 32u * waves);
+    const uint64_t base = s.tiles_x * heads;
+    uint64_t splits = base >= kCus ? 1 : (2 * kCus + base - 1) / base;
+    const uint64_t most = other_tiles / 2 ? other_tiles / 2 : 1;
+    if (splits > most) splits = most;
+    s.per_split = div_up(other_tiles, splits);
+    s.splits = div_up(other_tiles, s.per_split);
+}
+void plan_fwd(Shape& s, int& waves) { plan(s, s.rows, div_up(s.Nk, key_tile(padded(s.D))), waves); }
+void plan_dkdv(Shape& s, int& waves) { plan(s, s.Nk, s.group * div_up(s.Nq, query_tile(padded(s.D))), waves); }
+
+template <typename T, int DP, int NW>
+void launch_fwd(const void* q, const void* k, const void* v, void* o, void* o_lo, float* lse, float* part, float* ml, const Shape& s, hipStream_t st) {
+    hipLaunchKernelGGL((k_fwd<T, DP, NW>), dim3(s.tiles_x * s.splits * s.B * s.Hk), dim3(64 * NW), 0, st, static_cast<const T*>(q), static_cast<const T*>(k),
+                       static_cast<const T*>(v), static_cast<T*>(o), static_cast<T*>(o_lo), lse, part, ml, s);
+}
+template <typename T> void join_o(const float* part, const float* ml, const Shape& s, void* o, void* o_lo, float* lse, hipStream_t st) {
+    const uint64_t n = (uint64_t)s.B * s.H * s.Nq * (s.D / 4);
+    hipLaunchKernelGGL(k_join_o<T>, dim3((uint32_t)((n + 255) / 256)), dim3(256), 0, st, part, ml, s, static_cast<T*>(o), static_cast<T*>(o_lo), lse);
+}
+template <typename T>
+void join_sum(const float* pa, const float* pb, uint32_t splits, uint32_t B, uint32_t H, uint32_t N, uint32_t D, void* oa, void* ob, hipStream_t st) {
+    const uint64_t n = (uint64_t)B * H * N * (D / 4);
+    hipLaunchKernelGGL(k_join_sum<T>, dim3((uint32_t)((n + 255) / 256), ob ? 2 : 1), dim3(256), 0, st, pa, pb, splits, B, H, N, D, static_cast<T*>(oa),
+                       static_cast<T*>(ob));
+}
+template <typename T> void prep(const void* v, const void* o, const void* o_lo, const void* dy, const float* lse, const Shape& s, float* delta, float* rows2, float* v2, hipStream_t st) {
+    const uint32_t bh = s.B * s.Hk;
+    const dim3 grid(bh * (prep_blocks(s.rows) + (Half<T>::kScaled ? prep_blocks(s.Nk) : 0)));
+    const T *vp = static_cast<const T*>(v), *op = static_cast<const T*>(o), *lp = static_cast<const T*>(o_lo), *yp = static_cast<const T*>(dy);
+    if (s.D <= 64) hipLaunchKernelGGL((k_prep<T, 8>), grid, dim3(256), 0, st, vp, op, lp, yp, lse, s, delta, rows2, v2);
+    else if (s.D <= 128) hipLaunchKernelGGL((k_prep<T, 16>), grid, dim3(256), 0, st, vp, op, lp, yp, lse, s, delta, rows2, v2);
+    else hipLaunchKernelGGL((k_prep<T, 32>), grid, dim3(256), 0, st, vp, op, lp, yp, lse, s, delta, rows2, v2);
+}
+
+const char* shape_error(uint32_t B, uint32_t H, uint32_t Hk, uint32_t Nq, uint32_t Nk, uint32_t D) {
+    if (!B || !H || !Hk || !Nq || !Nk) return "empty problem";
+    if (H % Hk) return "the key heads do not divide the query heads";
+    if (D == 0 || D % 8 || D > 256) return "the head width must be a multiple of 8 up to 256";
+    if (Nq >= 0x40000000u || Nk >= 0x40000000u || (uint64_t)(H / Hk) * Nq >= 0x40000000u) return "more than 2^30 queries or keys";
+    if ((uint64_t)B * H * ((uint64_t)Nq + Nk) >= 0x40000000ull) return "more than 2^30 rows";
+    return nullptr;
+}
+void fill(Shape& s, uint32_t B, uint32_t H, uint32_t Hk, uint32_t Nq, uint32_t Nk, uint32_t D) {
+    memset(&s, 0, sizeof s);
+    s.B = B; s.H = H; s.Hk = Hk; s.Nq = Nq; s.Nk = Nk; s.D = D;
+    s.group = H / Hk; s.rows = s.group * Nq;
+}
+void fill_call(Shape& s, const uint64_t* qs, const uint64_t* ks, const uint64_t* vs, const void* mask, float scale, int causal) {
+    s.q_sb = qs[0]; s.q_sn = qs[1]; s.q_sh = qs[2];
+    s.k_sb = ks[0]; s.k_sn = ks[1]; s.k_sh = ks[2];
+    s.v_sb = vs[0]; s.v_sn = vs[1]; s.v_sh = vs[2];
+    s.mask = static_cast<const uint8_t*>(mask);
+    s.causal = causal != 0;
+    s.off = (int)s.Nk - (int)s.Nq;
+    s.scale = scale;
+    s.c = scale * 1.4426950408889634f;
+}
+bool strides_ok(const uint64_t* a, const uint64_t* b, const uint64_t* c) {
+    uint64_t all = 0;
+    for (int i = 0; i < 3; i++) all |= a[i] | b[i] | c[i];
+    return all % 8 == 0;
+}
+uint64_t up16(uint64_t floats) { return (floats + 3) / 4 * 4; }
+struct BwdLayout { uint64_t rows2, v2, pq, pk, pv, total; };   // float offsets behind delta
+BwdLayout bwd_layout(const Shape& s0) {
+    Shape a = s0, b = s0;
+    int wa, wb;
+    plan_fwd(a, wa);
+    plan_dkdv(b, wb);
+    const uint64_t heads = (uint64_t)s0.B * s0.Hk;
+    BwdLayout l;
+    l.rows2 = up16(heads * s0.rows);
+    l.v2 = l.rows2 + up16(heads * prep_blocks(s0.rows));
+    l.pq = l.v2 + up16(heads * prep_blocks(s0.Nk));
+    l.pk = l.pq + (a.splits > 1 ? a.splits * heads * s0.rows * s0.D : 0);
+    const uint64_t one = b.splits > 1 ? b.splits * heads * s0.Nk * s0.D : 0;
+    l.pv = l.pk + one;
+    l.total = l.pv + one;
+    return l;
+}
+
+}  // namespace
+
+extern "C" {
+
+uint64_t sdfx_attention_train_scratch_bytes(uint32_t B, uint32_t H, uint32_t Hk, uint32_t Nq, uint32_t Nk, uint32_t D, int backward) {
+    if (shape_error(B, H, Hk, Nq, Nk, D)) return 0;
+    Shape s;
+    fill(s, B, H, Hk, Nq, Nk, D);
+    if (backward) return bwd_layout(s).total * 4;
+    int waves;
+    plan_fwd(s, waves);
+    return s.splits > 1 ? ((uint64_t)s.splits * B * s.Hk * s.rows * (D + 2)) * 4 : 0;
+}
+
+int sdfx_attention_train_forward(const void* q, const void* k, const void* v, const void* key_mask, uint32_t B, uint32_t H, uint32_t Hk, uint32_t Nq,
+                                 uint32_t Nk, uint32_t D, const uint64_t* q_strides, const uint64_t* k_strides, const uint64_t* v_strides, float scale,
+                                 int causal, int bf16, void* o, void* o_lo, float* lse, float* scratch, sdfx_stream_t stream) {
+    SDFX_REQUIRE(q && k && v && o && q_strides && k_strides && v_strides, "attention_train_forward: null pointer");
+    const char* e = shape_error(B, H, Hk, Nq, Nk, D);
+    SDFX_REQUIRE(!e, "attention_train_forward: %s (B=%u H=%u Hk=%u Nq=%u Nk=%u D=%u)", e, B, H, Hk, Nq, Nk, D);
+    SDFX_REQUIRE(scale > 0.f && scale < 3e38f, "attention_train_forward: the scale must be positive and finite");
+    SDFX_REQUIRE(strides_ok(q_strides, k_strides, v_strides) && ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) |
+                 reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(o_lo) | reinterpret_cast<uintptr_t>(scratch)) % 16) == 0,
+                 "attention_train_forward: rows must be 16-byte aligned");
+    Shape s;
+    fill(s, B, H, Hk, Nq, Nk, D);
+    fill_call(s, q_strides, k_strides, v_strides, key_mask, scale, causal);
+    int waves;
+    plan_fwd(s, waves);
+    SDFX_REQUIRE(s.splits == 1 || scratch, "attention_train_forward: this shape needs scratch");
+    float* ml = s.splits > 1 ? scratch + (uint64_t)s.splits * B * s.Hk * s.rows * D : nullptr;
+    hipStream_t st = as_stream(stream);
+    SDFX_ATTN_DISPATCH(launch_fwd, q, k, v, o, o_lo, lse, scratch, ml, s, st);
+    if (s.splits > 1) {
+        if (bf16) join_o<__bf16>(scratch, ml, s, o, o_lo, lse, st);
+        else join_o<_Float16>(scratch, ml, s, o, o_lo, lse, st);
+    }
+    return check_launch("attention_train_forward");
+}
+
+int sdfx_attention_train_backward(const void* q, const void* k, const void* v, const void* key_mask, const void* o, const void* o_lo, const float* lse,
+                                  const void* dy, uint32_t B, uint32_t H, uint32_t Hk, uint32_t Nq, uint32_t Nk, uint32_t D, const uint64_t* q_strides,
+                                  const uint64_t* k_strides, const uint64_t* v_strides, float scale, int causal, int bf16, void* dq, void* dk, void* dv,
+                                  float* scratch, sdfx_stream_t stream) {
+    SDFX_REQUIRE(q && k && v && o && o_lo && lse && dy && scratch && q_strides && k_strides && v_strides, "attention_train_backward: null pointer");
+    SDFX_REQUIRE(!dk == !dv, "attention_train_backward: dk and dv come together");
+    const char* e = shape_error(B, H, Hk, Nq, Nk, D);
+    SDFX_REQUIRE(!e, "attention_train_backward: %s (B=%u H=%u Hk=%u Nq=%u Nk=%u D=%u)", e, B, H, Hk, Nq, Nk, D);
+    SDFX_REQUIRE(scale > 0.f && scale < 3e38f, "attention_train_backward: the scale must be positive and finite");
+    SDFX_REQUIRE(strides_ok(q_strides, k_strides, v_strides) && ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) |
+                 reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(o_lo) | reinterpret_cast<uintptr_t>(dy) |
+                 reinterpret_cast<uintptr_t>(dq) | reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv) | reinterpret_cast<uintptr_t>(scratch)) % 16) == 0,
+                 "attention_train_backward: rows must be 16-byte aligned");
+    Shape s;
+    fill(s, B, H, Hk, Nq, Nk, D);
+    fill_call(s, q_strides, k_strides, v_strides, key_mask, scale, causal);
+    const BwdLayout l = bwd_layout(s);
+    hipStream_t st = as_stream(stream);
+    BwdArgs a;
+    a.q = q; a.k = k; a.v = v; a.dy = dy; a.lse = lse;
+    a.delta = scratch; a.rows2 = scratch + l.rows2; a.v2 = scratch + l.v2;
+    a.dq = dq; a.dk = dk; a.dv = dv;
+    if (bf16) prep<__bf16>(v, o, o_lo, dy, lse, s, scratch, scratch + l.rows2, scratch + l.v2, st);
+    else prep<_Float16>(v, o, o_lo, dy, lse, s, scratch, scratch + l.rows2, scratch + l.v2, st);
+    if (dk) {
+        Shape t = s;
+        int waves;
+        plan_dkdv(t, waves);
+        a.part = scratch + l.pk; a.part2 = scratch + l.pv;
+        launch_dkdv(a, t, bf16, waves, st);
+        if (t.splits > 1) {
+            if (bf16) join_sum<__bf16>(a.part, a.part2, t.splits, B, Hk, Nk, D, dk, dv, st);
+            else join_sum<_Float16>(a.part, a.part2, t.splits, B, Hk, Nk, D, dk, dv, st);
+        }
+    }
+    if (dq) {
+        Shape t = s;
+        int waves;
+        plan_fwd(t, waves);
+        a.part = scratch + l.pq; a.part2 = nullptr;
+        launch_dq(a, t, bf16, waves, st);
+        if (t.splits > 1) {
+            if (bf16) join_sum<__bf16>(a.part, nullptr, t.splits, B, H, Nq, D, dq, nullptr, st);
+            else join_sum<_Float16>(a.part, nullptr, t.splits, B, H, Nq, D, dq, nullptr, st);
+        }
+    }
+    return check_launch("attention_train_backward");
+}
+
+}  // extern "C"

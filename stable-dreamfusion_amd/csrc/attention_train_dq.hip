@@ -1,0 +1,126 @@
+// attention_train_dq.hip — dq = scale ds k of attention's gradient (attention_train.h). A wave owns 32 rows: q and dy in registers, the key /
+// value tiles shared by the workgroup's waves in LDS, double-buffered. Per 32 keys: s^T = k q^T and dp^T = v dy^T, p = exp2(s c - lse) with the
+// forward's log-sum-exp, ds = p (dp - delta) with the lane's own delta, dq^T += k^T ds^T. One pass, no row statistics to find.
+#include "attention_train.h"
+
+namespace sdfx_attn {
+namespace {
+
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_dq(BwdArgs a, Shape s) {
+    constexpr int KT = key_tile(DP), KS = DP / 16, DT = (DP + 31) / 32, NB = KT / 32;
+    typedef Tile<DP, KT, 64 * NW> L;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[4 * L::BYTES + kTileSlack];
+    uint8_t* const ldsV = lds;
+    uint8_t* const ldsK = lds + 2 * L::BYTES;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, x = lane & 31u, hi = lane >> 5;
+    const uint32_t per_bh = s.tiles_x * s.splits;
+    const uint32_t lid = xcd_contiguous(blockIdx.x, per_bh * s.B * s.Hk);
+    const uint32_t bh = lid / per_bh, rest = lid - bh * per_bh, split = rest / s.tiles_x, xt = rest - split * s.tiles_x;
+    const uint32_t b = bh / s.Hk, hk = bh - b * s.Hk;
+    const uint32_t r0 = xt * NW * 32u, w0 = r0 + wave * 32u;
+    const Row row = row_of(s, w0 + x, hk);
+    const T* kb = static_cast<const T*>(a.k) + (size_t)b * s.k_sb + (size_t)hk * s.k_sh;
+    const T* vb = static_cast<const T*>(a.v) + (size_t)b * s.v_sb + (size_t)hk * s.v_sh;
+
+    typename Half<T>::v8 qf[KS], yf[KS];
+    row_fragments<T, KS>(qf, static_cast<const T*>(a.q) + (size_t)b * s.q_sb + (size_t)row.qi * s.q_sn + (size_t)row.head * s.q_sh, s.D, hi);
+    row_fragments<T, KS>(yf, static_cast<const T*>(a.dy) + (((size_t)b * s.Nq + row.qi) * s.H + row.head) * s.D, s.D, hi);
+    const size_t at = (size_t)bh * s.rows + row.R;
+    const float lse = a.lse[at];
+    float g = 1.f;
+    if (Half<T>::kScaled) g = grad_scale(a.rows2 + (size_t)bh * prep_blocks(s.rows), prep_blocks(s.rows), a.v2 + (size_t)bh * prep_blocks(s.Nk), prep_blocks(s.Nk), lane);
+    const float nlse = Half<T>::kShift - lse, ndelta = -a.delta[at] * g;
+
+    uint32_t kend = s.Nk;
+    int wave_lo = 0x7fffffff, wave_hi = 0x7fffffff;
+    if (s.causal) {
+        uint32_t lo, hi_q;
+        query_range(s, r0, min(r0 + NW * 32u, s.rows) - 1u, lo, hi_q);
+        kend = (uint32_t)max(0, min((int)s.Nk, (int)hi_q + s.off + 1));
+        query_range(s, min(w0, s.rows - 1u), min(w0 + 32u, s.rows) - 1u, lo, hi_q);
+        wave_lo = (int)lo + s.off; wave_hi = (int)hi_q + s.off;
+    }
+    const uint32_t t0 = split * s.per_split, t1 = min(t0 + s.per_split, (kend + KT - 1) / KT);
+
+    f32x16 acc[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++) acc[dt] = zero16();
+    if (t0 < t1) {
+        u4v rk[L::PT], rv[L::PT];
+        request<L>(rk, kb, s.k_sn, t0 * KT, s.Nk, s.D, tid, 64 * NW);
+        request<L>(rv, vb, s.v_sn, t0 * KT, s.Nk, s.D, tid, 64 * NW);
+        uint64_t live = live_keys<KT>(s, mask_byte<KT>(s, b, t0, lane), t0, lane);
+        stash<L>(ldsK, rk, live, tid, 64 * NW);
+        stash<L>(ldsV, rv, live, tid, 64 * NW);
+        __syncthreads();
+        for (uint32_t j = t0; j < t1; j++) {
+            const uint32_t buf = (j - t0) & 1u;
+            uint8_t next_byte = 0;
+            if (j + 1 < t1) {
+                request<L>(rk, kb, s.k_sn, (j + 1) * KT, s.Nk, s.D, tid, 64 * NW);
+                request<L>(rv, vb, s.v_sn, (j + 1) * KT, s.Nk, s.D, tid, 64 * NW);
+                next_byte = mask_byte<KT>(s, b, j + 1, lane);
+            }
+            const uint8_t* kt = ldsK + buf * L::BYTES;
+            const uint8_t* vt = ldsV + buf * L::BYTES;
+            if (live != 0 && (int)(j * KT) <= wave_hi) {
+                const bool some_hidden = live != all_keys<KT>() || (int)(j * KT + KT - 1) > wave_lo;
+#pragma unroll
+                for (int st = 0; st < NB; st++) {
+                    f32x16 sc = zero16(), dp = zero16();
+#pragma unroll
+                    for (int ks = 0; ks < KS; ks++) sc = mma(row_operand<T, L>(kt, st, ks, x, hi), qf[ks], sc);
+#pragma unroll
+                    for (int ks = 0; ks < KS; ks++) dp = mma(row_operand<T, L>(vt, st, ks, x, hi), yf[ks], dp);
+                    if (some_hidden) hide(sc, live, row.lim, j * KT, st, hi);
+#pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], s.c, nlse));
+                        sc[r] = p * __builtin_fmaf(dp[r], g, ndelta);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const typename Half<T>::v8 f = operand<T>(sc, e);            // (ds rounded to the inputs' type)
+#pragma unroll
+                        for (int dt = 0; dt < DT; dt++) acc[dt] = mma(col_operand<T, L>(kt, 2 * st + e, dt, lane), f, acc[dt]);
+                    }
+                }
+            }
+            if (j + 1 < t1) {
+                live = live_keys<KT>(s, next_byte, j + 1, lane);
+                stash<L>(ldsK + (buf ^ 1u) * L::BYTES, rk, live, tid, 64 * NW);
+                stash<L>(ldsV + (buf ^ 1u) * L::BYTES, rv, live, tid, 64 * NW);
+            }
+            __syncthreads();
+        }
+    }
+    if (!row.on) return;
+    const bool empty = lse == INFINITY;                       // a row that sees nothing has no gradient, whatever its dy holds
+    const float f = s.scale * (Half<T>::kScaled ? 1.f / 32768.f : 1.f) / g;
+    float* pp = s.splits > 1 ? a.part + ((size_t)split * s.B * s.Hk * s.rows + at) * s.D : nullptr;
+    T* op = static_cast<T*>(a.dq) + (((size_t)b * s.Nq + row.qi) * s.H + row.head) * s.D;
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; q4++) {
+            const uint32_t c0 = 32u * dt + 8u * q4 + 4u * hi;
+            if (c0 < s.D) {
+                float w[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) w[i] = empty ? 0.f : acc[dt][4 * q4 + i] * f;
+                if (pp) *reinterpret_cast<f4*>(pp + c0) = f4{w[0], w[1], w[2], w[3]};
+                else store4(op + c0, w[0], w[1], w[2], w[3]);
+            }
+        }
+}
+
+template <typename T, int DP, int NW> void go(const BwdArgs& a, const Shape& s, hipStream_t st) {
+    hipLaunchKernelGGL((k_dq<T, DP, NW>), dim3(s.tiles_x * s.splits * s.B * s.Hk), dim3(64 * NW), 0, st, a, s);
+}
+
+}  // namespace
+
+void launch_dq(const BwdArgs& a, const Shape& s, int bf16, int waves, hipStream_t st) { SDFX_ATTN_DISPATCH(go, a, s, st); }
+
+}  // namespace sdfx_attn

@@ -1,0 +1,340 @@
+"""csrc/attention_train*.hip, groupnorm_train.hip and geglu_train.hip against float64 with elementwise bounds (tests/train_ops_ref.py)."""
+import pytest
+import torch
+
+import train_ops_ref as ref
+from sdfx_nerf.attention import attention
+from sdfx_nerf.groupnorm import eight_bits, geglu, group_norm_act
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+
+
+def _rn(dev, *shape, seed=0, dtype=F16, scale=1.0):
+    return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * scale).to(dtype).to(dev)
+
+
+def _heads(dev, B, H, N, d, seed, dtype, scale=1.0):
+    """[B, H, N, d] as the transformer blocks form it: a projection's [B, N, H d] output viewed."""
+    return _rn(dev, B, N, H * d, seed=seed, dtype=dtype, scale=scale).view(B, N, H, d).transpose(1, 2)
+
+
+def _mask(dev, kind, B, Nk, seed=7):
+    if kind == "none":
+        return None
+    g = torch.Generator().manual_seed(seed)
+    if kind == "holes":
+        return (torch.rand(B, Nk, generator=g) < 0.6).to(dev)
+    n = torch.randint(1, Nk + 1, (B,), generator=g)
+    if B > 1:
+        n[0] = 0                                   # a batch entry without a key
+    return (torch.arange(Nk)[None] < n[:, None]).to(dev)
+
+
+def _attend(q, k, v, dy, mask=None, causal=False, scale=None):
+    q, k, v = (t.detach().requires_grad_(True) for t in (q, k, v))
+    o = attention(q, k, v, mask, causal, scale)
+    return [o.detach(), *torch.autograd.grad(o, (q, k, v), dy)]
+
+
+def _compare(got, want, bound):
+    for n, g, w, b in zip(("o", "dq", "dk", "dv"), got, want, bound):
+        ref.check(n, g, w, b)
+
+
+@pytest.mark.parametrize("dtype,B,H,Hk,Nq,Nk,d,causal,mask,spread", [
+    (F16, 1, 1, 1, 1, 1, 8, False, "none", 1.0),              # one score: p = 1, no gradient for q and k
+    (F16, 1, 3, 1, 2, 31, 16, False, "none", 1.0),
+    (BF16, 2, 8, 8, 64, 77, 160, False, "prompt", 1.0),
+    (F16, 2, 4, 2, 33, 65, 40, True, "none", 2.0),            # more keys than queries
+    (BF16, 1, 6, 2, 130, 100, 64, True, "holes", 1.0),        # more queries than keys: rows without a key
+    (F16, 3, 2, 2, 100, 200, 80, False, "prompt", 1.0),
+    (F16, 1, 2, 1, 257, 1000, 128, False, "none", 1.0),
+    (BF16, 1, 2, 2, 70, 300, 256, False, "none", 1.0),
+    (F16, 1, 2, 1, 40, 90, 200, True, "holes", 1.0),
+    (F16, 1, 3, 1, 5, 4000, 72, False, "holes", 1.0),         # few queries: the key axis is split
+    (BF16, 1, 2, 2, 3001, 20, 48, False, "none", 1.0),        # few keys: the query axis is split
+    (F16, 2, 8, 8, 1024, 1024, 40, False, "none", 1.0),
+    (BF16, 1, 4, 1, 1, 777, 128, False, "prompt", 2.0),
+    (BF16, 2, 12, 4, 300, 300, 64, True, "none", 2.0),
+    (F16, 1, 4, 4, 1100, 1100, 56, True, "prompt", 1.0),
+    (BF16, 1, 8, 8, 1024, 77, 104, False, "prompt", 1.0),
+    (F16, 4, 16, 16, 70, 500, 128, False, "none", 1.0),       # whole workgroups of four waves
+    (BF16, 4, 16, 16, 130, 140, 256, True, "none", 1.0),
+    (F16, 4, 16, 16, 130, 140, 160, False, "holes", 1.0),
+])
+def test_attention_and_its_gradient(dev, dtype, B, H, Hk, Nq, Nk, d, causal, mask, spread):
+    q, k, v = _heads(dev, B, H, Nq, d, 1, dtype, spread), _heads(dev, B, Hk, Nk, d, 2, dtype, spread), _heads(dev, B, Hk, Nk, d, 3, dtype)
+    dy, m = _rn(dev, B, Nq, H * d, seed=4, dtype=dtype), _mask(dev, mask, B, Nk)
+    got = _attend(q, k, v, dy, m, causal)
+    _compare(got, *ref.attention(q, k, v, dy, m, causal))
+    again = _attend(q, k, v, dy, m, causal)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))                 # nothing depends on the order of workgroups
+    with torch.no_grad():
+        assert torch.equal(attention(q, k, v, m, causal), got[0])             # the same output when nothing is kept
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_masked_places_may_hold_anything(dev, dtype, causal):
+    """Infinities and NaN in masked keys and values, and in the dy of rows without a key, reach nothing; masked keys get zero gradients."""
+    B, H, N, d = 3, 2, 150, 40
+    q, k, v, dy = (_heads(dev, B, H, N, d, i, dtype) for i in (1, 2, 3, 4))
+    m = _mask(dev, "holes", B, N)
+    m[:, 64:128] = False                          # a whole tile
+    m[1] = False                                  # a batch entry
+    m[2, :30] = False                             # with the causal mask: rows 0 .. 29 of entry 2 see nothing
+    dy = dy.transpose(1, 2).reshape(B, N, H * d).clone()
+    clean = _attend(q, k, v, dy, m, causal)
+    hid = ~m[:, None, :, None].expand_as(k)
+    k2, v2, dy2 = k.clone(), v.clone(), dy.clone()
+    k2[hid] = torch.tensor([float("nan"), float("inf"), -float("inf"), torch.finfo(dtype).min], device=dev, dtype=dtype).repeat(int(hid.sum()) // 4)
+    v2[hid] = float("nan")
+    dy2[1] = float("nan")
+    if causal:
+        dy2[2, :30] = float("inf")
+    got = _attend(q, k2, v2, dy2, m, causal)
+    assert all(torch.isfinite(t).all() for t in got)
+    assert not got[0][1].any() and not got[1][1].any() and not got[2][hid].any() and not got[3][hid].any()
+    _compare(got, *ref.attention(q, k, v, dy, m, causal))
+    assert torch.equal(got[0], clean[0])
+
+
+def test_attention_strides_views_and_shared_context(dev):
+    """q / k / v cut out of one stacked projection, a context expanded over the batch, an odd layout that is copied, a dy that is a view."""
+    B, H, N, d = 2, 4, 50, 40
+    qkv = _rn(dev, B, N, 3 * H * d, seed=1)
+    q, k, v = (qkv[..., i * H * d:(i + 1) * H * d].unflatten(-1, (H, d)).transpose(1, 2) for i in range(3))
+    dy = _rn(dev, B, N + 3, 2 * H * d, seed=2)[:, 3:, ::2]
+    _compare(_attend(q, k, v, dy), *ref.attention(q, k, v, dy))
+    ctx = _rn(dev, 1, H, 33, d, seed=3)
+    k2 = ctx.expand(B, H, 33, d)
+    _compare(_attend(q, k2, k2, dy), *ref.attention(q, k2, k2, dy))
+    leaf = ctx.clone().requires_grad_(True)                                # the gradient of a broadcast context is the sum over the batch
+    (g,) = torch.autograd.grad(attention(q, leaf.expand(B, H, 33, d), k2), leaf, dy)
+    want, bound = ref.attention(q, k2, k2, dy)
+    ref.check("ctx", g, want[2].sum(0, keepdim=True), bound[2].sum(0, keepdim=True) + ref.half_step(F16) * want[2].abs().sum(0, keepdim=True))
+    odd = _rn(dev, B, H, d, N + 1, seed=4)[..., 1:].transpose(2, 3)          # channel stride N + 1
+    _compare(_attend(odd, k, v, dy, scale=0.37), *ref.attention(odd, k, v, dy, scale=0.37))
+
+
+def test_attention_wanted_gradients_only(dev):
+    B, H, N, d = 1, 2, 60, 64
+    q, k, v, dy = (_heads(dev, B, H, N, d, i, F16) for i in (1, 2, 3, 4))
+    dy = dy.transpose(1, 2).reshape(B, N, H * d)
+    full = _attend(q, k, v, dy)
+    for which in ((0,), (1,), (2,), (1, 2)):
+        leaves = [t.detach().requires_grad_(i in which) for i, t in enumerate((q, k, v))]
+        o = attention(*leaves)
+        for i, g in zip(which, torch.autograd.grad(o, [leaves[i] for i in which], dy)):
+            assert torch.equal(g, full[1 + i])
+
+
+@pytest.mark.parametrize("size", [2.0 ** -12, 1.0, 2.0 ** 12])
+def test_attention_fp16_gradients_keep_their_digits_at_any_loss_scale(dev, size):
+    """2048 keys with nearly equal probabilities (2^-11 each) and dy scaled: ds would leave fp16's normal range without its power of two. The
+    relative error (2-norm) of every gradient stays at a few half steps wherever the gradient itself is a normal number."""
+    B, H, N, d = 1, 2, 2048, 64
+    q, k, v, dy = (_heads(dev, B, H, N, d, i, F16) for i in (1, 2, 3, 4))
+    q = q * 0.25
+    v = v * 8                                     # (gradients of q and k well above 2^-24)
+    dy = (dy.transpose(1, 2).reshape(B, N, H * d) * size).to(F16)
+    got = _attend(q, k, v, dy)
+    want, _ = ref.attention(q, k, v, dy)
+    for n, g, w in list(zip(("o", "dq", "dk", "dv"), got, want)):
+        big = w.abs() > 2.0 ** -13
+        if big.float().mean() > 0.1:
+            err = float((g.cpu().double() - w)[big].norm() / w[big].norm())
+            assert err <= 3 * ref.half_step(F16), (n, err)                   # p and ds rounded once, the result once: sqrt(2) half steps at most, and the sums
+
+
+def test_attention_on_another_stream_and_two_at_once(dev):
+    B, H, N, d = 1, 4, 700, 40
+    q, k, v, dy = (_heads(dev, B, H, N, d, i, BF16) for i in (1, 2, 3, 4))
+    dy = dy.transpose(1, 2).reshape(B, N, H * d).contiguous()
+    want = _attend(q, k, v, dy)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for s in streams:
+        with torch.cuda.stream(s):
+            got.append([_attend(q, k, v, dy) for _ in range(3)])
+    torch.cuda.synchronize()
+    for one in got:
+        for r in one:
+            assert all(torch.equal(a, b) for a, b in zip(r, want))
+
+
+# ---- group norm -----------------------------------------------------------------------------------------------------------------
+def _norm(x, G, w, b, dy, **kw):
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+    pre = kw.pop("pre", None)
+    if pre is not None:
+        pre = pre.detach().requires_grad_(True)
+    y = group_norm_act(leaves[0], G, leaves[1], leaves[2], pre=pre, **kw)
+    names = ["dx", "dweight", "dbias"] + ([] if pre is None else ["dpre"])
+    return dict(zip(names, torch.autograd.grad(y, leaves + ([] if pre is None else [pre]), dy)), y=y.detach())
+
+
+@pytest.mark.parametrize("checkpoint", ["full", "int8"])
+@pytest.mark.parametrize("dtype,params,N,C,H,W,G,act,pre", [
+    (F16, F16, 2, 320, 16, 16, 32, True, True),
+    (F16, F32, 1, 128, 64, 48, 32, True, False),
+    (BF16, BF16, 2, 1280, 8, 8, 32, True, True),
+    (BF16, F32, 3, 96, 37, 5, 8, False, True),
+    (F32, F32, 2, 64, 19, 23, 16, True, False),
+    (F32, F32, 1, 32, 1, 16, 1, False, False),
+    (F16, F16, 1, 2560, 4, 4, 32, True, False),          # the widest
+    (F16, F32, 5, 32, 3, 7, 32, True, True),             # one channel a group
+    (BF16, F32, 1, 64, 300, 301, 32, True, True),        # many slabs, a ragged end
+    (F16, F16, 1, 1024, 5, 5, 1, True, True),            # one group
+])
+def test_group_norm_and_its_gradient(dev, dtype, params, N, C, H, W, G, act, pre, checkpoint):
+    cl = lambda t: t.contiguous(memory_format=torch.channels_last)
+    shift = _rn(dev, 1, C, 1, 1, seed=9, dtype=F32)
+    x = cl((_rn(dev, N, C, H, W, seed=1, dtype=F32, scale=1.5) + shift).to(dtype))
+    dy = cl(_rn(dev, N, C, H, W, seed=2, dtype=dtype))
+    w, b = _rn(dev, C, seed=3, dtype=params), _rn(dev, C, seed=4, dtype=params)
+    e = _rn(dev, N, C, seed=5, dtype=dtype) if pre else None
+    got = _norm(x, G, w, b, dy, act=act, pre=e, checkpoint=checkpoint)
+    assert got["y"].is_contiguous(memory_format=torch.channels_last) and got["y"].dtype == dtype and got["dweight"].dtype == params
+    for n, (want, bound) in ref.group_norm(x, G, w, b, dy, act=act, pre=e, eight=checkpoint == "int8").items():
+        ref.check(n, got[n], want, bound)
+    again = _norm(x, G, w, b, dy, act=act, pre=e, checkpoint=checkpoint)
+    assert all(torch.equal(got[n], again[n]) for n in got)
+    with torch.no_grad():
+        assert torch.equal(group_norm_act(x, G, w, b, act=act, pre=e, checkpoint=checkpoint), got["y"])
+
+
+def test_group_norm_far_mean_other_layouts_and_wanted_gradients(dev):
+    x = (_rn(dev, 2, 32, 20, 20, seed=1, dtype=F32) * 0.5 + 60)             # the mean is 120 deviations away
+    w, b, dy = _rn(dev, 32, seed=2, dtype=F32), _rn(dev, 32, seed=3, dtype=F32), _rn(dev, 2, 32, 20, 20, seed=4, dtype=F32)
+    got = _norm(x, 4, w, b, dy)                                             # x and dy NCHW: copied
+    for n, (want, bound) in ref.group_norm(x, 4, w, b, dy).items():
+        ref.check(n, got[n], want, bound)
+    off = _rn(dev, 2, 20, 20, 33, seed=5, dtype=F16)[..., 1:].permute(0, 3, 1, 2)      # neither dense nor aligned
+    h = [t.half() for t in (w, b, dy)]
+    got = _norm(off, 4, *h)
+    for n, (want, bound) in ref.group_norm(off, 4, *h).items():
+        ref.check(n, got[n], want, bound)
+    xs, ws, bs = off.detach().requires_grad_(True), h[0].detach().requires_grad_(True), h[1]
+    (g,) = torch.autograd.grad(group_norm_act(xs, 4, ws.detach(), bs), xs, h[2])
+    (gw,) = torch.autograd.grad(group_norm_act(off, 4, ws, bs), ws, h[2])
+    assert torch.equal(g, got["dx"]) and torch.equal(gw, got["dweight"])
+    odd = _rn(dev, 2, 20, 4, 4, seed=6)                                     # 20 channels: the formulas in PyTorch ops
+    ww = torch.ones(20, device=dev, dtype=F16)
+    r = ref.group_norm(odd, 5, ww, ww, odd)
+    got = _norm(odd, 5, ww, ww, odd)
+    for n in r:
+        ref.check(n, got[n], *r[n])
+
+
+def test_eight_bit_input_with_infinities_poisons_its_block_and_group_only(dev):
+    """A block with an infinity decodes as NaN: the map's group is NaN anyway, other samples stay exact."""
+    x = _rn(dev, 2, 32, 4, 4, seed=1).contiguous(memory_format=torch.channels_last)
+    w, b, dy = _rn(dev, 32, seed=2), _rn(dev, 32, seed=3), _rn(dev, 2, 32, 4, 4, seed=4)
+    clean = _norm(x, 1, w, b, dy, checkpoint="int8")
+    bad = x.clone()
+    bad[1, 3, 2, 2] = float("inf")
+    got = _norm(bad, 1, w, b, dy, checkpoint="int8")
+    assert got["y"][1].isnan().any() and got["dx"][1].isnan().all() and torch.equal(got["dx"][0], clean["dx"][0])
+
+
+# ---- GEGLU ----------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("checkpoint", ["full", "int8"])
+@pytest.mark.parametrize("dtype,lead,n", [(F16, (2, 333), 320), (BF16, (77,), 64), (F32, (5, 3), 96), (F16, (1,), 32), (BF16, (4099,), 1280), (F32, (), 32)])
+def test_geglu_and_its_gradient(dev, dtype, lead, n, checkpoint):
+    x, dy = _rn(dev, *lead, 2 * n, seed=1, dtype=dtype, scale=2.0), _rn(dev, *lead, n, seed=2, dtype=dtype)
+    leaf = x.detach().requires_grad_(True)
+    y = geglu(leaf, checkpoint)
+    (dx,) = torch.autograd.grad(y, leaf, dy)
+    r = ref.geglu(x, dy, checkpoint == "int8")
+    ref.check("y", y, *r["y"])
+    ref.check("dx", dx, *r["dx"])
+    with torch.no_grad():
+        assert torch.equal(geglu(x, checkpoint), y)
+
+
+def test_geglu_far_arguments_views_and_other_widths(dev):
+    x = torch.tensor([[1.0, -1.0] * 8 + [0.0, -0.0, 40.0, -40.0, 6.0, -6.0, 300.0, -300.0] * 2], device=dev, dtype=F32)
+    dy = torch.ones(1, 16, device=dev)
+    leaf = x.clone().requires_grad_(True)
+    y = geglu(leaf, "full")
+    (dx,) = torch.autograd.grad(y, leaf, dy)
+    r = ref.geglu(x, dy)
+    ref.check("y", y, *r["y"])
+    ref.check("dx", dx, *r["dx"])
+    v = _rn(dev, 9, 300, seed=1)[:, 3:259]                                  # a view, off alignment
+    d = _rn(dev, 9, 256, seed=2)[:, ::2]
+    leaf = v.detach().requires_grad_(True)
+    y = geglu(leaf, "full")
+    (dx,) = torch.autograd.grad(y, leaf, d)
+    r = ref.geglu(v, d)
+    ref.check("y", y, *r["y"])
+    ref.check("dx", dx, *r["dx"])
+    leaf = _rn(dev, 9, 20, seed=3).requires_grad_(True)                     # 10 channels: the formulas in PyTorch ops
+    y = geglu(leaf, "full")
+    r = ref.geglu(leaf, torch.ones(9, 10))
+    ref.check("y", y, *r["y"])
+    ref.check("dx", torch.autograd.grad(y, leaf, torch.ones_like(y))[0], *r["dx"])
+
+
+def test_the_kernels_eight_bit_form_is_the_documented_one(dev):
+    """Codes and scale bytes as the forward writes them, decoded by the documented layout, against `eight_bits`."""
+    import _sdfx as S
+    x = _rn(dev, 65, 64, seed=1, dtype=F32) * torch.exp(8 * _rn(dev, 65, 1, seed=2, dtype=F32))
+    x[3] = 0
+    x[4, :32] *= 2.0 ** -130
+    x[5, 7], x[6, 40] = float("nan"), -float("inf")
+    y, saved = torch.empty(65, 32, device=dev), torch.empty(65 * 64 + 65 * 2, dtype=torch.uint8, device=dev)
+    S.call("sdfx_geglu_train_forward", S.ptr(x), 65, 32, 2, S.ptr(y), S.ptr(saved), S.stream())
+    saved = saved.cpu()                           # (2^n by torch.pow is exact on the CPU; on the GPU it is not)
+    codes, scale = saved[:65 * 64].view(torch.int8).view(65, 2, 32).double(), saved[65 * 64:].view(65, 2, 1).double()
+    step = torch.where(scale == 255, torch.full_like(scale, float("inf")), torch.pow(2.0, scale - 127))
+    got, want = (codes * step).view(65, 64), eight_bits(x).double().cpu()
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(torch.nan_to_num(got), torch.nan_to_num(want))
+
+
+# ---- together -------------------------------------------------------------------------------------------------------------------
+def test_captured_and_replayed(dev):
+    """Forward and backward of the three in one captured graph, replayed on new inputs with eager work in between: the eager results. Two
+    such graphs replayed on two streams at once share no workspace."""
+    B, H, N, d, C = 1, 4, 640, 40, 160
+    w, b = _rn(dev, C, seed=1, dtype=F32), _rn(dev, C, seed=2, dtype=F32)
+
+    def step(x, dy):
+        leaf, ww = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        n = group_norm_act(leaf, 32, ww, b, checkpoint="int8").permute(0, 2, 3, 1).reshape(B, N, C)
+        h = n.view(B, N, H, d).transpose(1, 2)
+        out = geglu(attention(h, h[:, :, :77], h[:, :, :77]) + n, "int8" if (C // 2) % 32 == 0 else "full")
+        return [out.detach(), *torch.autograd.grad(out, (leaf, ww), dy)]
+
+    make = lambda s: (_rn(dev, B, C, 20, 32, seed=s).contiguous(memory_format=torch.channels_last), _rn(dev, B, N, C // 2, seed=s + 50))
+    graphs = []
+    for i in range(2):
+        x, dy = make(0)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(x, dy)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step(x, dy)
+        graphs.append((g, x, dy, out))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for s in range(1, 5):
+        ins = [make(10 * s + i) for i in range(2)]
+        want = [step(*t) for t in ins]
+        for (g, x, dy, _), (nx, ny) in zip(graphs, ins):
+            x.copy_(nx)
+            dy.copy_(ny)
+        torch.cuda.synchronize()
+        for st, (g, *_) in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for (_, _, _, out), r in zip(graphs, want):
+            assert all(torch.equal(a, c) for a, c in zip(out, r))
