@@ -6,7 +6,6 @@ nothing in the shipped path routes around the HIP kernels.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import os
 
@@ -181,6 +180,28 @@ def lib() -> C.CDLL:
     return _LIB
 
 
+BIND_PATH = os.path.join(_HERE, "csrc", "_sdfx_train.so")
+_NATIVE = None
+
+
+def native():
+    """csrc/train_ops_bind.cpp (once): the training operators as C++ autograd functions over the library lib() opened."""
+    global _NATIVE
+    if _NATIVE is None:
+        if not os.path.exists(BIND_PATH):
+            raise RuntimeError(f"_sdfx_train.so not found at {BIND_PATH}: build it with `python stable-dreamfusion_amd/build.py` "
+                               "(or __graft_entry__.build())")
+        import importlib.machinery
+        import importlib.util
+        loader = importlib.machinery.ExtensionFileLoader("_sdfx_train", BIND_PATH)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_file_location("_sdfx_train", BIND_PATH, loader=loader))
+        loader.exec_module(module)
+        names = ["sdfx_last_error"] + [n for n in _SIGNATURES if "_train_" in n]
+        module.bind({n: C.cast(getattr(lib(), n), C.c_void_p).value for n in names if hasattr(lib(), n)})
+        _NATIVE = module
+    return _NATIVE
+
+
 class row_limit:
     """`with row_limit(total, period): ...` — sdfx_set_row_limit around the calls inside (include/sdfx.h): rows whose index modulo
     `period` is >= total[0] (an int32 device tensor) are padding for the hinted encoder forward, the field kernels and the binned
@@ -280,11 +301,6 @@ def check(rc: int) -> None:
 def stream() -> C.c_void_p:
     """hipStream_t of torch's current stream on the current device."""
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
-
-
-def on_device(t):
-    """A context in which the device of `t` is the current one (and stream() its current stream)."""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def ptr(t) -> C.c_void_p | None:

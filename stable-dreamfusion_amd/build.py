@@ -24,6 +24,7 @@ INCLUDE = os.path.normpath(os.path.join(HERE, "..", "include"))
 DEVTOOLS_KERNELS = os.path.normpath(os.path.join(HERE, "..", "tools", "devtools_kernels"))
 LIB = os.path.join(CSRC, "libsdfx_hip.so")
 DEV_LIB = os.path.join(CSRC, "libsdfx_hip_dev.so")
+BIND = os.path.join(CSRC, "_sdfx_train.so")      # train_ops_bind.cpp: the training operators as C++ autograd functions (host code only)
 SOURCES = ["sdfx_core.hip", "raymarching.hip", "gridencoder.hip", "gridencoder_fwd.hip", "gridencoder_bwd_binned.hip", "encoders.hip", "field.hip", "optim.hip", "shade.hip", "render.hip", "occupancy.hip", "infer.hip", "head.hip", "sds.hip", "dmtet.hip", "raster.hip", "groupnorm.hip", "groupnorm_train.hip", "geglu_train.hip", "conv.hip", "attention.hip", "attention_train.hip", "attention_train_dq.hip", "attention_train_dkdv.hip"]
 ARCH = "gfx950"
 # -ffp-contract=off: the march / encode arithmetic must not gain FMAs the source does not spell
@@ -64,11 +65,33 @@ def _compile(src: str, force: bool, verbose: bool, devtools: bool = False) -> st
     return obj
 
 
+def _build_bind(force: bool, verbose: bool) -> str:
+    """train_ops_bind.cpp against the installed torch, with the host compiler. It holds no kernel and does not link the HIP library: _sdfx.py
+    hands it the entry points of the library it opened."""
+    src = os.path.join(CSRC, "train_ops_bind.cpp")
+    newest = max(os.path.getmtime(f) for f in (src, os.path.join(INCLUDE, "sdfx.h"), os.path.abspath(__file__)))
+    if not force and os.path.exists(BIND) and os.path.getmtime(BIND) >= newest:
+        return BIND
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension
+    inc = [a for p in (*cpp_extension.include_paths(), sysconfig.get_paths()["include"], "/opt/rocm/include") for a in ("-isystem", p)]
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           "-DTORCH_EXTENSION_NAME=_sdfx_train", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *inc, src, "-o", BIND,
+           "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.check_call(cmd)
+    return BIND
+
+
 def build(force: bool = False, verbose: bool = False, devtools: bool = False) -> str:
     sources = [s for s in SOURCES if os.path.exists(os.path.join(CSRC, s))]
     lib = DEV_LIB if devtools else LIB
     with cf.ThreadPoolExecutor(max_workers=min(len(sources), os.cpu_count() or 1)) as ex:
+        bind = ex.submit(_build_bind, force, verbose)
         objs = list(ex.map(lambda s: _compile(s, force, verbose, devtools), sources))
+    bind.result()
     if force or not os.path.exists(lib) or os.path.getmtime(lib) < max(os.path.getmtime(o) for o in objs):
         cmd = [hipcc(), "--offload-arch=" + ARCH, "-shared", "-fPIC", "-o", lib] + objs
         if verbose:

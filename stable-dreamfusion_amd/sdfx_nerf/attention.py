@@ -13,8 +13,8 @@ import ctypes as C
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 import _devswitch
+import _sdfx
 
 _FUSED = _devswitch.get("SDFX_ATTENTION", 1)
 _U3 = C.c_uint32 * 3
@@ -54,62 +54,6 @@ def attention_bnc(q, k, v, waves=0, force=False):
                int(waves), S.ptr(out), S.stream())
         return out
     return F.scaled_dot_product_attention(q, k, v).transpose(1, 2).reshape(B, Nq, H * d)
-
-
-_U64x3 = C.c_uint64 * 3
-
-
-def _taken(t):
-    """`t` [B, H, n, d] as the kernels read it (unit channel stride, 16-byte rows): itself, or a copy."""
-    sb, sh, sn, sd = t.stride()
-    return t if sd == 1 and not (sb % 8 or sh % 8 or sn % 8 or t.data_ptr() % 16) else t.contiguous()
-
-
-def _strides(t):
-    sb, sh, sn, _ = t.stride()
-    return _U64x3(sb, sn, sh)
-
-
-class _AttentionFn(torch.autograd.Function):
-    """csrc/attention_train.hip. The scratch is allocated per call: calls on several streams, or graphs replayed at once, share none."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, key_mask, causal, scale, keep):
-        import _sdfx as S
-        (B, H, Nq, d), (_, Hk, Nk, _) = q.shape, k.shape
-        with S.on_device(q):
-            o = torch.empty(B, Nq, H * d, dtype=q.dtype, device=q.device)
-            o_lo = torch.empty_like(o) if keep else None
-            lse = torch.empty(B, H, Nq, dtype=torch.float32, device=q.device) if keep else None
-            nbytes = int(S.lib().sdfx_attention_train_scratch_bytes(B, H, Hk, Nq, Nk, d, 0))
-            scratch = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device) if nbytes else None
-            S.call("sdfx_attention_train_forward", S.ptr(q), S.ptr(k), S.ptr(v), S.ptr(key_mask), B, H, Hk, Nq, Nk, d, _strides(q), _strides(k),
-                   _strides(v), scale, causal, int(q.dtype == torch.bfloat16), S.ptr(o), S.ptr(o_lo), S.ptr(lse), S.ptr(scratch), S.stream())
-        if keep:
-            ctx.save_for_backward(q, k, v, key_mask, o, o_lo, lse)
-            ctx.args = (causal, scale)
-        return o
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        import _sdfx as S
-        q, k, v, key_mask, o, o_lo, lse = ctx.saved_tensors
-        causal, scale = ctx.args
-        (B, H, Nq, d), (_, Hk, Nk, _) = q.shape, k.shape
-        with S.on_device(q):
-            dy = dy.contiguous()
-            dy = dy if dy.data_ptr() % 16 == 0 else dy.clone()
-            new = lambda n, h: torch.empty(B, n, h, d, dtype=q.dtype, device=q.device)
-            dq = new(Nq, H) if ctx.needs_input_grad[0] else None
-            dk, dv = (new(Nk, Hk), new(Nk, Hk)) if ctx.needs_input_grad[1] or ctx.needs_input_grad[2] else (None, None)
-            nbytes = int(S.lib().sdfx_attention_train_scratch_bytes(B, H, Hk, Nq, Nk, d, 1))
-            scratch = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device)
-            S.call("sdfx_attention_train_backward", S.ptr(q), S.ptr(k), S.ptr(v), S.ptr(key_mask), S.ptr(o), S.ptr(o_lo), S.ptr(lse), S.ptr(dy), B, H,
-                   Hk, Nq, Nk, d, _strides(q), _strides(k), _strides(v), scale, causal, int(q.dtype == torch.bfloat16), S.ptr(dq), S.ptr(dk),
-                   S.ptr(dv), S.ptr(scratch), S.stream())
-        view = lambda t: None if t is None else t.transpose(1, 2)
-        return view(dq), view(dk), view(dv), None, None, None, None
 
 
 def _attention_plain(q, k, v, key_mask, causal, scale):
@@ -157,5 +101,4 @@ def attention(q, k, v, key_mask=None, causal=False, scale=None):
         return (q.sum() + k.sum() + v.sum()) * 0 + torch.zeros(B, Nq, H * d, dtype=q.dtype, device=q.device)
     if not (q.is_cuda and q.dtype in (torch.float16, torch.bfloat16) and d % 8 == 0 and d <= 256):
         return _attention_plain(q, k, v, key_mask, causal, scale)
-    keep = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
-    return _AttentionFn.apply(_taken(q), _taken(k), _taken(v), None if key_mask is None else key_mask.contiguous(), int(bool(causal)), scale, keep)
+    return _sdfx.native().attention(q, k, v, key_mask, causal, scale)

@@ -86,7 +86,7 @@ def add_bias_residual(a, b, bias):
 
 
 # ---- training forms ---------------------------------------------------------------------------------------------------------------
-_DTYPE = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_KERNEL_TYPES = (torch.float16, torch.bfloat16, torch.float32)
 _CHECKPOINTS = ("full", "int8")
 
 
@@ -108,51 +108,6 @@ def _check_checkpoint(checkpoint, channels, what):
         raise ValueError(f"{what}: checkpoint must be one of {_CHECKPOINTS}, got {checkpoint!r}")
     if checkpoint == "int8" and channels % 32:
         raise ValueError(f"{what}: the 8-bit checkpoint needs a multiple of 32 channels (got {channels})")
-
-
-def _dense16(t):
-    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.preserve_format)
-
-
-class _GroupNormTrainFn(torch.autograd.Function):
-    """csrc/groupnorm_train.hip. The scratch is allocated per call: calls on several streams, or graphs replayed at once, share none."""
-
-    @staticmethod
-    def forward(ctx, x, pre, weight, bias, groups, eps, act, eight, keep):
-        import _sdfx as S
-        N, C, H, W = x.shape
-        with S.on_device(x):
-            y = torch.empty_like(x)                        # (dense NHWC: the strides are kept)
-            nbytes = int(S.lib().sdfx_group_norm_train_scratch_bytes(N, H * W, C, groups))
-            mean_rstd = torch.empty(N * groups * 2, dtype=torch.float32, device=x.device)
-            scratch = torch.empty((nbytes + 7) // 8, dtype=torch.float64, device=x.device)
-            saved = torch.empty(x.numel() + x.numel() // 32, dtype=torch.uint8, device=x.device) if eight and keep else None
-            f32 = int(weight.dtype == torch.float32)
-            S.call("sdfx_group_norm_train_forward", S.ptr(x), S.ptr(pre), S.ptr(weight), S.ptr(bias), N, H * W, C, groups, eps, act, _DTYPE[x.dtype],
-                   f32, S.ptr(y), S.ptr(saved), S.ptr(mean_rstd), S.ptr(scratch), S.stream())
-        if keep:
-            ctx.save_for_backward(x if saved is None else saved, pre, weight, bias, mean_rstd)
-            ctx.args = (x.shape, groups, act, saved is not None, x.dtype, f32)
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        import _sdfx as S
-        x, pre, weight, bias, mean_rstd = ctx.saved_tensors
-        (N, C, H, W), groups, act, eight, dtype, f32 = ctx.args
-        want = ctx.needs_input_grad
-        with S.on_device(x):
-            dy = _dense16(dy.contiguous(memory_format=torch.channels_last))
-            nbytes = int(S.lib().sdfx_group_norm_train_scratch_bytes(N, H * W, C, groups))
-            scratch = torch.empty((nbytes + 7) // 8, dtype=torch.float64, device=x.device)
-            dx = torch.empty_like(dy) if want[0] else None
-            dpre = torch.empty_like(pre) if pre is not None and want[1] else None
-            dw = torch.empty_like(weight) if want[2] else None
-            db = torch.empty_like(bias) if want[3] else None
-            S.call("sdfx_group_norm_train_backward", S.ptr(x), int(eight), S.ptr(pre), S.ptr(dy), S.ptr(weight), S.ptr(bias), S.ptr(mean_rstd), N,
-                   H * W, C, groups, act, _DTYPE[dtype], f32, S.ptr(dx), S.ptr(dpre), S.ptr(dw), S.ptr(db), S.ptr(scratch), S.stream())
-        return dx, dpre, dw, db, None, None, None, None, None
 
 
 class _GroupNormPlainFn(torch.autograd.Function):
@@ -218,39 +173,10 @@ def group_norm_act(x, groups, weight, bias, eps=1e-5, act=True, pre=None, checkp
     _check_checkpoint(checkpoint, C, "group_norm_act")
     if x.numel() == 0:
         return x + (weight.sum() + bias.sum()).to(x.dtype) * 0 + (0 if pre is None else pre[:, :, None, None] * 0)
+    if x.is_cuda and x.dtype in _KERNEL_TYPES and C % 8 == 0 and C <= 2560 and groups <= 64 and H * W < 2 ** 31:
+        return _S.native().group_norm(x, pre, weight, bias, groups, eps, act, checkpoint == "int8")
     keep = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or bias.requires_grad or (pre is not None and pre.requires_grad))
-    args = (int(groups), float(eps), int(bool(act)), checkpoint == "int8", keep)
-    if x.is_cuda and x.dtype in _DTYPE and C % 8 == 0 and C <= 2560 and groups <= 64 and H * W < 2 ** 31:
-        x = _dense16(x.contiguous(memory_format=torch.channels_last))
-        return _GroupNormTrainFn.apply(x, None if pre is None else pre.contiguous(), weight.contiguous(), bias.contiguous(), *args)
-    return _GroupNormPlainFn.apply(x, pre, weight, bias, *args)
-
-
-class _GegluTrainFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, eight, keep):
-        import _sdfx as S
-        n = x.shape[-1] // 2
-        with S.on_device(x):
-            y = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
-            saved = torch.empty(x.numel() + x.numel() // 32, dtype=torch.uint8, device=x.device) if eight and keep else None
-            S.call("sdfx_geglu_train_forward", S.ptr(x), x.numel() // (2 * n), n, _DTYPE[x.dtype], S.ptr(y), S.ptr(saved), S.stream())
-        if keep:
-            ctx.save_for_backward(x if saved is None else saved)
-            ctx.args = (x.shape, saved is not None, x.dtype)
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        import _sdfx as S
-        (x,), (shape, eight, dtype) = ctx.saved_tensors, ctx.args
-        with S.on_device(x):
-            dy = _dense16(dy.contiguous())
-            dx = torch.empty(shape, dtype=dtype, device=x.device)
-            S.call("sdfx_geglu_train_backward", S.ptr(x), int(eight), S.ptr(dy), dx.numel() // shape[-1], shape[-1] // 2, _DTYPE[dtype], S.ptr(dx),
-                   S.stream())
-        return dx, None, None
+    return _GroupNormPlainFn.apply(x, pre, weight, bias, groups, eps, act, checkpoint == "int8", keep)
 
 
 class _GegluPlainFn(torch.autograd.Function):
@@ -287,10 +213,9 @@ def geglu(x, checkpoint=None):
         if x.dim() == 0 or x.shape[-1] % 2 or x.shape[-1] == 0 or not x.is_floating_point():
             raise ValueError(f"geglu: x must be a floating-point tensor with an even last dimension, got {x.dtype} {tuple(x.shape)}")
         _check_checkpoint(checkpoint, n, "geglu")
-        keep = torch.is_grad_enabled() and x.requires_grad
-        if x.is_cuda and x.dtype in _DTYPE and n % 8 == 0:
-            return _GegluTrainFn.apply(_dense16(x.contiguous()), checkpoint == "int8", keep)
-        return _GegluPlainFn.apply(x, checkpoint == "int8", keep)
+        if x.is_cuda and x.dtype in _KERNEL_TYPES and n % 8 == 0:
+            return _S.native().geglu(x, checkpoint == "int8")
+        return _GegluPlainFn.apply(x, checkpoint == "int8", torch.is_grad_enabled() and x.requires_grad)
     if (_FUSED and x.is_cuda and x.dtype == torch.float16 and not (x.requires_grad and torch.is_grad_enabled()) and x.is_contiguous()
             and x.shape[-1] % 16 == 0 and x.data_ptr() % 16 == 0):
         import _sdfx as S
