@@ -108,13 +108,13 @@ template <typename L> __device__ __forceinline__ void request(u4v (&r)[L::PT], c
         if (ch * 8u < D) r[i] = *reinterpret_cast<const u4v*>(static_cast<const uint16_t*>(p) + (size_t)at * sn + ch * 8u);
     }
 }
-// ... and into LDS; rows whose bit of `live` is clear as zeros (a masked key's values may be anything: 0 * NaN must not reach a product)
-template <typename L> __device__ __forceinline__ void stash(uint8_t* tile, const u4v (&r)[L::PT], uint64_t live, uint32_t tid, uint32_t th) {
+// ... and (the first `chunks` of each row) into LDS; rows whose bit of `live` is clear as zeros (a masked key's values may be anything: 0 * NaN must not reach a product)
+template <typename L> __device__ __forceinline__ void stash(uint8_t* tile, const u4v (&r)[L::PT], uint64_t live, uint32_t tid, uint32_t th,
+                                                                      uint32_t chunks = L::CH) {
 #pragma unroll
     for (int i = 0; i < L::PT; i++) {
-        const uint32_t c = tid + (uint32_t)i * th;
-        if (c < (uint32_t)L::NCH) {
-            const uint32_t row = c / L::CH, ch = c - row * L::CH;
+        const uint32_t c = tid + (uint32_t)i * th, row = c / L::CH, ch = c - row * L::CH;
+        if (c < (uint32_t)L::NCH && ch < chunks) {
             const bool on = (live >> row) & 1u;
             *reinterpret_cast<u4v*>(tile + row * L::PITCH + ch * 16u) = on ? r[i] : u4v{0u, 0u, 0u, 0u};
         }
@@ -165,7 +165,7 @@ __device__ __forceinline__ float grad_scale(const float* rows2, uint32_t nr, con
     const uint32_t e = __float_as_uint(m) >> 23;
     return __uint_as_float((252u - min(e, 251u)) << 23);
 }
-constexpr uint32_t kPrepRows = 64;         // rows per workgroup of k_prep = rows per entry of the maxima
+constexpr uint32_t kPrepRows = 32;         // rows per workgroup of k_prep = rows per entry of the maxima
 __host__ __device__ inline uint32_t prep_blocks(uint32_t n) { return (n + kPrepRows - 1) / kPrepRows; }
 
 // what the backward's kernels get beside the shape
@@ -179,10 +179,12 @@ constexpr int kWidths[] = {48, 64, 80, 128, 160, 256};      // channels a kernel
 
 // attention_train_dq.hip, attention_train_dkdv.hip: launch (shape's tiles_x / splits / per_split set for `waves` a workgroup)
 void launch_dq(const BwdArgs& a, const Shape& s, int bf16, int waves, hipStream_t st);
-void launch_dkdv(const BwdArgs& a, const Shape& s, int bf16, int waves, hipStream_t st);
-// rows of the tile each stages: keys (forward, dq) or queries (dk / dv)
-constexpr int key_tile(int dp) { return dp <= 128 ? 64 : 32; }
-constexpr int query_tile(int dp) { return dp <= 80 ? 64 : 32; }
+void launch_dkdv(const BwdArgs& a, const Shape& s, int bf16, hipStream_t st);
+// rows of the tile each stages: keys (forward, dq) or queries (dk / dv). One wave alone takes 32 and needs one buffer: its next tile waits in
+// registers until it is done with the last (17 KB of LDS at 128 channels: eight such workgroups a CU).
+constexpr int key_tile(int dp, int nw) { return dp <= 128 && nw == 4 ? 64 : 32; }
+constexpr int buffers(int nw) { return nw == 4 ? 2 : 1; }
+constexpr int query_tile(int dm) { return dm <= 80 ? 64 : 32; }
 inline int padded(uint32_t D) {
     for (int w : kWidths)
         if (D <= (uint32_t)w) return w;
@@ -200,13 +202,11 @@ inline int padded(uint32_t D) {
             default: fn<T, 256, nw>(__VA_ARGS__); break;                  \
         }                                                                 \
     } while (0)
-#define SDFX_ATTN_DISPATCH(fn, ...)                                       \
-    do {                                                                  \
-        if (bf16 && waves == 4) SDFX_ATTN_WIDTH(fn, __bf16, 4, __VA_ARGS__);        \
-        else if (bf16) SDFX_ATTN_WIDTH(fn, __bf16, 1, __VA_ARGS__);                 \
-        else if (waves == 4) SDFX_ATTN_WIDTH(fn, _Float16, 4, __VA_ARGS__);         \
-        else SDFX_ATTN_WIDTH(fn, _Float16, 1, __VA_ARGS__);                         \
-    } while (0)
+
+// In front of a rarely needed block of selects (5 instructions a score): keeps it a branch, which the compiler would otherwise fold into straight code
+__device__ __forceinline__ void keep_branch() { asm volatile(""); }
+// operands of the second products requested ahead of the exponentials: where a lane's registers hold them
+constexpr bool ahead(int dp) { return dp <= 64; }
 
 // the row a lane owns in the forward and in dq
 struct Row {

@@ -14,12 +14,12 @@ template <typename T, int DP, int NW>
 __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_fwd(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
                                                    T* __restrict__ o, T* __restrict__ o_lo, float* __restrict__ lse, float* __restrict__ part,
                                                    float* __restrict__ part_ml, Shape s) {
-    constexpr int KT = key_tile(DP), KS = DP / 16, DT = (DP + 31) / 32, NB = KT / 32;
+    constexpr int KT = key_tile(DP, NW), NBUF = buffers(NW), KS = DP / 16, DT = (DP + 31) / 32, NB = KT / 32;
     typedef Tile<DP, KT, 64 * NW> L;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[4 * L::BYTES + kTileSlack];
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * NBUF * L::BYTES + kTileSlack];
     uint8_t* const ldsK = lds;
-    uint8_t* const ldsV = lds + 2 * L::BYTES;
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, x = lane & 31u, hi = lane >> 5;
+    uint8_t* const ldsV = lds + NBUF * L::BYTES;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), x = lane & 31u, hi = lane >> 5;
     const uint32_t per_bh = s.tiles_x * s.splits;
     const uint32_t lid = xcd_contiguous(blockIdx.x, per_bh * s.B * s.Hk);
     const uint32_t bh = lid / per_bh, rest = lid - bh * per_bh, split = rest / s.tiles_x, xt = rest - split * s.tiles_x;
@@ -57,7 +57,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_fwd(const T* __re
         stash<L>(ldsV, rv, live, tid, 64 * NW);
         __syncthreads();
         for (uint32_t j = t0; j < t1; j++) {
-            const uint32_t buf = (j - t0) & 1u;
+            const uint32_t buf = (j - t0) % NBUF, nbuf = (j + 1 - t0) % NBUF;
             uint8_t next_byte = 0;
             if (j + 1 < t1) {
                 request<L>(rk, kb, s.k_sn, (j + 1) * KT, s.Nk, s.D, tid, 64 * NW);
@@ -75,45 +75,57 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_fwd(const T* __re
                     for (int ks = 0; ks < KS; ks++) sc[st] = mma(row_operand<T, L>(kt, st, ks, x, hi), qf[ks], sc[st]);
                 }
                 if (live != all_keys<KT>() || (int)(j * KT + KT - 1) > wave_lo) {
+                    keep_branch();
 #pragma unroll
                     for (int st = 0; st < NB; st++) hide(sc[st], live, row.lim, j * KT, st, hi);
+                }
+                // the value operands, requested ahead of the softmax (the compiler would read each in front of its product and wait)
+                typename Half<T>::v8 vo[2 * NB][DT];
+                if (ahead(DP)) {
+#pragma unroll
+                    for (int e = 0; e < 2 * NB; e++)
+#pragma unroll
+                        for (int dt = 0; dt < DT; dt++) vo[e][dt] = col_operand<T, L>(vt, e, dt, lane);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
                 float mx = -INFINITY;
 #pragma unroll
                 for (int st = 0; st < NB; st++)
 #pragma unroll
                     for (int r = 0; r < 16; r++) mx = fmaxf(mx, sc[st][r]);
-                mx = max_halves(mx);
-                const float m_new = fmaxf(m_run, mx * s.c);
-                const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
-                m_run = m_new;
+                mx = max_halves(mx) * s.c;
+                if (__ballot(mx > m_run)) {               // (some row has a new maximum: rare after the first tiles)
+                    const float m_new = fmaxf(m_run, mx), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+                    m_run = m_new;
+                    l_run *= alpha;
+#pragma unroll
+                    for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                        for (int r = 0; r < 16; r++) acc[dt][r] *= alpha;
+                }
                 float sum0 = 0.f, sum1 = 0.f;
-                typename Half<T>::v8 pf[2 * NB];
 #pragma unroll
                 for (int st = 0; st < NB; st++) {
 #pragma unroll
                     for (int r = 0; r < 16; r += 2) {
-                        sc[st][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[st][r], s.c, -m_new));
-                        sc[st][r + 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[st][r + 1], s.c, -m_new));
+                        sc[st][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[st][r], s.c, -m_run));
+                        sc[st][r + 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[st][r + 1], s.c, -m_run));
                         sum0 += sc[st][r]; sum1 += sc[st][r + 1];
                     }
-                    pf[2 * st] = operand<T>(sc[st], 0);          // (the probabilities' rounding: half a unit of each, as the inputs')
-                    pf[2 * st + 1] = operand<T>(sc[st], 1);
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const typename Half<T>::v8 pf = operand<T>(sc[st], e);          // (the probabilities' rounding: half a unit of each, as the inputs')
+#pragma unroll
+                        for (int dt = 0; dt < DT; dt++) acc[dt] = mma(ahead(DP) ? vo[2 * st + e][dt] : col_operand<T, L>(vt, 2 * st + e, dt, lane), pf, acc[dt]);
+                    }
                 }
-                l_run = __builtin_fmaf(l_run, alpha, sum0 + sum1);
-#pragma unroll
-                for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-                    for (int r = 0; r < 16; r++) acc[dt][r] *= alpha;
-#pragma unroll
-                for (int e = 0; e < 2 * NB; e++)
-#pragma unroll
-                    for (int dt = 0; dt < DT; dt++) acc[dt] = mma(col_operand<T, L>(vt, e, dt, lane), pf[e], acc[dt]);
+                l_run += sum0 + sum1;
             }
+            if (NBUF == 1) __syncthreads();
             if (j + 1 < t1) {
                 live = live_keys<KT>(s, next_byte, j + 1, lane);
-                stash<L>(ldsK + (buf ^ 1u) * L::BYTES, rk, live, tid, 64 * NW);
-                stash<L>(ldsV + (buf ^ 1u) * L::BYTES, rv, live, tid, 64 * NW);
+                stash<L>(ldsK + nbuf * L::BYTES, rk, live, tid, 64 * NW);
+                stash<L>(ldsV + nbuf * L::BYTES, rv, live, tid, 64 * NW);
             }
             __syncthreads();
         }
@@ -153,30 +165,38 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_fwd(const T* __re
         }
 }
 
-// o of the splits of each row: thread per (row, 4 channels)
+// o of the splits of each row: D / 4 channel quads x `parts` ranges of the splits are the threads of a row, the ranges added in order through LDS
 template <typename T>
-__global__ __launch_bounds__(256) void k_join_o(const float* __restrict__ part, const float* __restrict__ ml, Shape s, T* __restrict__ o,
+__global__ __launch_bounds__(256) void k_join_o(const float* __restrict__ part, const float* __restrict__ ml, Shape s, uint32_t parts, T* __restrict__ o,
                                                T* __restrict__ o_lo, float* __restrict__ lse) {
-    const uint32_t per = s.D / 4;
+    __shared__ f4 red[256];
+    __shared__ float redl[256];
+    const uint32_t quads = s.D / 4, per = quads * parts, rows_here = 256u / per;
     const uint64_t total = (uint64_t)s.B * s.H * s.Nq;
-    const uint64_t id = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    if (id >= total * per) return;
-    const uint64_t r = id / per;
-    const uint32_t c0 = (uint32_t)(id - r * per) * 4;
-    float m = -1e30f;
-    for (uint32_t i = 0; i < s.splits; i++) m = fmaxf(m, ml[2 * (i * total + r)]);
-    float l = 0.f;
+    const uint32_t local = threadIdx.x / per, in_row = threadIdx.x - local * per, pt = in_row / quads, c0 = (in_row - pt * quads) * 4;
+    const uint64_t r = (uint64_t)blockIdx.x * rows_here + local;
+    const bool on = local < rows_here && r < total;
+    float m = -1e30f, l = 0.f;
     f4 a = {0.f, 0.f, 0.f, 0.f};
-    for (uint32_t i = 0; i < s.splits; i++) {
-        const uint64_t at = i * total + r;
-        const float li = ml[2 * at + 1];
-        if (li == 0.f) continue;                      // nothing seen in this range
-        const float w = __builtin_amdgcn_exp2f(ml[2 * at] - m);
-        const f4 p = *reinterpret_cast<const f4*>(part + at * s.D + c0);
-        l = __builtin_fmaf(w, li, l);
+    if (on) {
+#pragma unroll 8
+        for (uint32_t i = 0; i < s.splits; i++) m = fmaxf(m, ml[2 * (i * total + r)]);
+        const uint32_t n = (s.splits + parts - 1) / parts, i1 = min((pt + 1) * n, s.splits);
+#pragma unroll 4
+        for (uint32_t i = pt * n; i < i1; i++) {
+            const uint64_t at = i * total + r;
+            const float li = ml[2 * at + 1], w = li == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml[2 * at] - m);      // (0: nothing seen in this range)
+            const f4 p = *reinterpret_cast<const f4*>(part + at * s.D + c0);
+            l = __builtin_fmaf(w, li, l);
 #pragma unroll
-        for (int j = 0; j < 4; j++) a[j] = __builtin_fmaf(w, p[j], a[j]);
+            for (int j = 0; j < 4; j++) a[j] = __builtin_fmaf(w, p[j], a[j]);
+        }
     }
+    red[threadIdx.x] = a;
+    redl[threadIdx.x] = l;
+    __syncthreads();
+    if (!on || pt) return;
+    for (uint32_t i = 1; i < parts; i++) { a += red[threadIdx.x + i * quads]; l += redl[threadIdx.x + i * quads]; }
     const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
     const uint32_t bh = (uint32_t)(r / s.Nq), qi = (uint32_t)(r - (uint64_t)bh * s.Nq), b = bh / s.H, h = bh - b * s.H;
     const size_t at = (((size_t)b * s.Nq + qi) * s.H + h) * s.D + c0;
@@ -218,7 +238,10 @@ __global__ __launch_bounds__(256) void k_prep(const T* __restrict__ v, const T* 
     const uint32_t lr = threadIdx.x % LR, c0 = lr * 8u;
     const uint32_t n = of_v ? s.Nk : s.rows, end = min((blk + 1) * kPrepRows, n);
     float most = 0.f;
-    for (uint32_t r = blk * kPrepRows + threadIdx.x / LR; r < end; r += 256 / LR) {
+#pragma unroll
+    for (uint32_t i = 0; i < (kPrepRows * LR + 255) / 256; i++) {
+        const uint32_t r = blk * kPrepRows + threadIdx.x / LR + i * (256 / LR);
+        if (r >= end) continue;
         float d = 0.f, q = 0.f;
         size_t at = 0;
         if (of_v) {
@@ -256,31 +279,43 @@ __global__ __launch_bounds__(256) void k_prep(const T* __restrict__ v, const T* 
 }
 
 // ---- launches -----------------------------------------------------------------------------------------------------------------------
-// Workgroups: 4 waves share a tile where that leaves every CU one or more; else one wave each. Then the other axis is split until
-// about two workgroups a CU run, two tiles each at least.
+// Workgroups of 4 waves share their tiles; 32 rows or fewer (a few queries against a long cache) take one wave each. Where that leaves CUs
+// without work the other axis is split, at least `least` tiles to a workgroup: a split costs float32 partials and a launch that adds them.
 constexpr uint32_t kCus = 256;
-void plan(Shape& s, uint32_t along, uint32_t other_tiles, int& waves) {
-    const uint64_t heads = (uint64_t)s.B * s.Hk;
-    waves = (uint64_t)div_up(along, 128) * heads >= kCus || along > 1024 ? 4 : 1;
+void plan(Shape& s, uint32_t along, uint32_t other_tiles, int waves, uint32_t least) {
     s.tiles_x = div_up(along, 32u * waves);
-    const uint64_t base = s.tiles_x * heads;
-    uint64_t splits = base >= kCus ? 1 : (2 * kCus + base - 1) / base;
-    const uint64_t most = other_tiles / 2 ? other_tiles / 2 : 1;
+    const uint64_t base = (uint64_t)s.tiles_x * s.B * s.Hk, want = waves == 4 ? 2 * kCus : 8 * kCus;
+    uint64_t splits = 2 * base >= want ? 1 : (want + base - 1) / base;
+    const uint64_t most = other_tiles / least ? other_tiles / least : 1;
     if (splits > most) splits = most;
     s.per_split = div_up(other_tiles, splits);
     s.splits = div_up(other_tiles, s.per_split);
 }
-void plan_fwd(Shape& s, int& waves) { plan(s, s.rows, div_up(s.Nk, key_tile(padded(s.D))), waves); }
-void plan_dkdv(Shape& s, int& waves) { plan(s, s.Nk, s.group * div_up(s.Nq, query_tile(padded(s.D))), waves); }
+void plan_rows(Shape& s, int& waves) {          // forward, dq
+    const int dp = padded(s.D);
+    waves = s.rows <= 32 && dp <= 160 ? 1 : 4;
+    plan(s, s.rows, div_up(s.Nk, key_tile(dp, waves)), waves, 4);
+}
+void plan_keys(Shape& s) { plan(s, s.Nk, s.group * div_up(s.Nq, query_tile((int)s.D)), 4, 4); }
 
 template <typename T, int DP, int NW>
 void launch_fwd(const void* q, const void* k, const void* v, void* o, void* o_lo, float* lse, float* part, float* ml, const Shape& s, hipStream_t st) {
     hipLaunchKernelGGL((k_fwd<T, DP, NW>), dim3(s.tiles_x * s.splits * s.B * s.Hk), dim3(64 * NW), 0, st, static_cast<const T*>(q), static_cast<const T*>(k),
                        static_cast<const T*>(v), static_cast<T*>(o), static_cast<T*>(o_lo), lse, part, ml, s);
 }
+// (one wave alone: head widths up to 160; see plan_rows)
+template <typename T, int DP, int NW>
+void launch_one(const void* q, const void* k, const void* v, void* o, void* o_lo, float* lse, float* part, float* ml, const Shape& s, hipStream_t st) {
+    launch_fwd<T, DP < 160 ? DP : 160, NW>(q, k, v, o, o_lo, lse, part, ml, s, st);
+}
 template <typename T> void join_o(const float* part, const float* ml, const Shape& s, void* o, void* o_lo, float* lse, hipStream_t st) {
-    const uint64_t n = (uint64_t)s.B * s.H * s.Nq * (s.D / 4);
-    hipLaunchKernelGGL(k_join_o<T>, dim3((uint32_t)((n + 255) / 256)), dim3(256), 0, st, part, ml, s, static_cast<T*>(o), static_cast<T*>(o_lo), lse);
+    const uint32_t quads = s.D / 4;
+    uint32_t parts = 256 / quads, most = (s.splits + 3) / 4;               // four splits to a thread
+    if (parts > most) parts = most;
+    const uint32_t rows_here = 256 / (quads * parts);
+    const uint64_t n = (uint64_t)s.B * s.H * s.Nq;
+    hipLaunchKernelGGL(k_join_o<T>, dim3((uint32_t)((n + rows_here - 1) / rows_here)), dim3(256), 0, st, part, ml, s, parts, static_cast<T*>(o),
+                       static_cast<T*>(o_lo), lse);
 }
 template <typename T>
 void join_sum(const float* pa, const float* pb, uint32_t splits, uint32_t B, uint32_t H, uint32_t N, uint32_t D, void* oa, void* ob, hipStream_t st) {
@@ -329,9 +364,9 @@ uint64_t up16(uint64_t floats) { return (floats + 3) / 4 * 4; }
 struct BwdLayout { uint64_t rows2, v2, pq, pk, pv, total; };   // float offsets behind delta
 BwdLayout bwd_layout(const Shape& s0) {
     Shape a = s0, b = s0;
-    int wa, wb;
-    plan_fwd(a, wa);
-    plan_dkdv(b, wb);
+    int waves;
+    plan_rows(a, waves);
+    plan_keys(b);
     const uint64_t heads = (uint64_t)s0.B * s0.Hk;
     BwdLayout l;
     l.rows2 = up16(heads * s0.rows);
@@ -354,7 +389,7 @@ uint64_t sdfx_attention_train_scratch_bytes(uint32_t B, uint32_t H, uint32_t Hk,
     fill(s, B, H, Hk, Nq, Nk, D);
     if (backward) return bwd_layout(s).total * 4;
     int waves;
-    plan_fwd(s, waves);
+    plan_rows(s, waves);
     return s.splits > 1 ? ((uint64_t)s.splits * B * s.Hk * s.rows * (D + 2)) * 4 : 0;
 }
 
@@ -372,11 +407,14 @@ int sdfx_attention_train_forward(const void* q, const void* k, const void* v, co
     fill(s, B, H, Hk, Nq, Nk, D);
     fill_call(s, q_strides, k_strides, v_strides, key_mask, scale, causal);
     int waves;
-    plan_fwd(s, waves);
+    plan_rows(s, waves);
     SDFX_REQUIRE(s.splits == 1 || scratch, "attention_train_forward: this shape needs scratch");
     float* ml = s.splits > 1 ? scratch + (uint64_t)s.splits * B * s.Hk * s.rows * D : nullptr;
     hipStream_t st = as_stream(stream);
-    SDFX_ATTN_DISPATCH(launch_fwd, q, k, v, o, o_lo, lse, scratch, ml, s, st);
+    if (bf16 && waves == 4) SDFX_ATTN_WIDTH(launch_fwd, __bf16, 4, q, k, v, o, o_lo, lse, scratch, ml, s, st);
+    else if (bf16) SDFX_ATTN_WIDTH(launch_one, __bf16, 1, q, k, v, o, o_lo, lse, scratch, ml, s, st);
+    else if (waves == 4) SDFX_ATTN_WIDTH(launch_fwd, _Float16, 4, q, k, v, o, o_lo, lse, scratch, ml, s, st);
+    else SDFX_ATTN_WIDTH(launch_one, _Float16, 1, q, k, v, o, o_lo, lse, scratch, ml, s, st);
     if (s.splits > 1) {
         if (bf16) join_o<__bf16>(scratch, ml, s, o, o_lo, lse, st);
         else join_o<_Float16>(scratch, ml, s, o, o_lo, lse, st);
@@ -410,10 +448,9 @@ int sdfx_attention_train_backward(const void* q, const void* k, const void* v, c
     else prep<_Float16>(v, o, o_lo, dy, lse, s, scratch, scratch + l.rows2, scratch + l.v2, st);
     if (dk) {
         Shape t = s;
-        int waves;
-        plan_dkdv(t, waves);
+        plan_keys(t);
         a.part = scratch + l.pk; a.part2 = scratch + l.pv;
-        launch_dkdv(a, t, bf16, waves, st);
+        launch_dkdv(a, t, bf16, st);
         if (t.splits > 1) {
             if (bf16) join_sum<__bf16>(a.part, a.part2, t.splits, B, Hk, Nk, D, dk, dv, st);
             else join_sum<_Float16>(a.part, a.part2, t.splits, B, Hk, Nk, D, dk, dv, st);
@@ -422,7 +459,7 @@ int sdfx_attention_train_backward(const void* q, const void* k, const void* v, c
     if (dq) {
         Shape t = s;
         int waves;
-        plan_fwd(t, waves);
+        plan_rows(t, waves);
         a.part = scratch + l.pq; a.part2 = nullptr;
         launch_dq(a, t, bf16, waves, st);
         if (t.splits > 1) {

@@ -1,41 +1,79 @@
 // attention_train_dkdv.hip — dk = scale ds^T q and dv = p^T dy of attention's gradient (attention_train.h). A wave owns 32 keys: k and v in
-// registers, tiles of queries (q, dy, their log-sum-exp and delta) shared by the workgroup's waves in LDS, double-buffered, over every
-// query head that shares the key head. Per 32 queries: s = q k^T, dp = dy v^T, p, ds, then dv^T += dy^T p, dk^T += q^T ds. A masked key
-// touches nothing but its own lane, whose result is written as zero.
+// registers, tiles of queries (q and dy) shared by the workgroup's waves in LDS, double-buffered, over every query head that shares the key
+// head. Per 32 queries: s = q k^T, dp = dy v^T, p, ds, then dv^T += dy^T p, dk^T += q^T ds. A masked key touches nothing but its own lane,
+// whose result is written as zero.
+// A lane's 16 scores belong to 16 queries, so their log-sum-exps and deltas cannot be lane scalars as in dq. Read from LDS they would take
+// as many cycles there as the operands (8 of 30 reads a block); instead they ride in the products: a row carries 8 extra channels, q's
+// with (shift - lse) / c and dy's with -delta as sums of 16-bit parts, k's and v's with the parts' weights, powers of two. s and dp come out
+// of the matrix cores complete. Parts: two of fp16 or three of bf16, 22 to 24 bits.
 #include "attention_train.h"
 
 namespace sdfx_attn {
 namespace {
 
-template <typename T, int DP, int NW>
-__global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape s) {
-    constexpr int QT = query_tile(DP), KS = DP / 16, DT = (DP + 31) / 32, NB = QT / 32;
+// The extra channels: part i of a value is rounded at weight w 2^(-step i), the rest goes to part i + 1.
+template <typename T> struct Parts;
+template <> struct Parts<_Float16> { static constexpr int N = 2, STEP = 11; };
+template <> struct Parts<__bf16> { static constexpr int N = 3, STEP = 8; };
+template <typename T> __device__ __forceinline__ u4v split_parts(float v, float w) {       // v = sum of parts * (w 2^(-STEP i)), w a power of two
+    typename Half<T>::v8 o = {};
+    float rest = v * (1.f / w);
+#pragma unroll
+    for (int i = 0; i < Parts<T>::N; i++) {
+        o[i] = (T)rest;
+        rest = i == 0 && !(__builtin_fabsf(rest) < INFINITY) ? 0.f : (rest - (float)o[i]) * (float)(1 << Parts<T>::STEP);
+    }
+    return __builtin_bit_cast(u4v, o);
+}
+template <typename T> __device__ __forceinline__ u4v part_weights(float w) {
+    typename Half<T>::v8 o = {};
+#pragma unroll
+    for (int i = 0; i < Parts<T>::N; i++) { o[i] = (T)w; w *= 1.f / (float)(1 << Parts<T>::STEP); }
+    return __builtin_bit_cast(u4v, o);
+}
+
+// CS: workgroups that share a key tile's output channels (2 at 256 channels, where dk and dv of 32 keys and the operands would fill the register file)
+template <typename T, int DM, int CS>
+__global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape s) {
+    constexpr int NW = 4, DP = (DM + 8 + 15) / 16 * 16;                  // channels with the extra ones, in whole K steps
+    constexpr int QT = query_tile(DM), KS = DP / 16, DT = (DM + 31) / 32 / CS, NB = QT / 32;
     typedef Tile<DP, QT, 64 * NW> L;
     __shared__ __attribute__((aligned(16))) uint8_t lds[4 * L::BYTES + kTileSlack];
-    __shared__ __attribute__((aligned(16))) float stat[2][2][QT];       // [buffer][shift - lse, -delta g][query]
     uint8_t* const ldsY = lds;
     uint8_t* const ldsQ = lds + 2 * L::BYTES;
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, x = lane & 31u, hi = lane >> 5;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), x = lane & 31u, hi = lane >> 5;
     const uint32_t per_bh = s.tiles_x * s.splits;
-    const uint32_t lid = xcd_contiguous(blockIdx.x, per_bh * s.B * s.Hk);
+    const uint32_t all = xcd_contiguous(blockIdx.x, per_bh * s.B * s.Hk * CS), lid = all / CS, dt0 = (all - lid * CS) * DT;
     const uint32_t bh = lid / per_bh, rest = lid - bh * per_bh, split = rest / s.tiles_x, xt = rest - split * s.tiles_x;
     const uint32_t b = bh / s.Hk, hk = bh - b * s.Hk;
     const uint32_t wg_key = xt * NW * 32u, w0 = wg_key + wave * 32u, key = w0 + x, kc = min(key, s.Nk - 1u);
     const bool seen = key < s.Nk && (!s.mask || s.mask[(size_t)b * s.Nk + kc] != 0);
     const bool wave_on = __ballot(seen) != 0;
+    float g = 1.f;
+    if (Half<T>::kScaled) g = grad_scale(a.rows2 + (size_t)bh * prep_blocks(s.rows), prep_blocks(s.rows), a.v2 + (size_t)bh * prep_blocks(s.Nk), prep_blocks(s.Nk), lane);
+    // weights of the parts: scores as (shift - lse) / c reaches 2^28 in fp16; |delta| <= 1 / (2 g)
+    const float ws = Half<T>::kScaled ? 4096.f : 1.f, wd = Half<T>::kScaled ? fminf(fmaxf(0.5f / g, 1.f / 8192.f), 32768.f) : 1.f;
+    const float inv_c = 1.f / s.c;
 
     typename Half<T>::v8 kf[KS], vf[KS];
     row_fragments<T, KS>(kf, static_cast<const T*>(a.k) + (size_t)b * s.k_sb + (size_t)kc * s.k_sn + (size_t)hk * s.k_sh, s.D, hi);
     row_fragments<T, KS>(vf, static_cast<const T*>(a.v) + (size_t)b * s.v_sb + (size_t)kc * s.v_sn + (size_t)hk * s.v_sh, s.D, hi);
-    float g = 1.f;
-    if (Half<T>::kScaled) g = grad_scale(a.rows2 + (size_t)bh * prep_blocks(s.rows), prep_blocks(s.rows), a.v2 + (size_t)bh * prep_blocks(s.Nk), prep_blocks(s.Nk), lane);
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++)
+        if (16u * ks + 8u * hi == s.D) {
+            kf[ks] = __builtin_bit_cast(typename Half<T>::v8, part_weights<T>(ws));
+            vf[ks] = __builtin_bit_cast(typename Half<T>::v8, part_weights<T>(wd));
+        }
+    // channels behind the extra ones are never staged: zero (0 * whatever LDS held must not be NaN)
+    for (uint32_t i = tid; i < (4 * L::BYTES + kTileSlack) / 16; i += 64 * NW) reinterpret_cast<u4v*>(lds)[i] = u4v{0u, 0u, 0u, 0u};
+    __syncthreads();
 
     // tiles: t = head in group * per_head + tile of queries; a causal workgroup starts each head at the first tile that sees its keys
     const uint32_t per_head = (s.Nq + QT - 1) / QT;
     const int first_q = s.causal ? (int)wg_key - s.off : 0;              // the first query that sees key wg_key
     const uint32_t skip = first_q > 0 ? min((uint32_t)first_q / QT, per_head) : 0u;
     const uint32_t t_end = min((split + 1) * s.per_split, s.group * per_head);
-    auto advance = [&](uint32_t t) -> uint32_t {                                     // the first tile from t on that is not skipped
+    auto advance = [&](uint32_t t) -> uint32_t {                         // the first tile from t on that is not skipped
         if (skip >= per_head) return t_end;
         while (t < t_end) {
             const uint32_t i = t % per_head;
@@ -65,11 +103,11 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, S
         const uint32_t q0 = (t % per_head) * QT, left = s.Nq - q0;
         uint64_t live = left >= 64u ? ~0ull : (1ull << left) - 1ull;
         if (empties) live &= __ballot(r_lse != INFINITY);
-        stash<L>(ldsQ + buf * L::BYTES, rq, live, tid, 64 * NW);
-        stash<L>(ldsY + buf * L::BYTES, ry, live, tid, 64 * NW);
-        if (wave == 0 && lane < (uint32_t)QT) {
-            stat[buf][0][lane] = Half<T>::kShift - r_lse;
-            stat[buf][1][lane] = r_lse == INFINITY ? 0.f : -r_delta * g;
+        stash<L>(ldsQ + buf * L::BYTES, rq, live, tid, 64 * NW, s.D / 8);
+        stash<L>(ldsY + buf * L::BYTES, ry, live, tid, 64 * NW, s.D / 8);
+        if (lane < (uint32_t)QT) {                                       // the rows' extra channels, one tensor's by each of two waves
+            if (wave == 0) *reinterpret_cast<u4v*>(ldsQ + buf * L::BYTES + lane * L::PITCH + s.D * 2u) = split_parts<T>((Half<T>::kShift - r_lse) * inv_c, ws);
+            if (wave == 1) *reinterpret_cast<u4v*>(ldsY + buf * L::BYTES + lane * L::PITCH + s.D * 2u) = split_parts<T>(r_lse == INFINITY ? 0.f : -r_delta, wd);
         }
     };
 
@@ -84,37 +122,49 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, S
         const int q0 = (int)((t % per_head) * QT);
         if (wave_on && (!s.causal || q0 + QT - 1 + s.off >= (int)w0)) {
             const bool diagonal = s.causal && q0 + s.off < (int)w0 + 31;
+            f32x16 sc[NB], dp[NB];
 #pragma unroll
             for (int st = 0; st < NB; st++) {
-                f32x16 sc = zero16(), dp = zero16();
+                sc[st] = zero16();
+                dp[st] = zero16();
 #pragma unroll
-                for (int ks = 0; ks < KS; ks++) sc = mma(row_operand<T, L>(qt, st, ks, x, hi), kf[ks], sc);
+                for (int ks = 0; ks < KS; ks++) sc[st] = mma(row_operand<T, L>(qt, st, ks, x, hi), kf[ks], sc[st]);
 #pragma unroll
-                for (int ks = 0; ks < KS; ks++) dp = mma(row_operand<T, L>(yt, st, ks, x, hi), vf[ks], dp);
+                for (int ks = 0; ks < KS; ks++) dp[st] = mma(row_operand<T, L>(yt, st, ks, x, hi), vf[ks], dp[st]);
+            }
+#pragma unroll
+            for (int st = 0; st < NB; st++) {
+                // this block's transposed operands, requested ahead of its exponentials (the compiler would read each in front of its product and wait)
+                typename Half<T>::v8 yo[2][DT], qo[2][DT];
+                if (ahead(DM)) {
+#pragma unroll
+                    for (int e = 0; e < 2; e++)
+#pragma unroll
+                        for (int dt = 0; dt < DT; dt++) {
+                            yo[e][dt] = col_operand<T, L>(yt, 2 * st + e, dt0 + dt, lane);
+                            qo[e][dt] = col_operand<T, L>(qt, 2 * st + e, dt0 + dt, lane);
+                        }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
                 if (diagonal) {                                          // query q0 + 32 st + 4 hi + i sees this key when it is not before it
+                    keep_branch();
                     const int first = (int)key - s.off - q0 - 32 * st - 4 * (int)hi;
 #pragma unroll
                     for (int r = 0; r < 16; r++)
-                        if ((r & 3) + 8 * (r >> 2) < first) sc[r] = -INFINITY;
+                        if ((r & 3) + 8 * (r >> 2) < first) sc[st][r] = -INFINITY;
                 }
 #pragma unroll
-                for (int q4 = 0; q4 < 4; q4++) {
-                    const f4 nl = *reinterpret_cast<const f4*>(&stat[buf][0][32 * st + 8 * q4 + 4 * hi]);
-                    const f4 nd = *reinterpret_cast<const f4*>(&stat[buf][1][32 * st + 8 * q4 + 4 * hi]);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int r = 4 * q4 + i;
-                        sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], s.c, nl[i]));
-                        dp[r] = sc[r] * __builtin_fmaf(dp[r], g, nd[i]);
-                    }
+                for (int r = 0; r < 16; r++) {
+                    sc[st][r] = __builtin_amdgcn_exp2f(sc[st][r] * s.c);
+                    dp[st][r] = sc[st][r] * (dp[st][r] * g);
                 }
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    const typename Half<T>::v8 pf = operand<T>(sc, e), df = operand<T>(dp, e);      // (p and ds rounded to the inputs' type)
+                    const typename Half<T>::v8 pf = operand<T>(sc[st], e), df = operand<T>(dp[st], e);      // (p and ds rounded to the inputs' type)
 #pragma unroll
-                    for (int dt = 0; dt < DT; dt++) dv[dt] = mma(col_operand<T, L>(yt, 2 * st + e, dt, lane), pf, dv[dt]);
+                    for (int dt = 0; dt < DT; dt++) dv[dt] = mma(ahead(DM) ? yo[e][dt] : col_operand<T, L>(yt, 2 * st + e, dt0 + dt, lane), pf, dv[dt]);
 #pragma unroll
-                    for (int dt = 0; dt < DT; dt++) dk[dt] = mma(col_operand<T, L>(qt, 2 * st + e, dt, lane), df, dk[dt]);
+                    for (int dt = 0; dt < DT; dt++) dk[dt] = mma(ahead(DM) ? qo[e][dt] : col_operand<T, L>(qt, 2 * st + e, dt0 + dt, lane), df, dk[dt]);
                 }
             }
         }
@@ -131,7 +181,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, S
     for (int dt = 0; dt < DT; dt++)
 #pragma unroll
         for (int q4 = 0; q4 < 4; q4++) {
-            const uint32_t c0 = 32u * dt + 8u * q4 + 4u * hi;
+            const uint32_t c0 = 32u * (dt0 + dt) + 8u * q4 + 4u * hi;
             if (c0 < s.D) {
                 float wk[4], wv[4];
 #pragma unroll
@@ -150,12 +200,24 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, S
         }
 }
 
-template <typename T, int DP, int NW> void go(const BwdArgs& a, const Shape& s, hipStream_t st) {
-    hipLaunchKernelGGL((k_dkdv<T, DP, NW>), dim3(s.tiles_x * s.splits * s.B * s.Hk), dim3(64 * NW), 0, st, a, s);
+template <typename T, int DM> void go(const BwdArgs& a, const Shape& s, hipStream_t st) {
+    constexpr int CS = DM == 256 ? 2 : 1;
+    hipLaunchKernelGGL((k_dkdv<T, DM, CS>), dim3(s.tiles_x * s.splits * s.B * s.Hk * CS), dim3(256), 0, st, a, s);
+}
+template <typename T> void by_width(const BwdArgs& a, const Shape& s, hipStream_t st) {
+    if (s.D <= 40) go<T, 40>(a, s, st);                // (40 and the 8 extra channels are three K steps)
+    else if (s.D <= 64) go<T, 64>(a, s, st);
+    else if (s.D <= 80) go<T, 80>(a, s, st);
+    else if (s.D <= 128) go<T, 128>(a, s, st);
+    else if (s.D <= 160) go<T, 160>(a, s, st);
+    else go<T, 256>(a, s, st);
 }
 
 }  // namespace
 
-void launch_dkdv(const BwdArgs& a, const Shape& s, int bf16, int waves, hipStream_t st) { SDFX_ATTN_DISPATCH(go, a, s, st); }
+void launch_dkdv(const BwdArgs& a, const Shape& s, int bf16, hipStream_t st) {
+    if (bf16) by_width<__bf16>(a, s, st);
+    else by_width<_Float16>(a, s, st);
+}
 
 }  // namespace sdfx_attn

@@ -8,12 +8,12 @@ namespace {
 
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_dq(BwdArgs a, Shape s) {
-    constexpr int KT = key_tile(DP), KS = DP / 16, DT = (DP + 31) / 32, NB = KT / 32;
+    constexpr int KT = key_tile(DP, NW), NBUF = buffers(NW), KS = DP / 16, DT = (DP + 31) / 32, NB = KT / 32;
     typedef Tile<DP, KT, 64 * NW> L;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[4 * L::BYTES + kTileSlack];
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * NBUF * L::BYTES + kTileSlack];
     uint8_t* const ldsV = lds;
-    uint8_t* const ldsK = lds + 2 * L::BYTES;
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, x = lane & 31u, hi = lane >> 5;
+    uint8_t* const ldsK = lds + NBUF * L::BYTES;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), x = lane & 31u, hi = lane >> 5;
     const uint32_t per_bh = s.tiles_x * s.splits;
     const uint32_t lid = xcd_contiguous(blockIdx.x, per_bh * s.B * s.Hk);
     const uint32_t bh = lid / per_bh, rest = lid - bh * per_bh, split = rest / s.tiles_x, xt = rest - split * s.tiles_x;
@@ -55,7 +55,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_dq(BwdArgs a, Sha
         stash<L>(ldsV, rv, live, tid, 64 * NW);
         __syncthreads();
         for (uint32_t j = t0; j < t1; j++) {
-            const uint32_t buf = (j - t0) & 1u;
+            const uint32_t buf = (j - t0) % NBUF, nbuf = (j + 1 - t0) % NBUF;
             uint8_t next_byte = 0;
             if (j + 1 < t1) {
                 request<L>(rk, kb, s.k_sn, (j + 1) * KT, s.Nk, s.D, tid, 64 * NW);
@@ -65,32 +65,50 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_dq(BwdArgs a, Sha
             const uint8_t* kt = ldsK + buf * L::BYTES;
             const uint8_t* vt = ldsV + buf * L::BYTES;
             if (live != 0 && (int)(j * KT) <= wave_hi) {
-                const bool some_hidden = live != all_keys<KT>() || (int)(j * KT + KT - 1) > wave_lo;
+                const bool masked = live != all_keys<KT>() || (int)(j * KT + KT - 1) > wave_lo;
+                f32x16 sc[NB], dp[NB];
 #pragma unroll
                 for (int st = 0; st < NB; st++) {
-                    f32x16 sc = zero16(), dp = zero16();
+                    sc[st] = zero16();
+                    dp[st] = zero16();
 #pragma unroll
-                    for (int ks = 0; ks < KS; ks++) sc = mma(row_operand<T, L>(kt, st, ks, x, hi), qf[ks], sc);
+                    for (int ks = 0; ks < KS; ks++) sc[st] = mma(row_operand<T, L>(kt, st, ks, x, hi), qf[ks], sc[st]);
 #pragma unroll
-                    for (int ks = 0; ks < KS; ks++) dp = mma(row_operand<T, L>(vt, st, ks, x, hi), yf[ks], dp);
-                    if (some_hidden) hide(sc, live, row.lim, j * KT, st, hi);
+                    for (int ks = 0; ks < KS; ks++) dp[st] = mma(row_operand<T, L>(vt, st, ks, x, hi), yf[ks], dp[st]);
+                }
+#pragma unroll
+                for (int st = 0; st < NB; st++) {
+                    // the transposed key operands, requested ahead of the exponentials (the compiler would read each in front of its product and wait)
+                    typename Half<T>::v8 ko[2][DT];
+                    if (ahead(DP)) {
+#pragma unroll
+                        for (int e = 0; e < 2; e++)
+#pragma unroll
+                            for (int dt = 0; dt < DT; dt++) ko[e][dt] = col_operand<T, L>(kt, 2 * st + e, dt, lane);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    if (masked) {
+                        keep_branch();
+                        hide(sc[st], live, row.lim, j * KT, st, hi);
+                    }
 #pragma unroll
                     for (int r = 0; r < 16; r++) {
-                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], s.c, nlse));
-                        sc[r] = p * __builtin_fmaf(dp[r], g, ndelta);
+                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[st][r], s.c, nlse));
+                        sc[st][r] = p * __builtin_fmaf(dp[st][r], g, ndelta);
                     }
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        const typename Half<T>::v8 f = operand<T>(sc, e);            // (ds rounded to the inputs' type)
+                        const typename Half<T>::v8 f = operand<T>(sc[st], e);            // (ds rounded to the inputs' type)
 #pragma unroll
-                        for (int dt = 0; dt < DT; dt++) acc[dt] = mma(col_operand<T, L>(kt, 2 * st + e, dt, lane), f, acc[dt]);
+                        for (int dt = 0; dt < DT; dt++) acc[dt] = mma(ahead(DP) ? ko[e][dt] : col_operand<T, L>(kt, 2 * st + e, dt, lane), f, acc[dt]);
                     }
                 }
             }
+            if (NBUF == 1) __syncthreads();
             if (j + 1 < t1) {
                 live = live_keys<KT>(s, next_byte, j + 1, lane);
-                stash<L>(ldsK + (buf ^ 1u) * L::BYTES, rk, live, tid, 64 * NW);
-                stash<L>(ldsV + (buf ^ 1u) * L::BYTES, rv, live, tid, 64 * NW);
+                stash<L>(ldsK + nbuf * L::BYTES, rk, live, tid, 64 * NW);
+                stash<L>(ldsV + nbuf * L::BYTES, rv, live, tid, 64 * NW);
             }
             __syncthreads();
         }
@@ -118,9 +136,15 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_dq(BwdArgs a, Sha
 template <typename T, int DP, int NW> void go(const BwdArgs& a, const Shape& s, hipStream_t st) {
     hipLaunchKernelGGL((k_dq<T, DP, NW>), dim3(s.tiles_x * s.splits * s.B * s.Hk), dim3(64 * NW), 0, st, a, s);
 }
+template <typename T, int DP, int NW> void go_one(const BwdArgs& a, const Shape& s, hipStream_t st) { go<T, DP < 160 ? DP : 160, NW>(a, s, st); }
 
 }  // namespace
 
-void launch_dq(const BwdArgs& a, const Shape& s, int bf16, int waves, hipStream_t st) { SDFX_ATTN_DISPATCH(go, a, s, st); }
+void launch_dq(const BwdArgs& a, const Shape& s, int bf16, int waves, hipStream_t st) {
+    if (bf16 && waves == 4) SDFX_ATTN_WIDTH(go, __bf16, 4, a, s, st);
+    else if (bf16) SDFX_ATTN_WIDTH(go_one, __bf16, 1, a, s, st);
+    else if (waves == 4) SDFX_ATTN_WIDTH(go, _Float16, 4, a, s, st);
+    else SDFX_ATTN_WIDTH(go_one, _Float16, 1, a, s, st);
+}
 
 }  // namespace sdfx_attn
