@@ -37,7 +37,7 @@ struct Shape {
     int causal, off;                      // query i sees keys <= i + off (off = Nk - Nq)
     float scale, c;                       // softmax scale; times log2(e)
     uint32_t tiles_x;                     // workgroups along rows (forward, dq) or keys (dk / dv)
-    uint32_t splits, per_split;           // the other axis: workgroups, tiles for each
+    uint32_t splits;                      // workgroups along the other axis
 };
 
 template <typename T> struct Half;
@@ -85,11 +85,15 @@ template <typename T> __device__ __forceinline__ typename Half<T>::v8 operand(co
     return v;
 }
 
+// In front of a rarely needed block of selects (5 instructions a score): keeps it a branch, which the compiler would otherwise fold into straight code
+__device__ __forceinline__ void keep_branch() { asm volatile(""); }
+
 // ---- tiles of ROWS rows in LDS, row-major, an odd number of 16-byte chunks a row (16 rows of a ds_read_b128 start in 16 bank quads) ----
 template <int DP, int ROWS, int TH> struct Tile {
     static constexpr int CH = DP / 8;
     static constexpr uint32_t PITCH = (uint32_t)(CH | 1) * 16u;
-    static constexpr uint32_t BYTES = (uint32_t)ROWS * PITCH;
+    static constexpr int ROWS_ = ROWS;
+    static constexpr uint32_t BYTES = (uint32_t)ROWS * PITCH + 16u;      // (and a slot that nothing reads: see Stage)
     static constexpr int NCH = ROWS * CH;
     static constexpr int PT = (NCH + TH - 1) / TH;           // chunks per thread
 };
@@ -97,28 +101,50 @@ template <int DP, int ROWS, int TH> struct Tile {
 // it (their results are rows of the product that nothing stores): bytes to have behind the last tile.
 constexpr uint32_t kTileSlack = 64;
 
-// rows base .. base + ROWS - 1 (clamped to n - 1) into registers; channels from D on are zero
-template <typename L> __device__ __forceinline__ void request(u4v (&r)[L::PT], const void* p, uint64_t sn, uint32_t base, uint32_t n, uint32_t D, uint32_t tid, uint32_t th) {
+// A thread's chunks of a tile: where each lies behind the tile's first row in memory (bytes; the first row's address is a scalar) and in LDS.
+// Only the D / 8 chunks a row has are moved; a kernel that reads further clears LDS once. A thread without a chunk of its own reads the
+// tile's last one and writes it to the 16 bytes behind the tile: no predicates in the loop.
+template <typename L, int TH> struct Stage {
+    uint32_t src[L::PT], dst[L::PT];
+    __device__ __forceinline__ void init(uint32_t D, uint64_t sn, uint32_t tid) {
+        const uint32_t chunks = D / 8, count = L::ROWS_ * chunks;
 #pragma unroll
-    for (int i = 0; i < L::PT; i++) {
-        const uint32_t c = min(tid + (uint32_t)i * th, (uint32_t)L::NCH - 1u);        // (threads past the tile repeat its last chunk)
-        const uint32_t row = c / L::CH, ch = c - row * L::CH;
-        const uint32_t at = min(base + row, n - 1u);
-        r[i] = u4v{0u, 0u, 0u, 0u};
-        if (ch * 8u < D) r[i] = *reinterpret_cast<const u4v*>(static_cast<const uint16_t*>(p) + (size_t)at * sn + ch * 8u);
-    }
-}
-// ... and (the first `chunks` of each row) into LDS; rows whose bit of `live` is clear as zeros (a masked key's values may be anything: 0 * NaN must not reach a product)
-template <typename L> __device__ __forceinline__ void stash(uint8_t* tile, const u4v (&r)[L::PT], uint64_t live, uint32_t tid, uint32_t th,
-                                                                      uint32_t chunks = L::CH) {
-#pragma unroll
-    for (int i = 0; i < L::PT; i++) {
-        const uint32_t c = tid + (uint32_t)i * th, row = c / L::CH, ch = c - row * L::CH;
-        if (c < (uint32_t)L::NCH && ch < chunks) {
-            const bool on = (live >> row) & 1u;
-            *reinterpret_cast<u4v*>(tile + row * L::PITCH + ch * 16u) = on ? r[i] : u4v{0u, 0u, 0u, 0u};
+        for (int i = 0; i < L::PT; i++) {
+            const uint32_t mine = tid + (uint32_t)i * TH, c = min(mine, count - 1u), row = c / chunks, ch = c - row * chunks;
+            src[i] = row * (uint32_t)sn * 2u + ch * 16u;
+            dst[i] = mine < count ? row * L::PITCH + ch * 16u : L::ROWS_ * L::PITCH;
         }
     }
+    __device__ __forceinline__ uint32_t row_of(int i) const { return min(dst[i] / L::PITCH, (uint32_t)L::ROWS_ - 1u); }
+    // `rows` of the tile exist (the others repeat the last)
+    __device__ __forceinline__ void request(u4v (&r)[L::PT], const void* first, uint64_t sn, uint32_t rows) const {
+        if (rows >= (uint32_t)L::ROWS_) {
+#pragma unroll
+            for (int i = 0; i < L::PT; i++) r[i] = *reinterpret_cast<const u4v*>(static_cast<const uint8_t*>(first) + src[i]);
+        } else {
+            keep_branch();
+#pragma unroll
+            for (int i = 0; i < L::PT; i++) {
+                const uint32_t row = row_of(i), past = row >= rows ? row - (rows - 1u) : 0u;
+                r[i] = *reinterpret_cast<const u4v*>(static_cast<const uint8_t*>(first) + (src[i] - past * (uint32_t)sn * 2u));
+            }
+        }
+    }
+    // into LDS; with `all` false, rows whose bit of `live` is clear as zeros (a masked key's values may be anything: 0 * NaN must not reach a product)
+    __device__ __forceinline__ void put(uint8_t* tile, u4v (&r)[L::PT], bool all, uint64_t live) const {
+        if (!all) {
+            keep_branch();
+#pragma unroll
+            for (int i = 0; i < L::PT; i++)
+                if (!((live >> row_of(i)) & 1u)) r[i] = u4v{0u, 0u, 0u, 0u};
+        }
+#pragma unroll
+        for (int i = 0; i < L::PT; i++) *reinterpret_cast<u4v*>(tile + dst[i]) = r[i];
+    }
+};
+__device__ __forceinline__ void clear_lds(uint8_t* lds, uint32_t bytes, uint32_t tid, uint32_t th) {
+    for (uint32_t i = tid; i < bytes / 16u; i += th) reinterpret_cast<u4v*>(lds)[i] = u4v{0u, 0u, 0u, 0u};
+    __syncthreads();
 }
 // A operand, rows of the tile: lane (x, hi) row 32 blk + x, channels 16 ks + 8 hi .. + 7
 template <typename T, typename L> __device__ __forceinline__ typename Half<T>::v8 row_operand(const uint8_t* tile, uint32_t blk, uint32_t ks, uint32_t x, uint32_t hi) {
@@ -203,10 +229,12 @@ inline int padded(uint32_t D) {
         }                                                                 \
     } while (0)
 
-// In front of a rarely needed block of selects (5 instructions a score): keeps it a branch, which the compiler would otherwise fold into straight code
-__device__ __forceinline__ void keep_branch() { asm volatile(""); }
+template <bool B> struct Flag { static constexpr bool value = B; };
 // operands of the second products requested ahead of the exponentials: where a lane's registers hold them
 constexpr bool ahead(int dp) { return dp <= 64; }
+
+// the tiles of `n` that split `i` of `splits` takes
+__device__ __forceinline__ uint32_t split_at(uint32_t n, uint32_t i, uint32_t splits) { return splits == 1 ? (i ? n : 0u) : (uint32_t)((uint64_t)n * i / splits); }
 
 // the row a lane owns in the forward and in dq
 struct Row {
@@ -230,20 +258,18 @@ __device__ __forceinline__ void query_range(const Shape& s, uint32_t a, uint32_t
     lo = ga == gb ? a - ga * s.Nq : 0u;
     hi = ga == gb ? b - ga * s.Nq : s.Nq - 1u;
 }
-// Keys of a tile that exist and are not masked, one bit each (the same in every wave). The byte is loaded early, the ballot taken later.
-template <int KT> __device__ __forceinline__ uint8_t mask_byte(const Shape& s, uint32_t b, uint32_t tile, uint32_t lane) {
-    const uint32_t key = tile * KT + lane;
-    if (!s.mask) return 1;
-    return s.mask[(size_t)b * s.Nk + min(key, s.Nk - 1u)];
-}
-template <int KT> __device__ __forceinline__ uint64_t live_keys(const Shape& s, uint8_t byte, uint32_t tile, uint32_t lane) {
-    return __ballot(lane < (uint32_t)KT && tile * KT + lane < s.Nk && byte != 0);
-}
 template <int KT> constexpr uint64_t all_keys() { return KT == 64 ? ~0ull : ((1ull << (KT & 63)) - 1ull); }
+// Keys of a tile that exist (`left` from its first on) and are not masked, one bit each, the same in every wave. The mask's byte is loaded early
+// (`row`: the batch entry's mask from the tile's first key on), the ballot taken later.
+__device__ __forceinline__ uint8_t mask_byte(const uint8_t* row, uint32_t left, uint32_t lane) { return row[min(lane, left - 1u)]; }
+template <int KT> __device__ __forceinline__ uint64_t live_keys(bool has_mask, uint8_t byte, uint32_t left, uint32_t lane) {
+    if (!has_mask) return left >= (uint32_t)KT ? all_keys<KT>() : (1ull << left) - 1ull;
+    return __ballot(lane < (uint32_t)KT && lane < left && byte != 0);
+}
 // -inf where the lane's row does not see the key: D element r of block st is key 32 st + (r & 3) + 8 (r >> 2) + 4 hi of the tile
-__device__ __forceinline__ void hide(f32x16& sc, uint64_t live, int lim, uint32_t tile0, int st, uint32_t hi) {
+__device__ __forceinline__ void hide(f32x16& sc, uint64_t live, int lim, int key0, int st, uint32_t hi) {
     const uint32_t bits = (uint32_t)(live >> (32 * st)) >> (4 * hi);
-    const int last = lim - (int)(tile0 + 32u * st + 4u * hi);
+    const int last = lim - (key0 + 32 * st + 4 * (int)hi);
 #pragma unroll
     for (int r = 0; r < 16; r++) {
         const int k = (r & 3) + 8 * (r >> 2);

@@ -42,7 +42,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_fwd(const T* __re
         query_range(s, min(w0, s.rows - 1u), min(w0 + 32u, s.rows) - 1u, lo, hi_q);
         wave_lo = (int)lo + s.off; wave_hi = (int)hi_q + s.off;
     }
-    const uint32_t t0 = split * s.per_split, t1 = min(t0 + s.per_split, (kend + KT - 1) / KT);
+    const uint32_t tiles = (kend + KT - 1) / KT, t0 = split_at(tiles, split, s.splits), t1 = split_at(tiles, split + 1, s.splits);
 
     f32x16 acc[DT];
 #pragma unroll
@@ -50,23 +50,37 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_fwd(const T* __re
     float m_run = -1e30f, l_run = 0.f;
     if (t0 < t1) {
         u4v rk[L::PT], rv[L::PT];
-        request<L>(rk, kb, s.k_sn, t0 * KT, s.Nk, s.D, tid, 64 * NW);
-        request<L>(rv, vb, s.v_sn, t0 * KT, s.Nk, s.D, tid, 64 * NW);
-        uint64_t live = live_keys<KT>(s, mask_byte<KT>(s, b, t0, lane), t0, lane);
-        stash<L>(ldsK, rk, live, tid, 64 * NW);
-        stash<L>(ldsV, rv, live, tid, 64 * NW);
+        Stage<L, 64 * NW> stk, stv;
+        stk.init(s.D, s.k_sn, tid);
+        stv.init(s.D, s.v_sn, tid);
+        if (DP != s.D) clear_lds(lds, sizeof lds, tid, 64 * NW);
+        // the next tile to request: its rows, the keys left from it on, its part of the mask
+        const T *kp = kb + (size_t)t0 * KT * s.k_sn, *vp = vb + (size_t)t0 * KT * s.v_sn;
+        const uint64_t k_step = (uint64_t)KT * s.k_sn, v_step = (uint64_t)KT * s.v_sn;
+        const bool has_mask = s.mask != nullptr;
+        const uint8_t* mp = has_mask ? s.mask + (size_t)b * s.Nk + t0 * KT : nullptr;
+        uint32_t left = s.Nk - t0 * KT;
+        uint8_t byte = 1;
+        auto ask = [&]() {
+            stk.request(rk, kp, s.k_sn, left);
+            stv.request(rv, vp, s.v_sn, left);
+            if (has_mask) byte = mask_byte(mp, left, lane);
+        };
+        ask();
+        uint64_t live = live_keys<KT>(has_mask, byte, left, lane);
+        stk.put(ldsK, rk, live == all_keys<KT>(), live);
+        stv.put(ldsV, rv, live == all_keys<KT>(), live);
         __syncthreads();
-        for (uint32_t j = t0; j < t1; j++) {
-            const uint32_t buf = (j - t0) % NBUF, nbuf = (j + 1 - t0) % NBUF;
-            uint8_t next_byte = 0;
+        uint32_t buf = 0;
+        int key0 = (int)(t0 * KT);
+        for (uint32_t j = t0; j < t1; j++, key0 += KT) {
             if (j + 1 < t1) {
-                request<L>(rk, kb, s.k_sn, (j + 1) * KT, s.Nk, s.D, tid, 64 * NW);
-                request<L>(rv, vb, s.v_sn, (j + 1) * KT, s.Nk, s.D, tid, 64 * NW);
-                next_byte = mask_byte<KT>(s, b, j + 1, lane);
+                kp += k_step; vp += v_step; mp += KT; left -= KT;
+                ask();
             }
             const uint8_t* kt = ldsK + buf * L::BYTES;
             const uint8_t* vt = ldsV + buf * L::BYTES;
-            if (live != 0 && (int)(j * KT) <= wave_hi) {
+            if (live != 0 && key0 <= wave_hi) {
                 f32x16 sc[NB];
 #pragma unroll
                 for (int st = 0; st < NB; st++) {
@@ -74,10 +88,10 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_fwd(const T* __re
 #pragma unroll
                     for (int ks = 0; ks < KS; ks++) sc[st] = mma(row_operand<T, L>(kt, st, ks, x, hi), qf[ks], sc[st]);
                 }
-                if (live != all_keys<KT>() || (int)(j * KT + KT - 1) > wave_lo) {
+                if (live != all_keys<KT>() || key0 + KT - 1 > wave_lo) {
                     keep_branch();
 #pragma unroll
-                    for (int st = 0; st < NB; st++) hide(sc[st], live, row.lim, j * KT, st, hi);
+                    for (int st = 0; st < NB; st++) hide(sc[st], live, row.lim, key0, st, hi);
                 }
                 // the value operands, requested ahead of the softmax (the compiler would read each in front of its product and wait)
                 typename Half<T>::v8 vo[2 * NB][DT];
@@ -88,6 +102,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_fwd(const T* __re
                         for (int dt = 0; dt < DT; dt++) vo[e][dt] = col_operand<T, L>(vt, e, dt, lane);
                     __builtin_amdgcn_sched_barrier(0);
                 }
+                __builtin_amdgcn_s_setprio(1);            // (a wave in its softmax ahead of one that feeds the matrix cores: the two overlap)
                 float mx = -INFINITY;
 #pragma unroll
                 for (int st = 0; st < NB; st++)
@@ -120,12 +135,14 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_fwd(const T* __re
                     }
                 }
                 l_run += sum0 + sum1;
+                __builtin_amdgcn_s_setprio(0);
             }
             if (NBUF == 1) __syncthreads();
             if (j + 1 < t1) {
-                live = live_keys<KT>(s, next_byte, j + 1, lane);
-                stash<L>(ldsK + nbuf * L::BYTES, rk, live, tid, 64 * NW);
-                stash<L>(ldsV + nbuf * L::BYTES, rv, live, tid, 64 * NW);
+                if (NBUF == 2) buf ^= 1u;
+                live = live_keys<KT>(has_mask, byte, left, lane);
+                stk.put(ldsK + buf * L::BYTES, rk, live == all_keys<KT>(), live);
+                stv.put(ldsV + buf * L::BYTES, rv, live == all_keys<KT>(), live);
             }
             __syncthreads();
         }
@@ -288,8 +305,7 @@ void plan(Shape& s, uint32_t along, uint32_t other_tiles, int waves, uint32_t le
     uint64_t splits = 2 * base >= want ? 1 : (want + base - 1) / base;
     const uint64_t most = other_tiles / least ? other_tiles / least : 1;
     if (splits > most) splits = most;
-    s.per_split = div_up(other_tiles, splits);
-    s.splits = div_up(other_tiles, s.per_split);
+    s.splits = (uint32_t)splits;
 }
 void plan_rows(Shape& s, int& waves) {          // forward, dq
     const int dp = padded(s.D);
@@ -338,6 +354,7 @@ const char* shape_error(uint32_t B, uint32_t H, uint32_t Hk, uint32_t Nq, uint32
     if (D == 0 || D % 8 || D > 256) return "the head width must be a multiple of 8 up to 256";
     if (Nq >= 0x40000000u || Nk >= 0x40000000u || (uint64_t)(H / Hk) * Nq >= 0x40000000u) return "more than 2^30 queries or keys";
     if ((uint64_t)B * H * ((uint64_t)Nq + Nk) >= 0x40000000ull) return "more than 2^30 rows";
+    if ((uint64_t)H * D >= (1u << 24)) return "more than 2^24 channels";
     return nullptr;
 }
 void fill(Shape& s, uint32_t B, uint32_t H, uint32_t Hk, uint32_t Nq, uint32_t Nk, uint32_t D) {
@@ -358,7 +375,8 @@ void fill_call(Shape& s, const uint64_t* qs, const uint64_t* ks, const uint64_t*
 bool strides_ok(const uint64_t* a, const uint64_t* b, const uint64_t* c) {
     uint64_t all = 0;
     for (int i = 0; i < 3; i++) all |= a[i] | b[i] | c[i];
-    return all % 8 == 0;
+    const uint64_t token = a[1] | b[1] | c[1];          // (offsets inside a tile of 64 rows are 32-bit)
+    return all % 8 == 0 && token < (1ull << 24);
 }
 uint64_t up16(uint64_t floats) { return (floats + 3) / 4 * 4; }
 struct BwdLayout { uint64_t rows2, v2, pq, pk, pv, total; };   // float offsets behind delta
@@ -402,7 +420,7 @@ int sdfx_attention_train_forward(const void* q, const void* k, const void* v, co
     SDFX_REQUIRE(scale > 0.f && scale < 3e38f, "attention_train_forward: the scale must be positive and finite");
     SDFX_REQUIRE(strides_ok(q_strides, k_strides, v_strides) && ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) |
                  reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(o_lo) | reinterpret_cast<uintptr_t>(scratch)) % 16) == 0,
-                 "attention_train_forward: rows must be 16-byte aligned");
+                 "attention_train_forward: rows must be 16-byte aligned, token strides below 2^24");
     Shape s;
     fill(s, B, H, Hk, Nq, Nk, D);
     fill_call(s, q_strides, k_strides, v_strides, key_mask, scale, causal);
@@ -434,7 +452,7 @@ int sdfx_attention_train_backward(const void* q, const void* k, const void* v, c
     SDFX_REQUIRE(strides_ok(q_strides, k_strides, v_strides) && ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) |
                  reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(o_lo) | reinterpret_cast<uintptr_t>(dy) |
                  reinterpret_cast<uintptr_t>(dq) | reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv) | reinterpret_cast<uintptr_t>(scratch)) % 16) == 0,
-                 "attention_train_backward: rows must be 16-byte aligned");
+                 "attention_train_backward: rows must be 16-byte aligned, token strides below 2^24");
     Shape s;
     fill(s, B, H, Hk, Nq, Nk, D);
     fill_call(s, q_strides, k_strides, v_strides, key_mask, scale, causal);

@@ -65,23 +65,14 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
             vf[ks] = __builtin_bit_cast(typename Half<T>::v8, part_weights<T>(wd));
         }
     // channels behind the extra ones are never staged: zero (0 * whatever LDS held must not be NaN)
-    for (uint32_t i = tid; i < (4 * L::BYTES + kTileSlack) / 16; i += 64 * NW) reinterpret_cast<u4v*>(lds)[i] = u4v{0u, 0u, 0u, 0u};
-    __syncthreads();
+    clear_lds(lds, sizeof lds, tid, 64 * NW);
 
-    // tiles: t = head in group * per_head + tile of queries; a causal workgroup starts each head at the first tile that sees its keys
+    // Tiles: i of a head in the group, heads in turn; a causal workgroup starts each head at the first tile that sees one of its keys.
     const uint32_t per_head = (s.Nq + QT - 1) / QT;
     const int first_q = s.causal ? (int)wg_key - s.off : 0;              // the first query that sees key wg_key
-    const uint32_t skip = first_q > 0 ? min((uint32_t)first_q / QT, per_head) : 0u;
-    const uint32_t t_end = min((split + 1) * s.per_split, s.group * per_head);
-    auto advance = [&](uint32_t t) -> uint32_t {                         // the first tile from t on that is not skipped
-        if (skip >= per_head) return t_end;
-        while (t < t_end) {
-            const uint32_t i = t % per_head;
-            if (i >= skip) break;
-            t += skip - i;
-        }
-        return min(t, t_end);
-    };
+    const uint32_t skip = first_q > 0 ? min((uint32_t)first_q / QT, per_head) : 0u, useful = per_head - skip;
+    const uint32_t u0 = split_at(s.group * useful, split, s.splits);
+    uint32_t todo = split_at(s.group * useful, split + 1, s.splits) - u0;
     // rows without a visible key (possible under a causal mask with a key mask or more queries than keys): their dy must not reach the sums
     const bool empties = s.causal && (s.mask || s.off < 0);
 
@@ -90,36 +81,58 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
     for (int dt = 0; dt < DT; dt++) { dk[dt] = zero16(); dv[dt] = zero16(); }
 
     u4v rq[L::PT], ry[L::PT];
+    Stage<L, 64 * NW> stq, sty;
+    const uint64_t y_sn = (uint64_t)s.H * s.D;
+    stq.init(s.D, s.q_sn, tid);
+    sty.init(s.D, y_sn, tid);
     float r_lse = 0.f, r_delta = 0.f;
-    auto ask = [&](uint32_t t) {
-        const uint32_t gi = t / per_head, q0 = (t - gi * per_head) * QT, head = hk * s.group + gi;
-        request<L>(rq, static_cast<const T*>(a.q) + (size_t)b * s.q_sb + (size_t)head * s.q_sh, s.q_sn, q0, s.Nq, s.D, tid, 64 * NW);
-        request<L>(ry, static_cast<const T*>(a.dy) + (size_t)b * s.Nq * s.H * s.D + (size_t)head * s.D, (uint64_t)s.H * s.D, q0, s.Nq, s.D, tid, 64 * NW);
-        const size_t at = (size_t)bh * s.rows + (size_t)gi * s.Nq + min(q0 + lane, s.Nq - 1u);
-        r_lse = lane < (uint32_t)QT && q0 + lane < s.Nq ? a.lse[at] : INFINITY;       // (every wave: the empty rows' ballot is uniform)
-        r_delta = a.delta[at];
+    // the next tile to request: its queries, and its rows' statistics (their ballot is uniform: every wave loads them)
+    const uint32_t gi0 = useful ? u0 / useful : 0u;
+    uint32_t head = hk * s.group + gi0, ni = skip + (u0 - gi0 * useful), nq0 = ni * QT;
+    const T *qp, *yp;
+    size_t stat_at;
+    auto start = [&]() {                                                 // of tile `ni` of query head `head`
+        qp = static_cast<const T*>(a.q) + (size_t)b * s.q_sb + (size_t)head * s.q_sh + (size_t)nq0 * s.q_sn;
+        yp = static_cast<const T*>(a.dy) + ((size_t)b * s.Nq + nq0) * y_sn + (size_t)head * s.D;
+        stat_at = ((size_t)b * s.H + head) * s.Nq + nq0;
     };
-    auto put = [&](uint32_t t, uint32_t buf) {
-        const uint32_t q0 = (t % per_head) * QT, left = s.Nq - q0;
+    auto ask = [&]() {
+        const uint32_t left = s.Nq - nq0, in = min(lane, left - 1u);
+        stq.request(rq, qp, s.q_sn, left);
+        sty.request(ry, yp, y_sn, left);
+        r_lse = lane < left ? a.lse[stat_at + in] : INFINITY;
+        r_delta = a.delta[stat_at + in];
+    };
+    auto advance = [&]() {
+        nq0 += QT;
+        if (++ni == per_head) {
+            ni = skip; nq0 = skip * QT; head++;
+            start();
+        } else {
+            qp += (uint64_t)QT * s.q_sn; yp += (uint64_t)QT * y_sn; stat_at += QT;
+        }
+    };
+    auto put = [&](uint32_t buf) {
+        const uint32_t left = s.Nq - nq0;
         uint64_t live = left >= 64u ? ~0ull : (1ull << left) - 1ull;
         if (empties) live &= __ballot(r_lse != INFINITY);
-        stash<L>(ldsQ + buf * L::BYTES, rq, live, tid, 64 * NW, s.D / 8);
-        stash<L>(ldsY + buf * L::BYTES, ry, live, tid, 64 * NW, s.D / 8);
+        const bool whole = left >= (uint32_t)QT && !empties;
+        stq.put(ldsQ + buf * L::BYTES, rq, whole, live);
+        sty.put(ldsY + buf * L::BYTES, ry, whole, live);
         if (lane < (uint32_t)QT) {                                       // the rows' extra channels, one tensor's by each of two waves
             if (wave == 0) *reinterpret_cast<u4v*>(ldsQ + buf * L::BYTES + lane * L::PITCH + s.D * 2u) = split_parts<T>((Half<T>::kShift - r_lse) * inv_c, ws);
             if (wave == 1) *reinterpret_cast<u4v*>(ldsY + buf * L::BYTES + lane * L::PITCH + s.D * 2u) = split_parts<T>(r_lse == INFINITY ? 0.f : -r_delta, wd);
         }
     };
 
-    uint32_t t = advance(split * s.per_split), buf = 0;
-    if (t < t_end) { ask(t); put(t, 0); }
+    uint32_t buf = 0;
+    if (todo) { start(); ask(); put(0); }
     __syncthreads();
-    while (t < t_end) {
-        const uint32_t next = advance(t + 1);
-        if (next < t_end) ask(next);
+    for (; todo; todo--) {
         const uint8_t* qt = ldsQ + buf * L::BYTES;
         const uint8_t* yt = ldsY + buf * L::BYTES;
-        const int q0 = (int)((t % per_head) * QT);
+        const int q0 = (int)nq0;
+        if (todo > 1) { advance(); ask(); }
         if (wave_on && (!s.causal || q0 + QT - 1 + s.off >= (int)w0)) {
             const bool diagonal = s.causal && q0 + s.off < (int)w0 + 31;
             f32x16 sc[NB], dp[NB];
@@ -156,7 +169,7 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
                     sc[st][r] = __builtin_amdgcn_exp2f(sc[st][r] * s.c);
-                    dp[st][r] = sc[st][r] * (dp[st][r] * g);
+                    dp[st][r] = sc[st][r] * (Half<T>::kScaled ? dp[st][r] * g : dp[st][r]);
                 }
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
@@ -168,10 +181,11 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
                 }
             }
         }
-        if (next < t_end) put(next, buf ^ 1u);
+        if (todo > 1) {
+            buf ^= 1u;
+            put(buf);
+        }
         __syncthreads();
-        t = next;
-        buf ^= 1u;
     }
     if (key >= s.Nk) return;
     const float fv = Half<T>::kScaled ? 1.f / 32768.f : 1.f, fk = s.scale * fv / g;

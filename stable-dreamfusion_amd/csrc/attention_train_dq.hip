@@ -41,31 +41,45 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_dq(BwdArgs a, Sha
         query_range(s, min(w0, s.rows - 1u), min(w0 + 32u, s.rows) - 1u, lo, hi_q);
         wave_lo = (int)lo + s.off; wave_hi = (int)hi_q + s.off;
     }
-    const uint32_t t0 = split * s.per_split, t1 = min(t0 + s.per_split, (kend + KT - 1) / KT);
+    const uint32_t tiles = (kend + KT - 1) / KT, t0 = split_at(tiles, split, s.splits), t1 = split_at(tiles, split + 1, s.splits);
 
     f32x16 acc[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) acc[dt] = zero16();
     if (t0 < t1) {
         u4v rk[L::PT], rv[L::PT];
-        request<L>(rk, kb, s.k_sn, t0 * KT, s.Nk, s.D, tid, 64 * NW);
-        request<L>(rv, vb, s.v_sn, t0 * KT, s.Nk, s.D, tid, 64 * NW);
-        uint64_t live = live_keys<KT>(s, mask_byte<KT>(s, b, t0, lane), t0, lane);
-        stash<L>(ldsK, rk, live, tid, 64 * NW);
-        stash<L>(ldsV, rv, live, tid, 64 * NW);
+        Stage<L, 64 * NW> stk, stv;
+        stk.init(s.D, s.k_sn, tid);
+        stv.init(s.D, s.v_sn, tid);
+        if (DP != s.D) clear_lds(lds, sizeof lds, tid, 64 * NW);
+        // the next tile to request: its rows, the keys left from it on, its part of the mask
+        const T *kp = kb + (size_t)t0 * KT * s.k_sn, *vp = vb + (size_t)t0 * KT * s.v_sn;
+        const uint64_t k_step = (uint64_t)KT * s.k_sn, v_step = (uint64_t)KT * s.v_sn;
+        const bool has_mask = s.mask != nullptr;
+        const uint8_t* mp = has_mask ? s.mask + (size_t)b * s.Nk + t0 * KT : nullptr;
+        uint32_t left = s.Nk - t0 * KT;
+        uint8_t byte = 1;
+        auto ask = [&]() {
+            stk.request(rk, kp, s.k_sn, left);
+            stv.request(rv, vp, s.v_sn, left);
+            if (has_mask) byte = mask_byte(mp, left, lane);
+        };
+        ask();
+        uint64_t live = live_keys<KT>(has_mask, byte, left, lane);
+        stk.put(ldsK, rk, live == all_keys<KT>(), live);
+        stv.put(ldsV, rv, live == all_keys<KT>(), live);
         __syncthreads();
-        for (uint32_t j = t0; j < t1; j++) {
-            const uint32_t buf = (j - t0) % NBUF, nbuf = (j + 1 - t0) % NBUF;
-            uint8_t next_byte = 0;
+        uint32_t buf = 0;
+        int key0 = (int)(t0 * KT);
+        for (uint32_t j = t0; j < t1; j++, key0 += KT) {
             if (j + 1 < t1) {
-                request<L>(rk, kb, s.k_sn, (j + 1) * KT, s.Nk, s.D, tid, 64 * NW);
-                request<L>(rv, vb, s.v_sn, (j + 1) * KT, s.Nk, s.D, tid, 64 * NW);
-                next_byte = mask_byte<KT>(s, b, j + 1, lane);
+                kp += k_step; vp += v_step; mp += KT; left -= KT;
+                ask();
             }
             const uint8_t* kt = ldsK + buf * L::BYTES;
             const uint8_t* vt = ldsV + buf * L::BYTES;
-            if (live != 0 && (int)(j * KT) <= wave_hi) {
-                const bool masked = live != all_keys<KT>() || (int)(j * KT + KT - 1) > wave_lo;
+            if (live != 0 && key0 <= wave_hi) {
+                const bool masked = live != all_keys<KT>() || key0 + KT - 1 > wave_lo;
                 f32x16 sc[NB], dp[NB];
 #pragma unroll
                 for (int st = 0; st < NB; st++) {
@@ -89,13 +103,15 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_dq(BwdArgs a, Sha
                     }
                     if (masked) {
                         keep_branch();
-                        hide(sc[st], live, row.lim, j * KT, st, hi);
+                        hide(sc[st], live, row.lim, key0, st, hi);
                     }
+                    __builtin_amdgcn_s_setprio(1);        // (a wave at its exponentials ahead of one that feeds the matrix cores: the two overlap)
 #pragma unroll
                     for (int r = 0; r < 16; r++) {
                         const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[st][r], s.c, nlse));
                         sc[st][r] = p * __builtin_fmaf(dp[st][r], g, ndelta);
                     }
+                    __builtin_amdgcn_s_setprio(0);
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         const typename Half<T>::v8 f = operand<T>(sc[st], e);            // (ds rounded to the inputs' type)
@@ -106,9 +122,10 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_dq(BwdArgs a, Sha
             }
             if (NBUF == 1) __syncthreads();
             if (j + 1 < t1) {
-                live = live_keys<KT>(s, next_byte, j + 1, lane);
-                stash<L>(ldsK + nbuf * L::BYTES, rk, live, tid, 64 * NW);
-                stash<L>(ldsV + nbuf * L::BYTES, rv, live, tid, 64 * NW);
+                if (NBUF == 2) buf ^= 1u;
+                live = live_keys<KT>(has_mask, byte, left, lane);
+                stk.put(ldsK + buf * L::BYTES, rk, live == all_keys<KT>(), live);
+                stv.put(ldsV + buf * L::BYTES, rv, live == all_keys<KT>(), live);
             }
             __syncthreads();
         }

@@ -82,7 +82,7 @@ uint32_t u(int64_t v) { return (uint32_t)v; }
 struct Strides { uint64_t s[3]; };
 Strides strides(const Tensor& t) { return {{(uint64_t)t.stride(0), (uint64_t)t.stride(2), (uint64_t)t.stride(1)}}; }    // batch, token, head
 Tensor rows16(const Tensor& t) {          // as the kernels read it, or a copy
-    const bool ok = t.stride(3) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && t.stride(2) % 8 == 0 &&
+    const bool ok = t.stride(3) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && t.stride(2) % 8 == 0 && t.stride(2) < (1 << 24) &&
                     reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
     return ok ? t : t.contiguous();
 }
