@@ -607,13 +607,13 @@ int sdfx_attention_train_backward(const void* q, const void* k, const void* v, c
 /*
  * Extension (no reference kernel) — the group norm above with every gradient, for blocks that train. dtype: 0 fp16, 1 bf16, 2 float32
  * (x, pre, y, dy, dx, dpre); gamma / beta / dgamma / dbeta have that type, or float32 with params_f32 != 0. x[N, HW, C] is
- * channels-last memory, C % 8 == 0, C <= 2560, G <= 64, C % G == 0; map pointers 16-byte aligned.
+ * channels-last memory, C % 8 == 0, C <= 2560, G <= 64, C % G == 0; maps, pre, gamma and beta 16-byte aligned.
  * forward: y = act(norm(x + pre) * gamma + beta); mean_rstd[N, G, 2] and, when saved8 is not NULL (C % 32 == 0), the 8-bit form of x:
  *   N HW C code bytes, then N HW C / 32 scale bytes (block of 32 channels: step 2^(scale - 127), scale 255 = the block holds an
  *   infinity or a NaN and decodes as NaN). pre[N, C] may be NULL.
  * backward: x is the forward's x, or its saved8 with eight_bits != 0. dx / dpre / dgamma / dbeta may each be NULL. With the 8-bit input the
  *   derivative is evaluated at the decoded x with the forward's statistics.
- * scratch: sdfx_group_norm_train_scratch_bytes(N, HW, C, G) bytes, 8-byte aligned, uninitialised (0: the shape is not taken).
+ * scratch: sdfx_group_norm_train_scratch_bytes(N, HW, C, G) bytes, uninitialised (0: the shape is not taken).
  */
 uint64_t sdfx_group_norm_train_scratch_bytes(uint32_t N, uint32_t HW, uint32_t C, uint32_t G);
 int sdfx_group_norm_train_forward(const void* x, const void* pre, const void* gamma, const void* beta, uint32_t N, uint32_t HW, uint32_t C, uint32_t G,

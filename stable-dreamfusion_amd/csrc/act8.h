@@ -5,7 +5,7 @@
 // channels shares the step 2^(floor(log2 max|x|) - 6), at least 2^-126; its scale byte is the step's biased exponent, and
 // code = clamp(round-half-even(x / step), -127, 127): half a step off at most (one step where the largest magnitudes clamp), i.e.
 // 2^-7 .. 2^-6 of the block's maximum. Steps are powers of two so that x / step and code * step are exact: the codes do not depend on
-// how a division is rounded. A block that holds an infinity or a NaN gets scale byte 255 and codes 0: it decodes as 0 * inf = NaN.
+// how a division is rounded. A block that holds an infinity or a NaN gets scale byte 255 and codes 0: it decodes as NaN.
 // Signed bytes with a shared exponent rather than e4m3: the 7 bits resolve 2^-7 of the maximum everywhere, e4m3's 3 mantissa bits
 // 2^-4 of each value (rms 2.6 % against 0.7 % of the deviation of a normal block).
 #pragma once
@@ -69,6 +69,11 @@ __device__ __forceinline__ void store8(__bf16* p, const float (&f)[8]) {
     }
     *reinterpret_cast<u4n*>(p) = w;
 }
+// eight consecutive parameters of the activation's type or float32 (16-byte aligned)
+template <typename T> __device__ __forceinline__ void load_params(const void* p, size_t c, bool f32, float (&f)[8]) {
+    if (f32) widen(load8(static_cast<const float*>(p) + c), f);
+    else widen(load8(static_cast<const T*>(p) + c), f);
+}
 // a parameter of the activation's type or float32
 template <typename T> __device__ __forceinline__ float load_param(const void* p, size_t i, bool f32) {
     return f32 ? static_cast<const float*>(p)[i] : (float)static_cast<const T*>(p)[i];
@@ -107,9 +112,10 @@ __device__ __forceinline__ u2n encode8(const float (&f)[8], uint32_t& scale) {
     return c;
 }
 __device__ __forceinline__ void decode8(u2n c, uint32_t scale, float (&f)[8]) {
-    const float step = __uint_as_float(scale << 23);          // (scale 255: infinity, 0 * inf = NaN)
+    const float step = __uint_as_float(scale << 23), low = -128.f * step;          // (scale 255: infinity, inf - inf = NaN)
+    const u2n w = c ^ u2n{0x80808080u, 0x80808080u};          // code + 128: one conversion and one fma a value, both exact
 #pragma unroll
-    for (int i = 0; i < 8; i++) f[i] = (float)(int8_t)((c[i >> 2] >> (8 * (i & 3))) & 255u) * step;
+    for (int i = 0; i < 8; i++) f[i] = __builtin_fmaf((float)((w[i >> 2] >> (8 * (i & 3))) & 255u), step, low);
 }
 
 // an input read back in the backward: the activation itself (Q8 false) or its 8-bit form

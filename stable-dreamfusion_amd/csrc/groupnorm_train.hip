@@ -7,12 +7,14 @@
 // 8-bit input the backward's reads of x halve.
 //   forward   k_stats     per (sample, pixel slab): sums of d and d^2 per group, d = u - pivot, pivot = the group's first value: the
 //                         difference E[d^2] - E[d]^2 stays accurate for a map whose mean is far from zero
-//             k_finish    per (sample, group): slab partials combined in double -> mean, rstd
+//             k_finish    per (sample, group): slab partials combined in double -> mean, rstd. Up to kInlineSlabs slabs a sample every
+//                         workgroup of k_apply combines them itself (one launch less; at most 64 KB out of L2 each)
 //             k_apply     y, and the 8-bit form of x
 //   backward  k_bwd_stats per (sample, slab): sums of dz, dz xh (and xh, for dpre) per channel
-//             k_bwd_finish  per (sample, group): over slabs, in double -> channel sums, the two means, and dpre from the same sums:
-//                           sum over pixels of dx = rstd (gamma S_dz - n m1 - m2 S_xh)
-//             k_bwd_apply dx; its first threads add the channel sums over samples: dgamma, dbeta
+//                         and of g, g xh per group
+//             k_bwd_finish  per (sample, group): the two means, in double; inline like k_finish
+//             k_bwd_apply dx; then its waves take channels in turn: the sums over slabs and samples, in double -> dgamma, dbeta, and dpre
+//                         from the same sums: sum over pixels of dx = rstd (gamma S_dz - n m1 - m2 S_xh)
 // No atomics: partials are combined in a fixed order, results are bit-reproducible.
 #include "act8.h"
 
@@ -23,6 +25,7 @@ namespace {
 constexpr uint32_t kMaxGroups = 64;
 constexpr uint32_t kMaxThreads = 320;        // C / 8 <= 320 vectors per pixel
 constexpr uint32_t kTrip = 4;                // pixels whose loads a thread issues together
+constexpr uint32_t kInlineSlabs = 256;       // slabs a sample up to which every consumer combines them itself
 
 struct Shape {
     uint32_t N, HW, C, G;
@@ -31,6 +34,8 @@ struct Shape {
     uint32_t slabs, P;       // workgroups per sample, pixels per slab
     float eps;
     int pf32;                // gamma / beta (and their gradients) are float32
+    int inl;                 // the consumers combine the slabs' sums themselves
+    uint32_t lanes;          // lanes that add a channel's slabs (a power of two)
 };
 
 bool make_shape(uint32_t N, uint32_t HW, uint32_t C, uint32_t G, Shape& s) {
@@ -47,6 +52,9 @@ bool make_shape(uint32_t N, uint32_t HW, uint32_t C, uint32_t G, Shape& s) {
     s.P = div_up(div_up(HW, slabs), trip) * trip;
     s.slabs = div_up(HW, s.P);
     s.eps = 0.f; s.pf32 = 0;
+    s.inl = s.slabs <= kInlineSlabs;
+    s.lanes = 1;
+    while (s.lanes < 64 && s.lanes * 4 < s.slabs) s.lanes *= 2;
     return true;
 }
 
@@ -56,6 +64,12 @@ __device__ __forceinline__ bool my_place(const Shape& s, uint32_t& pp, uint32_t&
     cv = threadIdx.x - pp * s.cvs;
     return threadIdx.x < s.ppi * s.cvs;
 }
+// the groups of a thread's 8 channels, and a walk through them
+struct GroupWalk {
+    uint32_t g, r;
+    __device__ __forceinline__ GroupWalk(const Shape& s, uint32_t c) : g(c / s.cpg), r(c - g * s.cpg) {}
+    __device__ __forceinline__ void next(const Shape& s) { if (++r == s.cpg) { r = 0; g++; } }
+};
 template <typename T> __device__ __forceinline__ float pivot_of(const T* x, const T* pre, const Shape& s, uint32_t n, uint32_t g) {
     const float p = pre ? (float)pre[(size_t)n * s.C + g * s.cpg] : 0.f;
     return (float)x[(size_t)n * s.HW * s.C + g * s.cpg] + p;
@@ -65,20 +79,63 @@ __device__ __forceinline__ double wave_sum(double v) {
     for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
     return v;
 }
+// Slab partials of the groups' two sums: item k = 2 g + which of slab w at k * item + w * slab behind the sample's first. Combined inline they
+// lie slab by slab (a workgroup reads whole rows), for the finish kernels item by item (a wave reads one item's).
+struct Partials { uint32_t item, slab; };
+__host__ __device__ inline Partials partials_of(const Shape& s) { return s.inl ? Partials{1u, 2u * s.G} : Partials{s.slabs, 1u}; }
+
+// every workgroup's own combination: sums[2 G] in LDS (doubles), scr LDS doubles [threads]; the same order in every workgroup
+__device__ __forceinline__ void combine_inline(const Shape& s, const float* __restrict__ partial, double* scr, double* sums) {
+    const uint32_t K = 2 * s.G, J = s.threads >= K ? s.threads / K : 1u;
+    for (uint32_t k0 = 0; k0 < K; k0 += s.threads) {                      // (one round unless the workgroup has fewer threads than items)
+        const uint32_t j = threadIdx.x / (K < s.threads ? K : s.threads), k = k0 + threadIdx.x - j * (K < s.threads ? K : s.threads);
+        double a = 0.0;
+        if (j < J && k < K) {
+            for (uint32_t w = j; w < s.slabs; w += 8 * J) {                // eight partials a trip, loaded together
+                float v[8];
+#pragma unroll
+                for (uint32_t u = 0; u < 8; u++) v[u] = partial[(size_t)min(w + u * J, s.slabs - 1) * K + k];
+#pragma unroll
+                for (uint32_t u = 0; u < 8; u++)
+                    if (w + u * J < s.slabs) a += (double)v[u];
+            }
+        }
+        scr[threadIdx.x] = a;
+        __syncthreads();
+        if (j == 0 && k < K) {
+            for (uint32_t i = 1; i < J; i++) a += scr[threadIdx.x + i * K];
+            sums[k] = a;
+        }
+        __syncthreads();
+    }
+}
+template <typename T>
+__device__ __forceinline__ void moments(const Shape& s, const T* x, const T* pre, uint32_t n, uint32_t g, double a, double b, float& mean, float& rstd) {
+    const double cnt = (double)s.HW * s.cpg;
+    a /= cnt; b /= cnt;
+    double var = b - a * a;
+    var = var > 0.0 || var != var ? var : 0.0;                             // (a NaN stays one)
+    mean = (float)((double)pivot_of(x, pre, s, n, g) + a);
+    rstd = (float)(1.0 / sqrt(var + (double)s.eps));
+}
 
 // ---- forward --------------------------------------------------------------------------------------------------------------------
-// partial[n][g][which][slab]
 template <typename T>
 __global__ __launch_bounds__(kMaxThreads) void k_stats(const T* __restrict__ x, const T* __restrict__ pre, Shape s, float* __restrict__ partial) {
     extern __shared__ float part[];          // [2][ppi][C], then [2][C]
     const uint32_t n = blockIdx.x / s.slabs, slab = blockIdx.x - n * s.slabs;
     uint32_t pp, cv;
     if (my_place(s, pp, cv)) {
-        float e[8], sum[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sq[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        float e[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sum[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sq[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (pre) widen(load8(pre + (size_t)n * s.C + cv * 8), e);
+        GroupWalk w(s, cv * 8);
+        float pivot = pivot_of(x, pre, s, n, w.g);
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const uint32_t c = cv * 8 + i;
-            e[i] = (pre ? (float)pre[(size_t)n * s.C + c] : 0.f) - pivot_of(x, pre, s, n, c / s.cpg);
+            e[i] -= pivot;
+            const uint32_t g = w.g;
+            w.next(s);
+            if (i < 7 && w.g != g) pivot = pivot_of(x, pre, s, n, w.g);
         }
         const uint32_t p1 = min((slab + 1) * s.P, s.HW);
         const T* base = x + (size_t)n * s.HW * s.C + cv * 8;
@@ -110,11 +167,12 @@ __global__ __launch_bounds__(kMaxThreads) void k_stats(const T* __restrict__ x, 
         chan[k] = a;
     }
     __syncthreads();
+    const Partials lay = partials_of(s);
     for (uint32_t k = threadIdx.x; k < 2 * s.G; k += s.threads) {
-        const uint32_t which = k >= s.G, g = k - which * s.G;
+        const uint32_t which = k & 1u, g = k >> 1;
         float a = 0.f;
         for (uint32_t c = 0; c < s.cpg; c++) a += chan[which * s.C + g * s.cpg + c];
-        partial[(((size_t)n * s.G + g) * 2 + which) * s.slabs + slab] = a;
+        partial[(size_t)n * 2 * s.G * s.slabs + (size_t)k * lay.item + (size_t)slab * lay.slab] = a;
     }
 }
 
@@ -127,31 +185,36 @@ __global__ __launch_bounds__(64) void k_finish(const T* __restrict__ x, const T*
     double a = 0.0, b = 0.0;
     for (uint32_t w = threadIdx.x; w < s.slabs; w += 64) { a += (double)p[w]; b += (double)p[s.slabs + w]; }
     a = wave_sum(a); b = wave_sum(b);
-    if (threadIdx.x == 0) {
-        const double cnt = (double)s.HW * s.cpg;
-        a /= cnt; b /= cnt;
-        double var = b - a * a;
-        var = var > 0.0 || var != var ? var : 0.0;                 // (a NaN stays one)
-        mean_rstd[(size_t)blockIdx.x * 2] = (float)((double)pivot_of(x, pre, s, n, g) + a);
-        mean_rstd[(size_t)blockIdx.x * 2 + 1] = (float)(1.0 / sqrt(var + (double)s.eps));
-    }
+    if (threadIdx.x == 0) moments(s, x, pre, n, g, a, b, mean_rstd[(size_t)blockIdx.x * 2], mean_rstd[(size_t)blockIdx.x * 2 + 1]);
 }
 
 template <typename T, bool ACT, bool Q8>
-__global__ __launch_bounds__(kMaxThreads) void k_apply(const T* __restrict__ x, const T* __restrict__ pre, Shape s, const float* __restrict__ mean_rstd,
-                                                        const void* __restrict__ gamma, const void* __restrict__ beta, T* __restrict__ y,
-                                                        u2n* __restrict__ codes, uint8_t* __restrict__ scales) {
+__global__ __launch_bounds__(kMaxThreads) void k_apply(const T* __restrict__ x, const T* __restrict__ pre, Shape s, const float* __restrict__ partial,
+                                                        float* __restrict__ mean_rstd, const void* __restrict__ gamma, const void* __restrict__ beta,
+                                                        T* __restrict__ y, u2n* __restrict__ codes, uint8_t* __restrict__ scales) {
+    __shared__ double scr[kMaxThreads], sums[2 * kMaxGroups];
+    __shared__ float mom[2 * kMaxGroups];
     const uint32_t n = blockIdx.x / s.slabs, slab = blockIdx.x - n * s.slabs;
+    if (s.inl) {
+        combine_inline(s, partial + (size_t)n * 2 * s.G * s.slabs, scr, sums);
+        for (uint32_t g = threadIdx.x; g < s.G; g += s.threads) {
+            moments(s, x, pre, n, g, sums[2 * g], sums[2 * g + 1], mom[2 * g], mom[2 * g + 1]);
+            if (slab == 0) { mean_rstd[((size_t)n * s.G + g) * 2] = mom[2 * g]; mean_rstd[((size_t)n * s.G + g) * 2 + 1] = mom[2 * g + 1]; }
+        }
+    } else
+        for (uint32_t k = threadIdx.x; k < 2 * s.G; k += s.threads) mom[k] = mean_rstd[(size_t)n * s.G * 2 + k];
+    __syncthreads();
     uint32_t pp, cv;
     if (!my_place(s, pp, cv)) return;
-    float mean[8], a[8], b[8];
+    float a[8], b[8], e[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    load_params<T>(gamma, cv * 8, s.pf32, a);
+    load_params<T>(beta, cv * 8, s.pf32, b);
+    if (pre) widen(load8(pre + (size_t)n * s.C + cv * 8), e);
+    GroupWalk w(s, cv * 8);
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const uint32_t c = cv * 8 + i, g = c / s.cpg;
-        const float* mr = mean_rstd + ((size_t)n * s.G + g) * 2;
-        mean[i] = mr[0] - (pre ? (float)pre[(size_t)n * s.C + c] : 0.f);
-        a[i] = mr[1] * load_param<T>(gamma, c, s.pf32);
-        b[i] = load_param<T>(beta, c, s.pf32);
+    for (int i = 0; i < 8; i++, w.next(s)) {
+        a[i] *= mom[2 * w.g + 1];
+        b[i] = __builtin_fmaf(e[i] - mom[2 * w.g], a[i], b[i]);           // (x + e - mean) a + beta = x a + b
     }
     const uint32_t p1 = min((slab + 1) * s.P, s.HW);
     const size_t at0 = (size_t)n * s.HW * s.cvs + cv;
@@ -172,7 +235,7 @@ __global__ __launch_bounds__(kMaxThreads) void k_apply(const T* __restrict__ x, 
             }
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float z = __builtin_fmaf(f[i] - mean[i], a[i], b[i]);
+                const float z = __builtin_fmaf(f[i], a[i], b[i]);
                 f[i] = ACT ? z * fast_sigmoid(z) : z;
             }
             store8(y + at * 8, f);
@@ -186,28 +249,37 @@ template <bool ACT> __device__ __forceinline__ float dz_of(float xh, float dy, f
     const float z = __builtin_fmaf(xh, gamma, beta), sg = fast_sigmoid(z);
     return dy * sg * __builtin_fmaf(z, 1.0f - sg, 1.0f);
 }
+// what a backward thread keeps of its 8 channels: xh = x r + m
+struct Chan8 { float r[8], m[8], ga[8], be[8]; };
+template <typename T>
+__device__ __forceinline__ void load_chan(Chan8& k, const Shape& s, uint32_t n, uint32_t cv, const float* mean_rstd, const T* pre, const void* gamma, const void* beta) {
+    float e[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    load_params<T>(gamma, cv * 8, s.pf32, k.ga);
+    load_params<T>(beta, cv * 8, s.pf32, k.be);
+    if (pre) widen(load8(pre + (size_t)n * s.C + cv * 8), e);
+    GroupWalk w(s, cv * 8);
+#pragma unroll
+    for (int i = 0; i < 8; i++, w.next(s)) {
+        const float* mr = mean_rstd + ((size_t)n * s.G + w.g) * 2;
+        k.r[i] = mr[1];
+        k.m[i] = (e[i] - mr[0]) * mr[1];
+    }
+}
 
-// partial[n][which][c][slab], which: sum dz, sum dz xh and (with pre) sum xh
-template <typename T, bool ACT, bool Q8>
+// chan[n][which][c][slab], which: sum dz, sum dz xh and (PRE) sum xh; partial: the groups' sums of g = dz gamma and g xh
+template <typename T, bool ACT, bool Q8, bool PRE>
 __global__ __launch_bounds__(kMaxThreads) void k_bwd_stats(const void* __restrict__ x, const uint8_t* __restrict__ scales, const T* __restrict__ pre,
                                                             const T* __restrict__ dy, Shape s, const float* __restrict__ mean_rstd,
-                                                            const void* __restrict__ gamma, const void* __restrict__ beta, float* __restrict__ partial) {
-    extern __shared__ float part[];          // [3][ppi][C]
+                                                            const void* __restrict__ gamma, const void* __restrict__ beta, float* __restrict__ partial,
+                                                            float* __restrict__ chan) {
+    extern __shared__ float part[];          // [K][ppi][C], then gamma [C], then [2][C]
+    constexpr uint32_t K = PRE ? 3u : 2u;
     const uint32_t n = blockIdx.x / s.slabs, slab = blockIdx.x - n * s.slabs;
-    const uint32_t K = pre ? 3u : 2u;
     uint32_t pp, cv;
     if (my_place(s, pp, cv)) {
-        float mean[8], rstd[8], ga[8], be[8], s1[8], s2[8], s3[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const uint32_t c = cv * 8 + i, g = c / s.cpg;
-            const float* mr = mean_rstd + ((size_t)n * s.G + g) * 2;
-            mean[i] = mr[0] - (pre ? (float)pre[(size_t)n * s.C + c] : 0.f);
-            rstd[i] = mr[1];
-            ga[i] = load_param<T>(gamma, c, s.pf32);
-            be[i] = load_param<T>(beta, c, s.pf32);
-            s1[i] = s2[i] = s3[i] = 0.f;
-        }
+        Chan8 k;
+        load_chan(k, s, n, cv, mean_rstd, pre, gamma, beta);
+        float s1[8] = {0, 0, 0, 0, 0, 0, 0, 0}, s2[8] = {0, 0, 0, 0, 0, 0, 0, 0}, s3[8] = {0, 0, 0, 0, 0, 0, 0, 0};
         const uint32_t p1 = min((slab + 1) * s.P, s.HW);
         const size_t at0 = (size_t)n * s.HW * s.cvs + cv;
         for (uint32_t p = slab * s.P + pp; p < p1; p += kTrip * s.ppi) {
@@ -227,10 +299,10 @@ __global__ __launch_bounds__(kMaxThreads) void k_bwd_stats(const void* __restric
                 widen(vd[u], fd);
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const float xh = (fx[i] - mean[i]) * rstd[i], dz = dz_of<ACT>(xh, fd[i], ga[i], be[i]);
+                    const float xh = __builtin_fmaf(fx[i], k.r[i], k.m[i]), dz = dz_of<ACT>(xh, fd[i], k.ga[i], k.be[i]);
                     s1[i] += dz;
                     s2[i] = __builtin_fmaf(dz, xh, s2[i]);
-                    s3[i] += xh;
+                    if (PRE) s3[i] += xh;
                 }
             }
         }
@@ -239,143 +311,162 @@ __global__ __launch_bounds__(kMaxThreads) void k_bwd_stats(const void* __restric
             const size_t c = cv * 8 + i;
             part[(size_t)pp * s.C + c] = s1[i];
             part[(size_t)(s.ppi + pp) * s.C + c] = s2[i];
-            if (pre) part[(size_t)(2 * s.ppi + pp) * s.C + c] = s3[i];
+            if (PRE) part[(size_t)(2 * s.ppi + pp) * s.C + c] = s3[i];
+            if (pp == 0) part[K * s.ppi * s.C + c] = k.ga[i];
         }
     }
     __syncthreads();
+    const float* ga = part + K * s.ppi * s.C;
+    float* weighted = part + (K * s.ppi + 1) * s.C;
     for (uint32_t k = threadIdx.x; k < K * s.C; k += s.threads) {
         const uint32_t which = k / s.C, c = k - which * s.C;
         float a = 0.f;
         for (uint32_t p = 0; p < s.ppi; p++) a += part[(size_t)(which * s.ppi + p) * s.C + c];
-        partial[(((size_t)n * K + which) * s.C + c) * s.slabs + slab] = a;
+        chan[(((size_t)n * K + which) * s.C + c) * s.slabs + slab] = a;
+        if (which < 2) weighted[k] = a * ga[c];
+    }
+    __syncthreads();
+    const Partials lay = partials_of(s);
+    for (uint32_t k = threadIdx.x; k < 2 * s.G; k += s.threads) {
+        const uint32_t which = k & 1u, g = k >> 1;
+        float a = 0.f;
+        for (uint32_t c = 0; c < s.cpg; c++) a += weighted[which * s.C + g * s.cpg + c];
+        partial[(size_t)n * 2 * s.G * s.slabs + (size_t)k * lay.item + (size_t)slab * lay.slab] = a;
     }
 }
 
-// One workgroup per (sample, group), one wave per (which, channel) in turn: means[n][g][2], the channel sums chan[n][2][C] and dpre.
-constexpr uint32_t kFinishThreads = 512;
-template <typename T>
-__global__ __launch_bounds__(kFinishThreads) void k_bwd_finish(const float* __restrict__ partial, Shape s, const float* __restrict__ mean_rstd,
-                                                              const T* __restrict__ pre, const void* __restrict__ gamma, float* __restrict__ means,
-                                                              double* __restrict__ chan, T* __restrict__ dpre) {
-    extern __shared__ double sums[];          // [K][cpg]
-    __shared__ double mom[2];
-    const uint32_t n = blockIdx.x / s.G, g = blockIdx.x - n * s.G, K = pre ? 3u : 2u, items = K * s.cpg;
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    for (uint32_t k = wave; k < items; k += kFinishThreads / 64) {
-        const uint32_t which = k / s.cpg, c = g * s.cpg + (k - which * s.cpg);
-        const float* p = partial + (((size_t)n * K + which) * s.C + c) * s.slabs;
-        double a = 0.0;
-        for (uint32_t w = lane; w < s.slabs; w += 64) a += (double)p[w];
-        a = wave_sum(a);
-        if (lane == 0) {
-            sums[k] = a;
-            if (which < 2) chan[((size_t)n * 2 + which) * s.C + c] = a;
-        }
-    }
-    __syncthreads();
-    if (wave < 2) {                           // m1 = mean(g), m2 = mean(g xh)
-        double m = 0.0;
-        for (uint32_t c = lane; c < s.cpg; c += 64) m += sums[wave * s.cpg + c] * (double)load_param<T>(gamma, g * s.cpg + c, s.pf32);
-        m = wave_sum(m) / ((double)s.HW * s.cpg);
-        if (lane == 0) {
-            mom[wave] = m;
-            means[(size_t)blockIdx.x * 2 + wave] = (float)m;
-        }
-    }
-    if (!dpre) return;
-    __syncthreads();
-    const double rstd = (double)mean_rstd[(size_t)blockIdx.x * 2 + 1];
-    for (uint32_t k = threadIdx.x; k < s.cpg; k += kFinishThreads) {
-        const uint32_t c = g * s.cpg + k;
-        const double ga = (double)load_param<T>(gamma, c, s.pf32);
-        dpre[(size_t)n * s.C + c] = (T)(float)(rstd * (ga * sums[k] - (double)s.HW * mom[0] - mom[1] * sums[2 * s.cpg + k]));
-    }
+// one wave per (sample, group): the means of g and g xh
+__global__ __launch_bounds__(64) void k_bwd_finish(const float* __restrict__ partial, Shape s, float* __restrict__ means) {
+    const float* p = partial + (size_t)blockIdx.x * 2 * s.slabs;
+    double a = 0.0, b = 0.0;
+    for (uint32_t w = threadIdx.x; w < s.slabs; w += 64) { a += (double)p[w]; b += (double)p[s.slabs + w]; }
+    a = wave_sum(a); b = wave_sum(b);
+    const double cnt = (double)s.HW * s.cpg;
+    if (threadIdx.x == 0) { means[(size_t)blockIdx.x * 2] = (float)(a / cnt); means[(size_t)blockIdx.x * 2 + 1] = (float)(b / cnt); }
 }
 
-// dx, and (the first threads of the grid) dgamma / dbeta: the channel sums over samples in order. dx / dgamma / dbeta may be null.
-template <typename T, bool ACT, bool Q8>
+template <typename T, bool ACT, bool Q8, bool PRE>
 __global__ __launch_bounds__(kMaxThreads) void k_bwd_apply(const void* __restrict__ x, const uint8_t* __restrict__ scales, const T* __restrict__ pre,
                                                             const T* __restrict__ dy, Shape s, const float* __restrict__ mean_rstd,
-                                                            const float* __restrict__ means, const double* __restrict__ chan,
-                                                            const void* __restrict__ gamma, const void* __restrict__ beta, T* __restrict__ dx,
-                                                            void* __restrict__ dgamma, void* __restrict__ dbeta) {
-    if (dgamma || dbeta) {
-        for (uint32_t c = blockIdx.x * blockDim.x + threadIdx.x; c < s.C; c += gridDim.x * blockDim.x) {
-            double b = 0.0, g = 0.0;
-            for (uint32_t n = 0; n < s.N; n++) { b += chan[(size_t)n * 2 * s.C + c]; g += chan[((size_t)n * 2 + 1) * s.C + c]; }
-            if (dbeta) store_param<T>(dbeta, c, s.pf32, b);
-            if (dgamma) store_param<T>(dgamma, c, s.pf32, g);
-        }
-    }
-    if (!dx) return;
+                                                            const float* __restrict__ partial, const float* __restrict__ means,
+                                                            const float* __restrict__ chan, const void* __restrict__ gamma, const void* __restrict__ beta,
+                                                            T* __restrict__ dx, T* __restrict__ dpre, void* __restrict__ dgamma, void* __restrict__ dbeta) {
+    __shared__ double scr[kMaxThreads], sums[2 * kMaxGroups];
+    __shared__ float mom[2 * kMaxGroups];
+    constexpr uint32_t K = PRE ? 3u : 2u;
     const uint32_t n = blockIdx.x / s.slabs, slab = blockIdx.x - n * s.slabs;
+    if (s.inl) {
+        combine_inline(s, partial + (size_t)n * 2 * s.G * s.slabs, scr, sums);
+        const double cnt = (double)s.HW * s.cpg;
+        for (uint32_t k = threadIdx.x; k < 2 * s.G; k += s.threads) mom[k] = (float)(sums[k] / cnt);
+    } else
+        for (uint32_t k = threadIdx.x; k < 2 * s.G; k += s.threads) mom[k] = means[(size_t)n * s.G * 2 + k];
+    __syncthreads();
     uint32_t pp, cv;
-    if (!my_place(s, pp, cv)) return;
-    float mean[8], rstd[8], ga[8], be[8], m1[8], m2[8];
+    if (my_place(s, pp, cv) && dx) {
+        Chan8 k;
+        load_chan(k, s, n, cv, mean_rstd, pre, gamma, beta);
+        float m1[8], m2[8];
+        GroupWalk w(s, cv * 8);
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const uint32_t c = cv * 8 + i, g = c / s.cpg;
-        const size_t k = ((size_t)n * s.G + g) * 2;
-        mean[i] = mean_rstd[k] - (pre ? (float)pre[(size_t)n * s.C + c] : 0.f);
-        rstd[i] = mean_rstd[k + 1];
-        ga[i] = load_param<T>(gamma, c, s.pf32);
-        be[i] = load_param<T>(beta, c, s.pf32);
-        m1[i] = means[k]; m2[i] = means[k + 1];
-    }
-    const uint32_t p1 = min((slab + 1) * s.P, s.HW);
-    const size_t at0 = (size_t)n * s.HW * s.cvs + cv;
-    for (uint32_t p = slab * s.P + pp; p < p1; p += kTrip * s.ppi) {
-        Saved<T, Q8> vx[kTrip];
-        Raw8<T> vd[kTrip];
+        for (int i = 0; i < 8; i++, w.next(s)) { m1[i] = mom[2 * w.g]; m2[i] = mom[2 * w.g + 1]; }
+        const uint32_t p1 = min((slab + 1) * s.P, s.HW);
+        const size_t at0 = (size_t)n * s.HW * s.cvs + cv;
+        for (uint32_t p = slab * s.P + pp; p < p1; p += kTrip * s.ppi) {
+            Saved<T, Q8> vx[kTrip];
+            Raw8<T> vd[kTrip];
 #pragma unroll
-        for (uint32_t u = 0; u < kTrip; u++) {
-            const size_t at = at0 + (size_t)min(p + u * s.ppi, p1 - 1) * s.cvs;
-            vx[u] = load_saved<T, Q8>(x, scales, at);
-            vd[u] = load8(dy + at * 8);
-        }
-#pragma unroll
-        for (uint32_t u = 0; u < kTrip; u++) {
-            if (p + u * s.ppi >= p1) break;
-            float fx[8], fd[8];
-            widen_saved(vx[u], fx);
-            widen(vd[u], fd);
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float xh = (fx[i] - mean[i]) * rstd[i], dz = dz_of<ACT>(xh, fd[i], ga[i], be[i]);
-                fx[i] = rstd[i] * (__builtin_fmaf(dz, ga[i], -m1[i]) - xh * m2[i]);
+            for (uint32_t u = 0; u < kTrip; u++) {
+                const size_t at = at0 + (size_t)min(p + u * s.ppi, p1 - 1) * s.cvs;
+                vx[u] = load_saved<T, Q8>(x, scales, at);
+                vd[u] = load8(dy + at * 8);
             }
-            store8(dx + (at0 + (size_t)(p + u * s.ppi) * s.cvs) * 8, fx);
+#pragma unroll
+            for (uint32_t u = 0; u < kTrip; u++) {
+                if (p + u * s.ppi >= p1) break;
+                float fx[8], fd[8];
+                widen_saved(vx[u], fx);
+                widen(vd[u], fd);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float xh = __builtin_fmaf(fx[i], k.r[i], k.m[i]), dz = dz_of<ACT>(xh, fd[i], k.ga[i], k.be[i]);
+                    fx[i] = k.r[i] * (__builtin_fmaf(dz, k.ga[i], -m1[i]) - xh * m2[i]);
+                }
+                store8(dx + (at0 + (size_t)(p + u * s.ppi) * s.cvs) * 8, fx);
+            }
+        }
+    }
+    // The channels' gradients: L lanes to a channel (about four slabs a lane), the grid's lane groups in turn (dpre within the sample's
+    // workgroups, dgamma / dbeta in the first sample's).
+    const uint32_t L = s.lanes, sub = threadIdx.x & (L - 1u), per_wg = s.threads / L, first = slab * per_wg + threadIdx.x / L, stride = s.slabs * per_wg;
+    auto total = [&](uint32_t nn, uint32_t which, uint32_t c) {
+        const float* p = chan + (((size_t)nn * K + which) * s.C + c) * s.slabs;
+        double a = 0.0;
+        for (uint32_t w = sub; w < s.slabs; w += 4 * L) {
+            float v[4];
+#pragma unroll
+            for (uint32_t u = 0; u < 4; u++) v[u] = p[min(w + u * L, s.slabs - 1)];
+#pragma unroll
+            for (uint32_t u = 0; u < 4; u++)
+                if (w + u * L < s.slabs) a += (double)v[u];
+        }
+        for (uint32_t o = L / 2; o >= 1; o >>= 1) a += __shfl_xor(a, o, 64);
+        return a;
+    };
+    if (PRE && dpre) {
+        for (uint32_t c = first; c < s.C; c += stride) {
+            const double a = total(n, 0, c), h = total(n, 2, c);
+            const uint32_t g = c / s.cpg;
+            const double rstd = (double)mean_rstd[((size_t)n * s.G + g) * 2 + 1], ga = (double)load_param<T>(gamma, c, s.pf32);
+            if (sub == 0) dpre[(size_t)n * s.C + c] = (T)(float)(rstd * (ga * a - (double)s.HW * (double)mom[2 * g] - (double)mom[2 * g + 1] * h));
+        }
+    }
+    if (n == 0 && (dgamma || dbeta)) {
+        for (uint32_t c = first; c < s.C; c += stride) {
+            double a = 0.0, b = 0.0;
+            for (uint32_t nn = 0; nn < s.N; nn++) { a += total(nn, 0, c); b += total(nn, 1, c); }
+            if (sub == 0) {
+                if (dbeta) store_param<T>(dbeta, c, s.pf32, a);
+                if (dgamma) store_param<T>(dgamma, c, s.pf32, b);
+            }
         }
     }
 }
 
 // ---- launches -------------------------------------------------------------------------------------------------------------------
-uint64_t partial_floats(const Shape& s) { return (uint64_t)s.N * 3 * s.C * s.slabs; }
+uint64_t group_floats(const Shape& s) { return (uint64_t)s.N * 2 * s.G * s.slabs; }
+uint64_t chan_floats(const Shape& s) { return (uint64_t)s.N * 3 * s.C * s.slabs; }
 
 template <typename T, bool ACT, bool Q8>
 void forward(const void* x_, const void* pre_, const void* gamma, const void* beta, const Shape& s, void* y, uint8_t* saved, float* mean_rstd,
              float* scratch, hipStream_t st) {
     const T *x = static_cast<const T*>(x_), *pre = static_cast<const T*>(pre_);
     hipLaunchKernelGGL(k_stats<T>, dim3(s.N * s.slabs), dim3(s.threads), (2 * s.ppi + 2) * s.C * 4, st, x, pre, s, scratch);
-    hipLaunchKernelGGL(k_finish<T>, dim3(s.N * s.G), dim3(64), 0, st, x, pre, scratch, s, mean_rstd);
-    hipLaunchKernelGGL((k_apply<T, ACT, Q8>), dim3(s.N * s.slabs), dim3(s.threads), 0, st, x, pre, s, mean_rstd, gamma, beta, static_cast<T*>(y),
+    if (!s.inl) hipLaunchKernelGGL(k_finish<T>, dim3(s.N * s.G), dim3(64), 0, st, x, pre, scratch, s, mean_rstd);
+    hipLaunchKernelGGL((k_apply<T, ACT, Q8>), dim3(s.N * s.slabs), dim3(s.threads), 0, st, x, pre, s, scratch, mean_rstd, gamma, beta, static_cast<T*>(y),
                        reinterpret_cast<u2n*>(saved), saved + (size_t)s.N * s.HW * s.C);
 }
-template <typename T, bool ACT, bool Q8>
-void backward(const void* x, const void* pre_, const void* dy_, const void* gamma, const void* beta, const float* mean_rstd, const Shape& s,
-              void* dx, void* dpre, void* dgamma, void* dbeta, float* scratch, hipStream_t st) {
-    const T *pre = static_cast<const T*>(pre_), *dy = static_cast<const T*>(dy_);
+template <typename T, bool ACT, bool Q8, bool PRE>
+void backward_pre(const void* x, const T* pre, const T* dy, const void* gamma, const void* beta, const float* mean_rstd, const Shape& s, T* dx, T* dpre,
+                  void* dgamma, void* dbeta, float* scratch, hipStream_t st) {
     const uint8_t* scales = Q8 ? static_cast<const uint8_t*>(x) + (size_t)s.N * s.HW * s.C : nullptr;
-    float* means = scratch + partial_floats(s);
-    double* chan = reinterpret_cast<double*>(means + (size_t)s.N * s.G * 2);          // (partial_floats is a multiple of 8)
-    const uint32_t K = pre ? 3 : 2;
-    hipLaunchKernelGGL((k_bwd_stats<T, ACT, Q8>), dim3(s.N * s.slabs), dim3(s.threads), K * s.ppi * s.C * 4, st, x, scales, pre, dy, s, mean_rstd,
-                       gamma, beta, scratch);
-    hipLaunchKernelGGL(k_bwd_finish<T>, dim3(s.N * s.G), dim3(kFinishThreads), K * s.cpg * 8, st, scratch, s, mean_rstd, pre, gamma, means, chan,
-                       static_cast<T*>(dpre));
-    if (dx || dgamma || dbeta)
-        hipLaunchKernelGGL((k_bwd_apply<T, ACT, Q8>), dim3(s.N * s.slabs), dim3(s.threads), 0, st, x, scales, pre, dy, s, mean_rstd, means, chan, gamma,
-                           beta, static_cast<T*>(dx), dgamma, dbeta);
+    float *partial = scratch, *chan = partial + group_floats(s), *means = chan + chan_floats(s);
+    const uint32_t K = PRE ? 3 : 2;
+    hipLaunchKernelGGL((k_bwd_stats<T, ACT, Q8, PRE>), dim3(s.N * s.slabs), dim3(s.threads), (K * s.ppi + 3) * s.C * 4, st, x, scales, pre, dy, s,
+                       mean_rstd, gamma, beta, partial, chan);
+    if (!s.inl) hipLaunchKernelGGL(k_bwd_finish, dim3(s.N * s.G), dim3(64), 0, st, partial, s, means);
+    hipLaunchKernelGGL((k_bwd_apply<T, ACT, Q8, PRE>), dim3(s.N * s.slabs), dim3(s.threads), 0, st, x, scales, pre, dy, s, mean_rstd, partial, means,
+                       chan, gamma, beta, dx, dpre, dgamma, dbeta);
+}
+template <typename T, bool ACT, bool Q8>
+void backward(const void* x, const void* pre, const void* dy, const void* gamma, const void* beta, const float* mean_rstd, const Shape& s,
+              void* dx, void* dpre, void* dgamma, void* dbeta, float* scratch, hipStream_t st) {
+    const T* dyp = static_cast<const T*>(dy);
+    if (pre)
+        backward_pre<T, ACT, Q8, true>(x, static_cast<const T*>(pre), dyp, gamma, beta, mean_rstd, s, static_cast<T*>(dx), static_cast<T*>(dpre), dgamma,
+                                       dbeta, scratch, st);
+    else
+        backward_pre<T, ACT, Q8, false>(x, nullptr, dyp, gamma, beta, mean_rstd, s, static_cast<T*>(dx), nullptr, dgamma, dbeta, scratch, st);
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -406,7 +497,7 @@ extern "C" {
 uint64_t sdfx_group_norm_train_scratch_bytes(uint32_t N, uint32_t HW, uint32_t C, uint32_t G) {
     Shape s;
     if (!make_shape(N, HW, C, G, s)) return 0;
-    return (partial_floats(s) + (uint64_t)N * G * 2) * sizeof(float) + (uint64_t)N * 2 * C * sizeof(double);
+    return (group_floats(s) + chan_floats(s) + (uint64_t)N * G * 2) * sizeof(float);
 }
 
 int sdfx_group_norm_train_forward(const void* x, const void* pre, const void* gamma, const void* beta, uint32_t N, uint32_t HW, uint32_t C, uint32_t G,
@@ -418,7 +509,7 @@ int sdfx_group_norm_train_forward(const void* x, const void* pre, const void* ga
     SDFX_REQUIRE(make_shape(N, HW, C, G, s), "group_norm_train_forward: needs C %% 8 == 0, C %% G == 0, C <= %u, G <= %u (got N=%u HW=%u C=%u G=%u)",
                  kMaxThreads * 8, kMaxGroups, N, HW, C, G);
     SDFX_REQUIRE(!saved8 || C % 32 == 0, "group_norm_train_forward: the 8-bit form needs C %% 32 == 0 (got %u)", C);
-    SDFX_REQUIRE(aligned16(x) && aligned16(y) && aligned16(saved8), "group_norm_train_forward: x / y / saved8 misaligned");
+    SDFX_REQUIRE(aligned16(x) && aligned16(y) && aligned16(saved8) && aligned16(pre) && aligned16(gamma) && aligned16(beta), "group_norm_train_forward: misaligned pointer");
     SDFX_REQUIRE(eps >= 0.f, "group_norm_train_forward: negative eps");
     s.eps = eps; s.pf32 = params_f32 || dtype == 2;
     const bool eight = saved8 != nullptr;
@@ -436,7 +527,7 @@ int sdfx_group_norm_train_backward(const void* x, int eight_bits, const void* pr
                  kMaxThreads * 8, kMaxGroups, N, HW, C, G);
     SDFX_REQUIRE(!eight_bits || C % 32 == 0, "group_norm_train_backward: the 8-bit form needs C %% 32 == 0 (got %u)", C);
     SDFX_REQUIRE(pre || !dpre, "group_norm_train_backward: dpre without pre");
-    SDFX_REQUIRE(aligned16(x) && aligned16(dy) && aligned16(dx), "group_norm_train_backward: x / dy / dx misaligned");
+    SDFX_REQUIRE(aligned16(x) && aligned16(dy) && aligned16(dx) && aligned16(pre) && aligned16(gamma) && aligned16(beta), "group_norm_train_backward: misaligned pointer");
     s.pf32 = params_f32 || dtype == 2;
     const bool eight = eight_bits != 0;
     SDFX_GN_DISPATCH(backward, x, pre, dy, gamma, beta, mean_rstd, s, dx, dpre, dgamma, dbeta, scratch, as_stream(stream));

@@ -149,7 +149,8 @@ struct Norm : torch::autograd::Function<Norm> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x0, const std::optional<Tensor>& pre0, const Tensor& w0, const Tensor& b0, int64_t G, double eps,
                           bool act, bool eight, bool keep) {
         const c10::DeviceGuard guard(x0.device());
-        const Tensor x = dense16(x0, at::MemoryFormat::ChannelsLast), pre = pre0 ? pre0->contiguous() : Tensor(), w = w0.contiguous(), b = b0.contiguous();
+        const Tensor x = dense16(x0, at::MemoryFormat::ChannelsLast), pre = pre0 ? dense16(*pre0, at::MemoryFormat::Contiguous) : Tensor(),
+                     w = dense16(w0, at::MemoryFormat::Contiguous), b = dense16(b0, at::MemoryFormat::Contiguous);
         const int64_t N = x.size(0), C = x.size(1), HW = x.size(2) * x.size(3);
         const Tensor y = at::empty_like(x), stats = at::empty({N, G, 2}, x.options().dtype(at::kFloat));
         Tensor saved, scratch;
