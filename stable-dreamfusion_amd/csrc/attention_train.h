@@ -103,7 +103,8 @@ constexpr uint32_t kTileSlack = 64;
 
 // A thread's chunks of a tile: where each lies behind the tile's first row in memory (bytes; the first row's address is a scalar) and in LDS.
 // Only the D / 8 chunks a row has are moved; a kernel that reads further clears LDS once. A thread without a chunk of its own reads the
-// tile's last one and writes it to the 16 bytes behind the tile: no predicates in the loop.
+// tile's last one and writes it to the 16 bytes behind the tile: no predicate and no branch around a load (scalar branches there cost
+// 30 % of the dq kernel: the loads of a branch are waited for at its end).
 template <typename L, int TH> struct Stage {
     uint32_t src[L::PT], dst[L::PT];
     __device__ __forceinline__ void init(uint32_t D, uint64_t sn, uint32_t tid) {
@@ -180,13 +181,14 @@ template <typename T> __device__ __forceinline__ void store4(T* p, float a, floa
 // |dp - delta| <= 2 M, M = max |do row| max |v row| over the key head's rows (attention_train.hip: k_prep leaves the squares of
 // block maxima): g = 2^-k with 2 M g <= 1, so |2^15 p g (dp - delta)| <= 2^15 whatever the loss scale, and gradients down to 2^-29 of
 // that bound are normal numbers.
-__device__ __forceinline__ float grad_scale(const float* rows2, uint32_t nr, const float* v2, uint32_t nv, uint32_t lane) {
+__device__ __forceinline__ float grad_scale(const float* rows2, uint32_t nr, const float* v2, uint32_t nv, uint32_t lane, float& vmax) {
     float a = 0.f, b = 0.f;
     for (uint32_t i = lane; i < nr; i += 64) a = fmaxf(a, rows2[i]);
     for (uint32_t i = lane; i < nv; i += 64) b = fmaxf(b, v2[i]);
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) { a = fmaxf(a, __shfl_xor(a, o, 64)); b = fmaxf(b, __shfl_xor(b, o, 64)); }
-    const float m = sqrtf(a) * sqrtf(b);
+    vmax = sqrtf(b);
+    const float m = sqrtf(a) * vmax;
     if (!(m > 0.f) || m > 1e37f) return 1.f;
     const uint32_t e = __float_as_uint(m) >> 23;
     return __uint_as_float((252u - min(e, 251u)) << 23);

@@ -103,11 +103,13 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_fwd(const T* __re
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 __builtin_amdgcn_s_setprio(1);            // (a wave in its softmax ahead of one that feeds the matrix cores: the two overlap)
-                float mx = -INFINITY;
+                float mx = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
-                for (int st = 0; st < NB; st++)
-#pragma unroll
-                    for (int r = 0; r < 16; r++) mx = fmaxf(mx, sc[st][r]);
+                for (int r = 0; r < 16; r++) {
+                    mx = fmaxf(mx, sc[0][r]);
+                    if (NB == 2) mx1 = fmaxf(mx1, sc[NB - 1][r]);
+                }
+                mx = fmaxf(mx, mx1);
                 mx = max_halves(mx) * s.c;
                 if (__ballot(mx > m_run)) {               // (some row has a new maximum: rare after the first tiles)
                     const float m_new = fmaxf(m_run, mx), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
@@ -187,7 +189,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void k_join_o(const float* __restrict__ part, const float* __restrict__ ml, Shape s, uint32_t parts, T* __restrict__ o,
                                                T* __restrict__ o_lo, float* __restrict__ lse) {
     __shared__ f4 red[256];
-    __shared__ float redl[256];
+    __shared__ float redl[256], redm[256];
     const uint32_t quads = s.D / 4, per = quads * parts, rows_here = 256u / per;
     const uint64_t total = (uint64_t)s.B * s.H * s.Nq;
     const uint32_t local = threadIdx.x / per, in_row = threadIdx.x - local * per, pt = in_row / quads, c0 = (in_row - pt * quads) * 4;
@@ -196,24 +198,43 @@ __global__ __launch_bounds__(256) void k_join_o(const float* __restrict__ part, 
     float m = -1e30f, l = 0.f;
     f4 a = {0.f, 0.f, 0.f, 0.f};
     if (on) {
-#pragma unroll 8
-        for (uint32_t i = 0; i < s.splits; i++) m = fmaxf(m, ml[2 * (i * total + r)]);
         const uint32_t n = (s.splits + parts - 1) / parts, i1 = min((pt + 1) * n, s.splits);
-#pragma unroll 4
-        for (uint32_t i = pt * n; i < i1; i++) {
-            const uint64_t at = i * total + r;
-            const float li = ml[2 * at + 1], w = li == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml[2 * at] - m);      // (0: nothing seen in this range)
-            const f4 p = *reinterpret_cast<const f4*>(part + at * s.D + c0);
-            l = __builtin_fmaf(w, li, l);
+        for (uint32_t i = pt * n; i < i1; i += 4) {               // four splits a trip, loaded together; the sum follows their maximum
+            float mi[4], li[4];
+            f4 p[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) a[j] = __builtin_fmaf(w, p[j], a[j]);
+            for (uint32_t u = 0; u < 4; u++) {
+                const uint64_t at = min(i + u, i1 - 1u) * total + r;
+                mi[u] = ml[2 * at];
+                li[u] = i + u < i1 ? ml[2 * at + 1] : 0.f;
+                p[u] = *reinterpret_cast<const f4*>(part + at * s.D + c0);
+            }
+            const float mn = fmaxf(fmaxf(fmaxf(mi[0], mi[1]), fmaxf(mi[2], mi[3])), m), alpha = __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= alpha;
+            a = a * alpha;
+#pragma unroll
+            for (uint32_t u = 0; u < 4; u++) {
+                const float w = li[u] == 0.f ? 0.f : __builtin_amdgcn_exp2f(mi[u] - mn);                          // (0: nothing seen in this range)
+                l = __builtin_fmaf(w, li[u], l);
+#pragma unroll
+                for (int j = 0; j < 4; j++) a[j] = __builtin_fmaf(w, p[u][j], a[j]);
+            }
         }
     }
     red[threadIdx.x] = a;
     redl[threadIdx.x] = l;
+    redm[threadIdx.x] = m;
     __syncthreads();
     if (!on || pt) return;
-    for (uint32_t i = 1; i < parts; i++) { a += red[threadIdx.x + i * quads]; l += redl[threadIdx.x + i * quads]; }
+    for (uint32_t i = 1; i < parts; i++) m = fmaxf(m, redm[threadIdx.x + i * quads]);
+    l = 0.f;
+    a = f4{0.f, 0.f, 0.f, 0.f};
+    for (uint32_t i = 0; i < parts; i++) {
+        const float w = __builtin_amdgcn_exp2f(redm[threadIdx.x + i * quads] - m);
+        a += red[threadIdx.x + i * quads] * w;
+        l = __builtin_fmaf(redl[threadIdx.x + i * quads], w, l);
+    }
     const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
     const uint32_t bh = (uint32_t)(r / s.Nq), qi = (uint32_t)(r - (uint64_t)bh * s.Nq), b = bh / s.H, h = bh - b * s.H;
     const size_t at = (((size_t)b * s.Nq + qi) * s.H + h) * s.D + c0;
@@ -223,21 +244,30 @@ __global__ __launch_bounds__(256) void k_join_o(const float* __restrict__ part, 
     if (o_lo) store4(o_lo + at, a[0] - (float)(T)a[0], a[1] - (float)(T)a[1], a[2] - (float)(T)a[2], a[3] - (float)(T)a[3]);
 }
 
-// out[b, n, h, :] = sum over splits of part[split][b, h, n, :], in order (gridDim.y: a second pair)
+// out[b, n, h, :] = sum over splits of part[split][b, h, n, :], in order, for each of the gradients that were split (blockIdx.y)
+struct JoinSum { const float* part; void* out; uint32_t splits, H, N; };
+struct JoinSums { JoinSum of[3]; };
 template <typename T>
-__global__ __launch_bounds__(256) void k_join_sum(const float* __restrict__ pa, const float* __restrict__ pb, uint32_t splits, uint32_t B, uint32_t H,
-                                                 uint32_t N, uint32_t D, T* __restrict__ oa, T* __restrict__ ob) {
-    const float* part = blockIdx.y ? pb : pa;
-    T* out = blockIdx.y ? ob : oa;
+__global__ __launch_bounds__(256) void k_join_sum(JoinSums js, uint32_t B, uint32_t D) {
+    const JoinSum j = js.of[blockIdx.y];
     const uint32_t per = D / 4;
-    const uint64_t total = (uint64_t)B * H * N, id = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    const uint64_t total = (uint64_t)B * j.H * j.N, id = (uint64_t)blockIdx.x * 256 + threadIdx.x;
     if (id >= total * per) return;
     const uint64_t r = id / per;
     const uint32_t c0 = (uint32_t)(id - r * per) * 4;
     f4 a = {0.f, 0.f, 0.f, 0.f};
-    for (uint32_t i = 0; i < splits; i++) a += *reinterpret_cast<const f4*>(part + (i * total + r) * D + c0);
-    const uint32_t bh = (uint32_t)(r / N), n = (uint32_t)(r - (uint64_t)bh * N), b = bh / H, h = bh - b * H;
-    store4(out + (((size_t)b * N + n) * H + h) * D + c0, a[0], a[1], a[2], a[3]);
+    const float* p = j.part + r * D + c0;
+    const uint64_t step = total * D;
+    for (uint32_t i = 0; i < j.splits; i += 8) {                  // eight splits a trip, loaded together; added in order
+        f4 v[8];
+#pragma unroll
+        for (uint32_t u = 0; u < 8; u++) v[u] = *reinterpret_cast<const f4*>(p + min(i + u, j.splits - 1u) * step);
+#pragma unroll
+        for (uint32_t u = 0; u < 8; u++)
+            if (i + u < j.splits) a += v[u];
+    }
+    const uint32_t bh = (uint32_t)(r / j.N), n = (uint32_t)(r - (uint64_t)bh * j.N), b = bh / j.H, h = bh - b * j.H;
+    store4(static_cast<T*>(j.out) + (((size_t)b * j.N + n) * j.H + h) * D + c0, a[0], a[1], a[2], a[3]);
 }
 
 // ---- ahead of the gradient's kernels ---------------------------------------------------------------------------------------------
@@ -270,15 +300,17 @@ __global__ __launch_bounds__(256) void k_prep(const T* __restrict__ v, const T* 
         } else {
             const uint32_t g = r / s.Nq, qi = r - g * s.Nq;
             at = (((size_t)b * s.Nq + qi) * s.H + hk * s.group + g) * s.D + c0;
-            if (c0 < s.D && lse[(size_t)bh * s.rows + r] != INFINITY) {          // (the dy of a row that sees nothing may be anything)
+            if (c0 < s.D) {
                 const typename Half<T>::v8 y = *reinterpret_cast<const typename Half<T>::v8*>(dy + at), a = *reinterpret_cast<const typename Half<T>::v8*>(o + at),
                                            l = *reinterpret_cast<const typename Half<T>::v8*>(o_lo + at);
+                const bool on = lse[(size_t)bh * s.rows + r] != INFINITY;          // (the dy of a row that sees nothing may be anything)
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     const float f = (float)y[i];
                     d = __builtin_fmaf(f, (float)a[i] + (float)l[i], d);
                     q = __builtin_fmaf(f, f, q);
                 }
+                if (!on) d = q = 0.f;
             }
         }
 #pragma unroll
@@ -297,22 +329,23 @@ __global__ __launch_bounds__(256) void k_prep(const T* __restrict__ v, const T* 
 
 // ---- launches -----------------------------------------------------------------------------------------------------------------------
 // Workgroups of 4 waves share their tiles; 32 rows or fewer (a few queries against a long cache) take one wave each. Where that leaves CUs
-// without work the other axis is split, at least `least` tiles to a workgroup: a split costs float32 partials and a launch that adds them.
+// without work the other axis is split, two tiles at least to a workgroup: a split costs float32 partials and a launch that adds them (2 x 12
+// causal rows of 1001 x 64 make 192 workgroups: forward 31 us whole, 19 + 7 in three splits).
 constexpr uint32_t kCus = 256;
-void plan(Shape& s, uint32_t along, uint32_t other_tiles, int waves, uint32_t least) {
+void plan(Shape& s, uint32_t along, uint32_t other_tiles, int waves) {
     s.tiles_x = div_up(along, 32u * waves);
     const uint64_t base = (uint64_t)s.tiles_x * s.B * s.Hk, want = waves == 4 ? 2 * kCus : 8 * kCus;
     uint64_t splits = 2 * base >= want ? 1 : (want + base - 1) / base;
-    const uint64_t most = other_tiles / least ? other_tiles / least : 1;
+    const uint64_t most = other_tiles / 2 ? other_tiles / 2 : 1;
     if (splits > most) splits = most;
     s.splits = (uint32_t)splits;
 }
 void plan_rows(Shape& s, int& waves) {          // forward, dq
     const int dp = padded(s.D);
     waves = s.rows <= 32 && dp <= 160 ? 1 : 4;
-    plan(s, s.rows, div_up(s.Nk, key_tile(dp, waves)), waves, 4);
+    plan(s, s.rows, div_up(s.Nk, key_tile(dp, waves)), waves);
 }
-void plan_keys(Shape& s) { plan(s, s.Nk, s.group * div_up(s.Nq, query_tile((int)s.D)), 4, 4); }
+void plan_keys(Shape& s) { plan(s, s.Nk, s.group * div_up(s.Nq, query_tile((int)s.D)), 4); }
 
 template <typename T, int DP, int NW>
 void launch_fwd(const void* q, const void* k, const void* v, void* o, void* o_lo, float* lse, float* part, float* ml, const Shape& s, hipStream_t st) {
@@ -332,12 +365,6 @@ template <typename T> void join_o(const float* part, const float* ml, const Shap
     const uint64_t n = (uint64_t)s.B * s.H * s.Nq;
     hipLaunchKernelGGL(k_join_o<T>, dim3((uint32_t)((n + rows_here - 1) / rows_here)), dim3(256), 0, st, part, ml, s, parts, static_cast<T*>(o),
                        static_cast<T*>(o_lo), lse);
-}
-template <typename T>
-void join_sum(const float* pa, const float* pb, uint32_t splits, uint32_t B, uint32_t H, uint32_t N, uint32_t D, void* oa, void* ob, hipStream_t st) {
-    const uint64_t n = (uint64_t)B * H * N * (D / 4);
-    hipLaunchKernelGGL(k_join_sum<T>, dim3((uint32_t)((n + 255) / 256), ob ? 2 : 1), dim3(256), 0, st, pa, pb, splits, B, H, N, D, static_cast<T*>(oa),
-                       static_cast<T*>(ob));
 }
 template <typename T> void prep(const void* v, const void* o, const void* o_lo, const void* dy, const float* lse, const Shape& s, float* delta, float* rows2, float* v2, hipStream_t st) {
     const uint32_t bh = s.B * s.Hk;
@@ -464,15 +491,21 @@ int sdfx_attention_train_backward(const void* q, const void* k, const void* v, c
     a.dq = dq; a.dk = dk; a.dv = dv;
     if (bf16) prep<__bf16>(v, o, o_lo, dy, lse, s, scratch, scratch + l.rows2, scratch + l.v2, st);
     else prep<_Float16>(v, o, o_lo, dy, lse, s, scratch, scratch + l.rows2, scratch + l.v2, st);
+    JoinSums js;
+    uint32_t joins = 0;
+    uint64_t most = 0;
+    auto join = [&](const float* part, void* out, uint32_t splits, uint32_t heads, uint32_t n) {
+        if (splits == 1) return;
+        js.of[joins++] = {part, out, splits, heads, n};
+        if ((uint64_t)heads * n > most) most = (uint64_t)heads * n;
+    };
     if (dk) {
         Shape t = s;
         plan_keys(t);
         a.part = scratch + l.pk; a.part2 = scratch + l.pv;
         launch_dkdv(a, t, bf16, st);
-        if (t.splits > 1) {
-            if (bf16) join_sum<__bf16>(a.part, a.part2, t.splits, B, Hk, Nk, D, dk, dv, st);
-            else join_sum<_Float16>(a.part, a.part2, t.splits, B, Hk, Nk, D, dk, dv, st);
-        }
+        join(a.part, dk, t.splits, Hk, Nk);
+        join(a.part2, dv, t.splits, Hk, Nk);
     }
     if (dq) {
         Shape t = s;
@@ -480,10 +513,12 @@ int sdfx_attention_train_backward(const void* q, const void* k, const void* v, c
         plan_rows(t, waves);
         a.part = scratch + l.pq; a.part2 = nullptr;
         launch_dq(a, t, bf16, waves, st);
-        if (t.splits > 1) {
-            if (bf16) join_sum<__bf16>(a.part, nullptr, t.splits, B, H, Nq, D, dq, nullptr, st);
-            else join_sum<_Float16>(a.part, nullptr, t.splits, B, H, Nq, D, dq, nullptr, st);
-        }
+        join(a.part, dq, t.splits, H, Nq);
+    }
+    if (joins) {
+        const dim3 grid((uint32_t)((most * B * (D / 4) + 255) / 256), joins);
+        if (bf16) hipLaunchKernelGGL(k_join_sum<__bf16>, grid, dim3(256), 0, st, js, B, D);
+        else hipLaunchKernelGGL(k_join_sum<_Float16>, grid, dim3(256), 0, st, js, B, D);
     }
     return check_launch("attention_train_backward");
 }

@@ -49,15 +49,31 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
     const uint32_t wg_key = xt * NW * 32u, w0 = wg_key + wave * 32u, key = w0 + x, kc = min(key, s.Nk - 1u);
     const bool seen = key < s.Nk && (!s.mask || s.mask[(size_t)b * s.Nk + kc] != 0);
     const bool wave_on = __ballot(seen) != 0;
-    float g = 1.f;
-    if (Half<T>::kScaled) g = grad_scale(a.rows2 + (size_t)bh * prep_blocks(s.rows), prep_blocks(s.rows), a.v2 + (size_t)bh * prep_blocks(s.Nk), prep_blocks(s.Nk), lane);
-    // weights of the parts: scores as (shift - lse) / c reaches 2^28 in fp16; |delta| <= 1 / (2 g)
-    const float ws = Half<T>::kScaled ? 4096.f : 1.f, wd = Half<T>::kScaled ? fminf(fmaxf(0.5f / g, 1.f / 8192.f), 32768.f) : 1.f;
+    // fp16: ds g (g from grad_scale, |ds g| <= 1) times 2^15 is what the second product takes. g is put into v (`gv`, so that dp comes out with it)
+    // as long as the largest |v g| stays in 2^-6 .. 2^12, well inside fp16; beyond, what is left of it goes into the shift of p (large
+    // dy) or is left out (small dy: ds is then 2^-12 of its bound and more, still normal).
+    float gv = 1.f, shift = Half<T>::kShift, md = 1.f;
+    if (Half<T>::kScaled) {
+        float vmax;
+        const float g = grad_scale(a.rows2 + (size_t)bh * prep_blocks(s.rows), prep_blocks(s.rows), a.v2 + (size_t)bh * prep_blocks(s.Nk), prep_blocks(s.Nk), lane, vmax);
+        const float v1 = __uint_as_float(__float_as_uint(fminf(fmaxf(vmax, 1e-30f), 1e30f)) & 0x7f800000u);       // a power of two, vmax in v1 .. 2 v1
+        gv = fminf(fmaxf(g, 0.015625f / v1), 4096.f / v1);
+        if (gv > g) shift = fmaxf(Half<T>::kShift - __builtin_amdgcn_logf(gv / g), 0.f);
+        md = 0.5f * gv / g;                                              // >= the largest |delta gv|
+    }
+    // weights of the parts: scores as (shift - lse) / c reaches 2^28 in fp16
+    const float ws = Half<T>::kScaled ? 4096.f : 1.f, wd = Half<T>::kScaled ? fminf(fmaxf(md, 1.f / 8192.f), 32768.f) : 1.f;
     const float inv_c = 1.f / s.c;
 
     typename Half<T>::v8 kf[KS], vf[KS];
     row_fragments<T, KS>(kf, static_cast<const T*>(a.k) + (size_t)b * s.k_sb + (size_t)kc * s.k_sn + (size_t)hk * s.k_sh, s.D, hi);
     row_fragments<T, KS>(vf, static_cast<const T*>(a.v) + (size_t)b * s.v_sb + (size_t)kc * s.v_sn + (size_t)hk * s.v_sh, s.D, hi);
+    if (Half<T>::kScaled) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) vf[ks][i] = (T)((float)vf[ks][i] * gv);
+    }
 #pragma unroll
     for (int ks = 0; ks < KS; ks++)
         if (16u * ks + 8u * hi == s.D) {
@@ -120,8 +136,8 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
         stq.put(ldsQ + buf * L::BYTES, rq, whole, live);
         sty.put(ldsY + buf * L::BYTES, ry, whole, live);
         if (lane < (uint32_t)QT) {                                       // the rows' extra channels, one tensor's by each of two waves
-            if (wave == 0) *reinterpret_cast<u4v*>(ldsQ + buf * L::BYTES + lane * L::PITCH + s.D * 2u) = split_parts<T>((Half<T>::kShift - r_lse) * inv_c, ws);
-            if (wave == 1) *reinterpret_cast<u4v*>(ldsY + buf * L::BYTES + lane * L::PITCH + s.D * 2u) = split_parts<T>(r_lse == INFINITY ? 0.f : -r_delta, wd);
+            if (wave == 0) *reinterpret_cast<u4v*>(ldsQ + buf * L::BYTES + lane * L::PITCH + s.D * 2u) = split_parts<T>((shift - r_lse) * inv_c, ws);
+            if (wave == 1) *reinterpret_cast<u4v*>(ldsY + buf * L::BYTES + lane * L::PITCH + s.D * 2u) = split_parts<T>(r_lse == INFINITY ? 0.f : -r_delta * gv, wd);
         }
     };
 
@@ -137,14 +153,14 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
             const bool diagonal = s.causal && q0 + s.off < (int)w0 + 31;
             f32x16 sc[NB], dp[NB];
 #pragma unroll
-            for (int st = 0; st < NB; st++) {
-                sc[st] = zero16();
-                dp[st] = zero16();
+            for (int st = 0; st < NB; st++) sc[st] = dp[st] = zero16();
 #pragma unroll
-                for (int ks = 0; ks < KS; ks++) sc[st] = mma(row_operand<T, L>(qt, st, ks, x, hi), kf[ks], sc[st]);
+            for (int ks = 0; ks < KS; ks++)               // (the blocks' chains in turn: a product waits for the one before it in its chain)
 #pragma unroll
-                for (int ks = 0; ks < KS; ks++) dp[st] = mma(row_operand<T, L>(yt, st, ks, x, hi), vf[ks], dp[st]);
-            }
+                for (int st = 0; st < NB; st++) {
+                    sc[st] = mma(row_operand<T, L>(qt, st, ks, x, hi), kf[ks], sc[st]);
+                    dp[st] = mma(row_operand<T, L>(yt, st, ks, x, hi), vf[ks], dp[st]);
+                }
 #pragma unroll
             for (int st = 0; st < NB; st++) {
                 // this block's transposed operands, requested ahead of its exponentials (the compiler would read each in front of its product and wait)
@@ -169,7 +185,7 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
                     sc[st][r] = __builtin_amdgcn_exp2f(sc[st][r] * s.c);
-                    dp[st][r] = sc[st][r] * (Half<T>::kScaled ? dp[st][r] * g : dp[st][r]);
+                    dp[st][r] = sc[st][r] * dp[st][r];
                 }
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
@@ -188,7 +204,7 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
         __syncthreads();
     }
     if (key >= s.Nk) return;
-    const float fv = Half<T>::kScaled ? 1.f / 32768.f : 1.f, fk = s.scale * fv / g;
+    const float fv = __builtin_amdgcn_exp2f(-shift), fk = s.scale * fv / gv;
     const size_t at = (size_t)bh * s.Nk + key, pa = ((size_t)split * s.B * s.Hk * s.Nk + at) * s.D;
     const size_t oa = (((size_t)b * s.Nk + key) * s.Hk + hk) * s.D;
 #pragma unroll

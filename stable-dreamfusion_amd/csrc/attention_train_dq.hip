@@ -28,9 +28,13 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_dq(BwdArgs a, Sha
     row_fragments<T, KS>(yf, static_cast<const T*>(a.dy) + (((size_t)b * s.Nq + row.qi) * s.H + row.head) * s.D, s.D, hi);
     const size_t at = (size_t)bh * s.rows + row.R;
     const float lse = a.lse[at];
-    float g = 1.f;
-    if (Half<T>::kScaled) g = grad_scale(a.rows2 + (size_t)bh * prep_blocks(s.rows), prep_blocks(s.rows), a.v2 + (size_t)bh * prep_blocks(s.Nk), prep_blocks(s.Nk), lane);
-    const float nlse = Half<T>::kShift - lse, ndelta = -a.delta[at] * g;
+    float g = 1.f, vmax;
+    if (Half<T>::kScaled) g = grad_scale(a.rows2 + (size_t)bh * prep_blocks(s.rows), prep_blocks(s.rows), a.v2 + (size_t)bh * prep_blocks(s.Nk), prep_blocks(s.Nk), lane, vmax);
+    // ds = p (dp - delta) g: g joins the exponent (p is used for nothing else), -delta starts dp's sum on the matrix cores
+    const float nlse = Half<T>::kShift + (Half<T>::kScaled ? __builtin_amdgcn_logf(g) : 0.f) - lse, ndelta = -a.delta[at];
+    f32x16 dp0;
+#pragma unroll
+    for (int r = 0; r < 16; r++) dp0[r] = ndelta;
 
     uint32_t kend = s.Nk;
     int wave_lo = 0x7fffffff, wave_hi = 0x7fffffff;
@@ -82,14 +86,14 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_dq(BwdArgs a, Sha
                 const bool masked = live != all_keys<KT>() || key0 + KT - 1 > wave_lo;
                 f32x16 sc[NB], dp[NB];
 #pragma unroll
-                for (int st = 0; st < NB; st++) {
-                    sc[st] = zero16();
-                    dp[st] = zero16();
+                for (int st = 0; st < NB; st++) { sc[st] = zero16(); dp[st] = dp0; }
 #pragma unroll
-                    for (int ks = 0; ks < KS; ks++) sc[st] = mma(row_operand<T, L>(kt, st, ks, x, hi), qf[ks], sc[st]);
+                for (int ks = 0; ks < KS; ks++)           // (the blocks' chains in turn: a product waits for the one before it in its chain)
 #pragma unroll
-                    for (int ks = 0; ks < KS; ks++) dp[st] = mma(row_operand<T, L>(vt, st, ks, x, hi), yf[ks], dp[st]);
-                }
+                    for (int st = 0; st < NB; st++) {
+                        sc[st] = mma(row_operand<T, L>(kt, st, ks, x, hi), qf[ks], sc[st]);
+                        dp[st] = mma(row_operand<T, L>(vt, st, ks, x, hi), yf[ks], dp[st]);
+                    }
 #pragma unroll
                 for (int st = 0; st < NB; st++) {
                     // the transposed key operands, requested ahead of the exponentials (the compiler would read each in front of its product and wait)
@@ -109,7 +113,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_dq(BwdArgs a, Sha
 #pragma unroll
                     for (int r = 0; r < 16; r++) {
                         const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[st][r], s.c, nlse));
-                        sc[st][r] = p * __builtin_fmaf(dp[st][r], g, ndelta);
+                        sc[st][r] = p * dp[st][r];
                     }
                     __builtin_amdgcn_s_setprio(0);
 #pragma unroll
