@@ -246,9 +246,14 @@ class GroupNormAct(nn.GroupNorm):
     def __init__(self, num_groups, num_channels, eps=1e-5, act=False):
         super().__init__(num_groups, num_channels, eps=eps, affine=True)
         self.act = bool(act)
+        self.checkpoint = None      # "full" / "int8": the training form (`group_norm_act`), see sd15_arch.use_training_ops
 
     def forward(self, x, pre=None):
-        """`pre` [N, C] (optional, no gradient): the norm is taken of `x + pre[:, :, None, None]`."""
+        """`pre` [N, C] (optional; no gradient unless `checkpoint` is set): the norm is taken of `x + pre[:, :, None, None]`."""
+        if self.checkpoint is not None:
+            w, b = (t if t.dtype == x.dtype else t.float() for t in (self.weight, self.bias))
+            return group_norm_act(x, self.num_groups, w, b, self.eps, self.act, pre,
+                                  self.checkpoint if x.shape[1] % 32 == 0 else "full")
         if fused_ok(x, self.weight, self.bias, self.num_groups) and (pre is None or (
                 pre.dtype == torch.float16 and pre.shape == (x.shape[0], x.shape[1]) and pre.is_contiguous() and pre.data_ptr() % 16 == 0)):
             return _GroupNormActFn.apply(x, None if pre is None else pre.detach(), self.weight, self.bias, self.num_groups, self.eps, self.act)

@@ -22,7 +22,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import guidance as G
-from .attention import attention_bnc
+from .attention import attention, attention_bnc
 from .conv import conv3x3, conv_ok, linear_auto
 from .groupnorm import GroupNormAct, add_bias_residual, fused_ok, geglu
 import _devswitch
@@ -51,6 +51,9 @@ class ResBlock(nn.Module):
                 emb_act is not None and emb_act.requires_grad):
             return self._forward_fused(x, emb_act)
         h = self.conv1(self.norm1(x))                       # norm1 / norm2 include the SiLU
+        if self.temb is not None and self.norm2.checkpoint is not None:
+            h = self.conv2(self.norm2(h, pre=self.temb(emb_act)))       # (the sum rides in the norm, its gradient comes out of it)
+            return (x if self.skip is None else self.skip(x)) + h
         if self.temb is not None:
             h = h + self.temb(emb_act)[:, :, None, None]
         h = self.conv2(self.norm2(h))
@@ -108,6 +111,7 @@ class Attention(nn.Module):
         self.k = nn.Linear(ctx_dim or dim, dim, bias=qkv_bias)
         self.v = nn.Linear(ctx_dim or dim, dim, bias=qkv_bias)
         self.o = nn.Linear(dim, dim)
+        self.train_ops = False                # use_training_ops: attention with its own gradient kernels
 
     def _fused_weight(self, names):
         """The projections' weights stacked once (frozen parameters; rebuilt when one was replaced or written to): q / k / v of a
@@ -122,14 +126,19 @@ class Attention(nn.Module):
             cache[names] = (ver, stacked)
         return cache[names][1]
 
-    def forward(self, x, ctx=None, residual=None):
-        """attention(x, ctx) [+ residual]: the sum rides in the output projection's epilogue where csrc/conv.hip runs it."""
+    def forward(self, x, ctx=None, residual=None, ctx_mask=None):
+        """attention(x, ctx) [+ residual]: the sum rides in the output projection's epilogue where csrc/conv.hip runs it. `ctx_mask` [B, n]
+        bool: which tokens of the context are seen (a padded prompt's own)."""
         self_attn = ctx is None
         ctx = x if self_attn else ctx
         B, N, C = x.shape
         d = C // self.heads
         frozen = not (self.q.weight.requires_grad or self.k.weight.requires_grad or self.v.weight.requires_grad
                       or self.o.weight.requires_grad or self.o.bias.requires_grad)
+        if (self.train_ops or ctx_mask is not None) and d <= 256:
+            split = lambda t: t.view(B, -1, self.heads, d).transpose(1, 2)
+            out = self.o(attention(split(self.q(x)), split(self.k(ctx)), split(self.v(ctx)), key_mask=ctx_mask))
+            return out if residual is None else out + residual
         if _QKV_FUSION and frozen and x.is_cuda and d <= 256 and self.q.bias is None:
             heads = lambda t, i: t[..., i * C:(i + 1) * C].unflatten(-1, (self.heads, d)).transpose(1, 2)   # [B, H, n, d] view
             if self_attn:
@@ -164,8 +173,9 @@ class TransformerBlock(nn.Module):
         self.n1, self.n2, self.n3 = nn.LayerNorm(c), nn.LayerNorm(c), nn.LayerNorm(c)
         self.attn1, self.attn2 = Attention(c, None, heads), Attention(c, ctx_dim, heads)
         self.ff_in, self.ff_out = nn.Linear(c, 8 * c), nn.Linear(4 * c, c)
+        self.checkpoint = None                # use_training_ops: GEGLU with its own gradient kernel
 
-    def forward(self, x, ctx):
+    def forward(self, x, ctx, ctx_mask=None):
         B, C, H, W = x.shape
         fused = _BLOCK_FUSION and fused_ok(x, self.norm.weight, self.norm.bias, 32) and not self.proj_out.bias.requires_grad
         if fused:
@@ -175,13 +185,31 @@ class TransformerBlock(nn.Module):
         else:
             h = self.proj_in(self.norm(x)).flatten(2).transpose(1, 2)
         h = self.attn1(self.n1(h), None, h)                    # (+ h: in the output projection)
-        h = self.attn2(self.n2(h), ctx, h)
-        h = linear_auto(geglu(self.ff_in(self.n3(h))), self.ff_out.weight, self.ff_out.bias, h)
+        h = self.attn2(self.n2(h), ctx, h, ctx_mask)
+        u = self.ff_in(self.n3(h))
+        act = geglu(u) if self.checkpoint is None else geglu(u, checkpoint=self.checkpoint if u.shape[-1] % 64 == 0 else "full")
+        h = linear_auto(act, self.ff_out.weight, self.ff_out.bias, h)
         if fused:
             xr = x.permute(0, 2, 3, 1).reshape(B, H * W, C)       # channels-last memory IS [B, HW, C]
             out = linear_auto(h, self.proj_out.weight.reshape(C, C), self.proj_out.bias, xr)   # bias and residual in the epilogue
             return out.view(B, H, W, C).permute(0, 3, 1, 2)
         return x + self.proj_out(h.transpose(1, 2).reshape(B, C, H, W))
+
+
+def use_training_ops(module, checkpoint="int8"):
+    """Switches the group norms, attentions and feed-forwards inside `module` (a UNetSD15, a VAEEncoderSD15, or one of their blocks) to the
+    forms with gradient kernels — for fine-tuning them, an adapter on them, or a gradient through them — and returns it. `checkpoint`:
+    "int8" keeps the norms' and GEGLUs' inputs for the backward in 8 bits (half the memory of half precision; channel counts that are
+    no multiple of 32 as they are), "full" as they are, None switches back. Parameters and state_dict are untouched; convolutions
+    and projections stay PyTorch's when a gradient is wanted. Heads wider than 256 (the VAE's one) keep their matrix products."""
+    if checkpoint not in (None, "full", "int8"):
+        raise ValueError(f'use_training_ops: checkpoint must be "int8", "full" or None, got {checkpoint!r}')
+    for m in module.modules():
+        if isinstance(m, (GroupNormAct, TransformerBlock)):
+            m.checkpoint = checkpoint
+        elif isinstance(m, Attention):
+            m.train_ops = checkpoint is not None
+    return module
 
 
 class UNetSD15(nn.Module):
@@ -220,7 +248,8 @@ class UNetSD15(nn.Module):
         args = t.float()[:, None] * freqs[None]
         return torch.cat([torch.cos(args), torch.sin(args)], dim=-1)
 
-    def forward(self, x, t, encoder_hidden_states):
+    def forward(self, x, t, encoder_hidden_states, context_mask=None):
+        """`context_mask` [B, tokens] bool (optional): which tokens of `encoder_hidden_states` are seen."""
         emb = F.silu(self.time(self.time_embedding(t).to(x.dtype)))   # every ResNet block takes SiLU(emb): applied once here
         ctx = encoder_hidden_states.to(x.dtype)
         h = self.conv_in(x)
@@ -229,17 +258,17 @@ class UNetSD15(nn.Module):
             if isinstance(first, ResBlock):
                 h = first(h, emb)
                 if attn is not None:
-                    h = attn(h, ctx)
+                    h = attn(h, ctx, context_mask)
             else:
                 h = conv3x3(h, first.weight, first.bias, None, 2)   # stride-2 downsample
             hs.append(h)
         h = self.mid[0](h, emb)
-        h = self.mid[1](h, ctx)
+        h = self.mid[1](h, ctx, context_mask)
         h = self.mid[2](h, emb)
         for res, attn, upconv in self.up:
             h = res(torch.cat([h, hs.pop()], dim=1), emb)
             if attn is not None:
-                h = attn(h, ctx)
+                h = attn(h, ctx, context_mask)
             if upconv is not None:                           # nearest 2 x upsample + convolution (the kernel reads through the upsample)
                 h = conv3x3(h, upconv.weight, upconv.bias, None, 1, upsample=True)
         return self.conv_out(self.norm_out(h))

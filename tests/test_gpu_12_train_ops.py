@@ -338,3 +338,36 @@ def test_captured_and_replayed(dev):
         torch.cuda.synchronize()
         for (_, _, _, out), r in zip(graphs, want):
             assert all(torch.equal(a, c) for a, c in zip(out, r))
+
+
+@pytest.mark.parametrize("dtype,checkpoint", [(F16, "full"), (F16, "int8"), (BF16, "int8")])
+def test_prior_blocks_train_on_these_operators(dev, dtype, checkpoint):
+    """A ResNet block and a transformer block of the UNet with every parameter trainable, a padded prompt: outputs and all gradients
+    against the same blocks in float64 on the CPU with the same checkpoints. 2-norms: about 40 half-precision roundings on the way, half a step
+    rms 0.3 u each (u = 2^-11 / 2^-8), adding at random: 2 u; sums of products with cancellation a few times that. 8-bit codes follow inputs
+    that differ by those roundings: a code in 50 / 6 moves by a step of 2^-7 of its block's maximum."""
+    import copy
+    from sdfx_nerf.sd15_arch import ResBlock, TransformerBlock, use_training_ops
+    torch.manual_seed(0)
+    res, tr = ResBlock(64, 160, 96), TransformerBlock(160, 48, heads=4)
+    for m in (res, tr):
+        use_training_ops(m, checkpoint)
+    near = [copy.deepcopy(m).to(dtype) for m in (res, tr)]
+    far = [copy.deepcopy(m).double() for m in near]
+    near = [m.to(dev).to(memory_format=torch.channels_last) for m in near]
+    x, emb, ctx, dy = (_rn("cpu", *s, seed=i, dtype=dtype) for i, s in enumerate(((2, 64, 12, 8), (2, 96), (2, 20, 48), (2, 160, 12, 8))))
+    mask = torch.arange(20)[None] < torch.tensor([[20], [9]])
+
+    def step(blocks, cast):
+        a = [cast(t).detach().requires_grad_(True) for t in (x, emb, ctx)]
+        y = blocks[1](blocks[0](a[0], a[1]), a[2], mask.to(a[0].device))
+        ps = [p for m in blocks for p in m.parameters()]
+        return [y.detach(), *torch.autograd.grad(y, a + ps, cast(dy))]
+    got = step(near, lambda t: t.to(dev).contiguous(memory_format=torch.channels_last) if t.dim() == 4 else t.to(dev))
+    want = step(far, lambda t: t.double())
+    u = ref.half_step(dtype)
+    tol = 12 * u + (2 * 2.0 ** -7 if checkpoint == "int8" else 0)
+    for i, (g, w) in enumerate(zip(got, want)):
+        assert g.shape == w.shape and torch.isfinite(g).all()
+        err = float((g.cpu().double() - w).norm() / w.norm().clamp(min=1e-30))
+        assert err <= tol, (i, err, tol)

@@ -172,3 +172,48 @@ def test_c_abi_refuses_before_any_launch():
     assert lib.sdfx_geglu_train_forward(P, 4, 12, 0, P, None, None) == -1 and lib.sdfx_geglu_train_forward(P, 4, 40, 0, P, P, None) == -1
     assert lib.sdfx_geglu_train_forward(None, 4, 16, 0, P, None, None) == -1 and lib.sdfx_geglu_train_backward(P, 0, P, 4, 16, 5, P, None) == -1
     assert lib.sdfx_geglu_train_forward(P, 0, 16, 0, P, None, None) == 0          # no rows: nothing to do
+
+
+# ---- the prior's blocks on these operators ------------------------------------------------------------------------------------------
+def _small_unet(dtype):
+    from sdfx_nerf.sd15_arch import UNetSD15
+    torch.manual_seed(0)
+    return UNetSD15(in_ch=4, out_ch=4, base=32, mult=(1, 2), ctx_dim=24, heads=4, res_per_level=1).to(dtype)
+
+
+def test_a_unet_on_the_training_ops_has_the_gradients_of_the_plain_one():
+    """float64, checkpoint "full": the same outputs and parameter gradients to rounding; the switch goes back; a context mask equals a
+    shorter context."""
+    from sdfx_nerf.sd15_arch import use_training_ops
+    net = _small_unet(torch.float64)
+    x, t, ctx = _rn(2, 4, 8, 8, seed=1, dtype=torch.float64), torch.tensor([3, 500]), _rn(2, 7, 24, seed=2, dtype=torch.float64)
+    dy = _rn(2, 4, 8, 8, seed=3, dtype=torch.float64)
+    ps = list(net.parameters())
+    y0 = net(x, t, ctx)
+    g0 = torch.autograd.grad(y0, ps, dy)
+    y1 = use_training_ops(net, "full")(x, t, ctx)
+    g1 = torch.autograd.grad(y1, ps, dy)
+    assert torch.allclose(y0, y1, rtol=1e-10, atol=1e-12)
+    for a, b in zip(g0, g1):
+        assert float((a - b).norm()) <= 1e-9 * float(a.norm()) + 1e-12
+    mask = torch.arange(7)[None].expand(2, 7) < 5
+    assert torch.allclose(net(x, t, ctx, context_mask=mask), net(x, t, ctx[:, :5]), rtol=1e-10, atol=1e-12)
+    assert torch.equal(use_training_ops(net, None)(x, t, ctx), y0)
+    assert torch.allclose(net(x, t, ctx, context_mask=mask), net(x, t, ctx[:, :5]), rtol=1e-10, atol=1e-12)
+    with pytest.raises(ValueError):
+        use_training_ops(net, "int4")
+
+
+def test_a_unet_with_8_bit_checkpoints_keeps_its_outputs_and_nearly_its_gradients():
+    """The forward does not see the checkpoint. A gradient through one norm is off by the 8-bit input's error (rms of a step over a normal
+    block's deviation below 1 %) times a factor of order one; the errors of the dozen norms and GEGLUs add up at random."""
+    from sdfx_nerf.sd15_arch import use_training_ops
+    net = _small_unet(torch.float32)
+    x, t, ctx, dy = _rn(2, 4, 8, 8, seed=1), torch.tensor([3, 500]), _rn(2, 7, 24, seed=2), _rn(2, 4, 8, 8, seed=3)
+    ps = list(net.parameters())
+    y0 = use_training_ops(net, "full")(x, t, ctx)
+    g0 = torch.cat([g.flatten() for g in torch.autograd.grad(y0, ps, dy)])
+    y1 = use_training_ops(net, "int8")(x, t, ctx)
+    g1 = torch.cat([g.flatten() for g in torch.autograd.grad(y1, ps, dy)])
+    assert torch.equal(y0, y1)
+    assert not torch.equal(g0, g1) and float((g0 - g1).norm()) <= 0.1 * float(g0.norm())
