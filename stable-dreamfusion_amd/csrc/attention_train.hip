@@ -121,6 +121,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_fwd(const T* __re
                         for (int r = 0; r < 16; r++) acc[dt][r] *= alpha;
                 }
                 float sum0 = 0.f, sum1 = 0.f;
+                typename Half<T>::v8 pf[2 * NB];
 #pragma unroll
                 for (int st = 0; st < NB; st++) {
 #pragma unroll
@@ -131,12 +132,26 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_fwd(const T* __re
                     }
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        const typename Half<T>::v8 pf = operand<T>(sc[st], e);          // (the probabilities' rounding: half a unit of each, as the inputs')
+                        pf[2 * st + e] = operand<T>(sc[st], e);          // (the probabilities' rounding: half a unit of each, as the inputs')
 #pragma unroll
-                        for (int dt = 0; dt < DT; dt++) acc[dt] = mma(ahead(DP) ? vo[2 * st + e][dt] : col_operand<T, L>(vt, 2 * st + e, dt, lane), pf, acc[dt]);
+                        for (int dt = 0; dt < DT; dt++) acc[dt] = mma(ahead(DP) ? vo[2 * st + e][dt] : col_operand<T, L>(vt, 2 * st + e, dt, lane), pf[2 * st + e], acc[dt]);
                     }
                 }
                 l_run += sum0 + sum1;
+                // What that rounding left, where few keys carry a row: it shows in o, and the backward's delta is taken from o: the rounding of n
+                // equal probabilities is 1 / sqrt(n) of ds's own (4 of them, 2 a lane: half of it). In a long flat row only the first tiles
+                // take this (4096 x 40: 1 us; a bound of 16 cost 10). With or without a gradient to come: the same o.
+                if (__ballot(l_run < 2.f)) {
+                    keep_branch();
+#pragma unroll
+                    for (int st = 0; st < NB; st++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const typename Half<T>::v8 lo = left_over<T>(sc[st], e, pf[2 * st + e]);
+#pragma unroll
+                            for (int dt = 0; dt < DT; dt++) acc[dt] = mma(ahead(DP) ? vo[2 * st + e][dt] : col_operand<T, L>(vt, 2 * st + e, dt, lane), lo, acc[dt]);
+                        }
+                }
                 __builtin_amdgcn_s_setprio(0);
             }
             if (NBUF == 1) __syncthreads();
@@ -166,7 +181,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_fwd(const T* __re
     }
     // a row that sees nothing: zero, and a log-sum-exp of +inf, at which the backward's exp2(s - lse) is 0
     const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
-    if (lse && hi == 0) lse[at] = l > 0.f ? m_run + __builtin_amdgcn_logf(l) : (l == l ? INFINITY : l);
+    if (lse && hi == 0) lse[at] = l > 0.f ? mark_row(m_run + __builtin_amdgcn_logf(l), l) : (l == l ? INFINITY : l);
     T* op = o + (((size_t)b * s.Nq + row.qi) * s.H + row.head) * s.D;
     T* lp = o_lo ? o_lo + (((size_t)b * s.Nq + row.qi) * s.H + row.head) * s.D : nullptr;
 #pragma unroll
@@ -238,7 +253,7 @@ __global__ __launch_bounds__(256) void k_join_o(const float* __restrict__ part, 
     const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
     const uint32_t bh = (uint32_t)(r / s.Nq), qi = (uint32_t)(r - (uint64_t)bh * s.Nq), b = bh / s.H, h = bh - b * s.H;
     const size_t at = (((size_t)b * s.Nq + qi) * s.H + h) * s.D + c0;
-    if (lse && c0 == 0) lse[r] = l > 0.f ? m + __builtin_amdgcn_logf(l) : (l == l ? INFINITY : l);
+    if (lse && c0 == 0) lse[r] = l > 0.f ? mark_row(m + __builtin_amdgcn_logf(l), l) : (l == l ? INFINITY : l);
     a = a * inv;
     store4(o + at, a[0], a[1], a[2], a[3]);
     if (o_lo) store4(o_lo + at, a[0] - (float)(T)a[0], a[1] - (float)(T)a[1], a[2] - (float)(T)a[2], a[3] - (float)(T)a[3]);

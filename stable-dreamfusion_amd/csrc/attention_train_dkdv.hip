@@ -128,11 +128,13 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
             qp += (uint64_t)QT * s.q_sn; yp += (uint64_t)QT * y_sn; stat_at += QT;
         }
     };
+    bool few = false;                                                    // (some row of the tile)
     auto put = [&](uint32_t buf) {
         const uint32_t left = s.Nq - nq0;
         uint64_t live = left >= 64u ? ~0ull : (1ull << left) - 1ull;
         if (empties) live &= __ballot(r_lse != INFINITY);
         const bool whole = left >= (uint32_t)QT && !empties;
+        few = __ballot(marked(r_lse)) != 0;
         stq.put(ldsQ + buf * L::BYTES, rq, whole, live);
         sty.put(ldsY + buf * L::BYTES, ry, whole, live);
         if (lane < (uint32_t)QT) {                                       // the rows' extra channels, one tensor's by each of two waves
@@ -194,6 +196,12 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
                     for (int dt = 0; dt < DT; dt++) dv[dt] = mma(ahead(DM) ? yo[e][dt] : col_operand<T, L>(yt, 2 * st + e, dt0 + dt, lane), pf, dv[dt]);
 #pragma unroll
                     for (int dt = 0; dt < DT; dt++) dk[dt] = mma(ahead(DM) ? qo[e][dt] : col_operand<T, L>(qt, 2 * st + e, dt0 + dt, lane), df, dk[dt]);
+                    if (few) {
+                        keep_branch();
+                        const typename Half<T>::v8 lo = left_over<T>(dp[st], e, df);
+#pragma unroll
+                        for (int dt = 0; dt < DT; dt++) dk[dt] = mma(ahead(DM) ? qo[e][dt] : col_operand<T, L>(qt, 2 * st + e, dt0 + dt, lane), lo, dk[dt]);
+                    }
                 }
             }
         }

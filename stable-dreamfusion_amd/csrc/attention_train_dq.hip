@@ -28,6 +28,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_dq(BwdArgs a, Sha
     row_fragments<T, KS>(yf, static_cast<const T*>(a.dy) + (((size_t)b * s.Nq + row.qi) * s.H + row.head) * s.D, s.D, hi);
     const size_t at = (size_t)bh * s.rows + row.R;
     const float lse = a.lse[at];
+    const bool few = __ballot(row.on && marked(lse)) != 0;             // (some row of the wave)
     float g = 1.f, vmax;
     if (Half<T>::kScaled) g = grad_scale(a.rows2 + (size_t)bh * prep_blocks(s.rows), prep_blocks(s.rows), a.v2 + (size_t)bh * prep_blocks(s.Nk), prep_blocks(s.Nk), lane, vmax);
     // ds = p (dp - delta) g: g joins the exponent (p is used for nothing else), -delta starts dp's sum on the matrix cores
@@ -121,6 +122,12 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_dq(BwdArgs a, Sha
                         const typename Half<T>::v8 f = operand<T>(sc[st], e);            // (ds rounded to the inputs' type)
 #pragma unroll
                         for (int dt = 0; dt < DT; dt++) acc[dt] = mma(ahead(DP) ? ko[e][dt] : col_operand<T, L>(kt, 2 * st + e, dt, lane), f, acc[dt]);
+                        if (few) {
+                            keep_branch();
+                            const typename Half<T>::v8 lo = left_over<T>(sc[st], e, f);
+#pragma unroll
+                            for (int dt = 0; dt < DT; dt++) acc[dt] = mma(ahead(DP) ? ko[e][dt] : col_operand<T, L>(kt, 2 * st + e, dt, lane), lo, acc[dt]);
+                        }
                     }
                 }
             }
