@@ -38,6 +38,8 @@ struct Shape {
     float scale, c;                       // softmax scale; times log2(e)
     uint32_t tiles_x;                     // workgroups along rows (forward, dq) or keys (dk / dv)
     uint32_t splits;                      // workgroups along the other axis
+    float few;                            // a row whose probabilities sum to less than this, of the largest, is one that few keys carry
+    int exact;                            // few sums: every rounding of p and ds is made good (below, at mark_row)
 };
 
 template <typename T> struct Half;
@@ -231,22 +233,30 @@ inline int padded(uint32_t D) {
         }                                                                 \
     } while (0)
 
-template <bool B> struct Flag { static constexpr bool value = B; };
 // operands of the second products requested ahead of the exponentials: where a lane's registers hold them
 constexpr bool ahead(int dp) { return dp <= 64; }
 
 // the tiles of `n` that split `i` of `splits` takes
 __device__ __forceinline__ uint32_t split_at(uint32_t n, uint32_t i, uint32_t splits) { return splits == 1 ? (i ? n : 0u) : (uint32_t)((uint64_t)n * i / splits); }
 
-// A row that few keys carry: its probabilities sum to less than 4 of the largest. The rounding of its ds shows in dq and dk (their terms cancel
-// against each other: bf16, causal 1010 x 24, scores with a deviation of 4, dq 2.6e-3 off where its own rounding is 1.7e-3), so the backward
-// adds the part of ds that rounding left (1.7e-3; marking rows below 16 gains nothing that shows and costs dq 14 us at 4096 x 40, this 4). The mark is the log-sum-exp's lowest bit (one unit in its
-// last place, 2^-24 of it): the forward knows the sum, the backward only its logarithm.
-__device__ __forceinline__ float mark_row(float lse, float l) {
-    const uint32_t u = __float_as_uint(lse);
-    return lse < INFINITY ? __uint_as_float(l < 4.f ? u | 1u : u & ~1u) : lse;
+// p and ds are rounded to the inputs' type for the second products. In sums over many rows and keys these roundings average out against that of the
+// result: 1.41 times its own error alone. Two kinds of sums have little to average, and add a product with what the rounding left:
+//  - a row that few keys carry: its probabilities sum to less than `few` = 4 of the largest. The terms of its dq cancel against each other
+//    (bf16, causal 1010 x 24, scores with a deviation of 4: dq 2.6e-3 off where its own rounding is 1.7e-3; with the product 1.7e-3).
+//    Marking rows below 16 gains nothing that shows and costs dq 14 us at 4096 x 40, this 4.
+//  - at most 512 rows to a key head or at most 128 keys (`exact`: every row is marked, and dv takes the product too): sums of a
+//    few, or of probabilities that all lie at one place between two powers of two, are up to 2.5 times as far off.
+// A row that one key carries alone has no ds: dp and delta are the same number, and the few bits that differ would be all of the gradient
+// where no row has another. Its sum is 1 but for the exponent's rounding, half a unit of the maximum m's last place; other keys with as little
+// are taken for none (at m = 20 1.3e-6, about where dp - delta ends; beyond 64 the allowance grows no more).
+// The marks are the log-sum-exp's two lowest bits (2^-22 of it): the forward knows the sum, the backward only its logarithm.
+__device__ __forceinline__ float mark_row(float m, float l, float few) {
+    const float lse = m + __builtin_amdgcn_logf(l);
+    const uint32_t u = __float_as_uint(lse) & ~3u;
+    return lse < INFINITY ? __uint_as_float(__builtin_fabsf(l - 1.f) <= fminf(__builtin_fabsf(m), 64.f) * 0x1p-24f + 0x1p-23f ? u | 3u : l < few ? u | 1u : u) : lse;
 }
 __device__ __forceinline__ bool marked(float lse) { return lse < INFINITY && (__float_as_uint(lse) & 1u); }
+__device__ __forceinline__ bool alone(float lse) { return lse < INFINITY && (__float_as_uint(lse) & 3u) == 3u; }
 // what rounding elements 8 e .. 8 e + 7 of a D fragment to `hi` left, as an operand
 template <typename T> __device__ __forceinline__ typename Half<T>::v8 left_over(const f32x16& p, int e, const typename Half<T>::v8& hi) {
     typename Half<T>::v8 v;

@@ -141,7 +141,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_fwd(const T* __re
                 // What that rounding left, where few keys carry a row: it shows in o, and the backward's delta is taken from o: the rounding of n
                 // equal probabilities is 1 / sqrt(n) of ds's own (4 of them, 2 a lane: half of it). In a long flat row only the first tiles
                 // take this (4096 x 40: 1 us; a bound of 16 cost 10). With or without a gradient to come: the same o.
-                if (__ballot(l_run < 2.f)) {
+                if (__ballot(l_run < 0.5f * s.few)) {
                     keep_branch();
 #pragma unroll
                     for (int st = 0; st < NB; st++)
@@ -181,7 +181,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_fwd(const T* __re
     }
     // a row that sees nothing: zero, and a log-sum-exp of +inf, at which the backward's exp2(s - lse) is 0
     const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
-    if (lse && hi == 0) lse[at] = l > 0.f ? mark_row(m_run + __builtin_amdgcn_logf(l), l) : (l == l ? INFINITY : l);
+    if (lse && hi == 0) lse[at] = l > 0.f ? mark_row(m_run, l, s.few) : (l == l ? INFINITY : l);
     T* op = o + (((size_t)b * s.Nq + row.qi) * s.H + row.head) * s.D;
     T* lp = o_lo ? o_lo + (((size_t)b * s.Nq + row.qi) * s.H + row.head) * s.D : nullptr;
 #pragma unroll
@@ -253,7 +253,7 @@ __global__ __launch_bounds__(256) void k_join_o(const float* __restrict__ part, 
     const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
     const uint32_t bh = (uint32_t)(r / s.Nq), qi = (uint32_t)(r - (uint64_t)bh * s.Nq), b = bh / s.H, h = bh - b * s.H;
     const size_t at = (((size_t)b * s.Nq + qi) * s.H + h) * s.D + c0;
-    if (lse && c0 == 0) lse[r] = l > 0.f ? mark_row(m + __builtin_amdgcn_logf(l), l) : (l == l ? INFINITY : l);
+    if (lse && c0 == 0) lse[r] = l > 0.f ? mark_row(m, l, s.few) : (l == l ? INFINITY : l);
     a = a * inv;
     store4(o + at, a[0], a[1], a[2], a[3]);
     if (o_lo) store4(o_lo + at, a[0] - (float)(T)a[0], a[1] - (float)(T)a[1], a[2] - (float)(T)a[2], a[3] - (float)(T)a[3]);
@@ -403,6 +403,8 @@ void fill(Shape& s, uint32_t B, uint32_t H, uint32_t Hk, uint32_t Nq, uint32_t N
     memset(&s, 0, sizeof s);
     s.B = B; s.H = H; s.Hk = Hk; s.Nq = Nq; s.Nk = Nk; s.D = D;
     s.group = H / Hk; s.rows = s.group * Nq;
+    s.exact = s.rows <= 512 || Nk <= 128;
+    s.few = s.exact ? INFINITY : 4.f;
 }
 void fill_call(Shape& s, const uint64_t* qs, const uint64_t* ks, const uint64_t* vs, const void* mask, float scale, int causal) {
     s.q_sb = qs[0]; s.q_sn = qs[1]; s.q_sh = qs[2];

@@ -5,7 +5,8 @@
 // A lane's 16 scores belong to 16 queries, so their log-sum-exps and deltas cannot be lane scalars as in dq. Read from LDS they would take
 // as many cycles there as the operands (8 of 30 reads a block); instead they ride in the products: a row carries 8 extra channels, q's
 // with (shift - lse) / c and dy's with -delta as sums of 16-bit parts, k's and v's with the parts' weights, powers of two. s and dp come out
-// of the matrix cores complete. Parts: two of fp16 or three of bf16, 22 to 24 bits.
+// of the matrix cores complete. Three parts: 24 bits in bf16, in fp16 as many as the
+// weights' range allows, at least 22 (with two, ds of a row of 2 keys that one carries by 1e4 to 1 was 8e-4 off).
 #include "attention_train.h"
 
 namespace sdfx_attn {
@@ -13,7 +14,7 @@ namespace {
 
 // The extra channels: part i of a value is rounded at weight w 2^(-step i), the rest goes to part i + 1.
 template <typename T> struct Parts;
-template <> struct Parts<_Float16> { static constexpr int N = 2, STEP = 11; };
+template <> struct Parts<_Float16> { static constexpr int N = 3, STEP = 11; };
 template <> struct Parts<__bf16> { static constexpr int N = 3, STEP = 8; };
 template <typename T> __device__ __forceinline__ u4v split_parts(float v, float w) {       // v = sum of parts * (w 2^(-STEP i)), w a power of two
     typename Half<T>::v8 o = {};
@@ -33,7 +34,8 @@ template <typename T> __device__ __forceinline__ u4v part_weights(float w) {
 }
 
 // CS: workgroups that share a key tile's output channels (2 at 256 channels, where dk and dv of 32 keys and the operands would fill the register file)
-template <typename T, int DM, int CS>
+// EX: dv too takes the product with what the rounding of p left (mark_row, attention_train.h)
+template <typename T, int DM, int CS, bool EX>
 __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape s) {
     constexpr int NW = 4, DP = (DM + 8 + 15) / 16 * 16;                  // channels with the extra ones, in whole K steps
     constexpr int QT = query_tile(DM), KS = DP / 16, DT = (DM + 31) / 32 / CS, NB = QT / 32;
@@ -129,12 +131,14 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
         }
     };
     bool few = false;                                                    // (some row of the tile)
+    uint64_t lone = 0;                                                   // the tile's rows that one key carries alone
     auto put = [&](uint32_t buf) {
         const uint32_t left = s.Nq - nq0;
         uint64_t live = left >= 64u ? ~0ull : (1ull << left) - 1ull;
         if (empties) live &= __ballot(r_lse != INFINITY);
         const bool whole = left >= (uint32_t)QT && !empties;
-        few = __ballot(marked(r_lse)) != 0;
+        if (EX) lone = __ballot(alone(r_lse));
+        else few = __ballot(marked(r_lse)) != 0;
         stq.put(ldsQ + buf * L::BYTES, rq, whole, live);
         sty.put(ldsY + buf * L::BYTES, ry, whole, live);
         if (lane < (uint32_t)QT) {                                       // the rows' extra channels, one tensor's by each of two waves
@@ -189,6 +193,13 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
                     sc[st][r] = __builtin_amdgcn_exp2f(sc[st][r] * s.c);
                     dp[st][r] = sc[st][r] * dp[st][r];
                 }
+                if (EX && lone) {
+                    keep_branch();
+                    const uint32_t bits = (uint32_t)(lone >> (32 * st)) >> (4u * hi);
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+                        if (bits & (1u << ((r & 3) + 8 * (r >> 2)))) dp[st][r] = 0.f;
+                }
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     const typename Half<T>::v8 pf = operand<T>(sc[st], e), df = operand<T>(dp[st], e);      // (p and ds rounded to the inputs' type)
@@ -196,8 +207,13 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
                     for (int dt = 0; dt < DT; dt++) dv[dt] = mma(ahead(DM) ? yo[e][dt] : col_operand<T, L>(yt, 2 * st + e, dt0 + dt, lane), pf, dv[dt]);
 #pragma unroll
                     for (int dt = 0; dt < DT; dt++) dk[dt] = mma(ahead(DM) ? qo[e][dt] : col_operand<T, L>(qt, 2 * st + e, dt0 + dt, lane), df, dk[dt]);
-                    if (few) {
-                        keep_branch();
+                    if (EX) {
+                        const typename Half<T>::v8 lo = left_over<T>(sc[st], e, pf);
+#pragma unroll
+                        for (int dt = 0; dt < DT; dt++) dv[dt] = mma(ahead(DM) ? yo[e][dt] : col_operand<T, L>(yt, 2 * st + e, dt0 + dt, lane), lo, dv[dt]);
+                    }
+                    if (EX || few) {
+                        if (!EX) keep_branch();
                         const typename Half<T>::v8 lo = left_over<T>(dp[st], e, df);
 #pragma unroll
                         for (int dt = 0; dt < DT; dt++) dk[dt] = mma(ahead(DM) ? qo[e][dt] : col_operand<T, L>(qt, 2 * st + e, dt0 + dt, lane), lo, dk[dt]);
@@ -240,7 +256,9 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
 
 template <typename T, int DM> void go(const BwdArgs& a, const Shape& s, hipStream_t st) {
     constexpr int CS = DM == 256 ? 2 : 1;
-    hipLaunchKernelGGL((k_dkdv<T, DM, CS>), dim3(s.tiles_x * s.splits * s.B * s.Hk * CS), dim3(256), 0, st, a, s);
+    const dim3 grid(s.tiles_x * s.splits * s.B * s.Hk * CS);
+    if (s.exact) hipLaunchKernelGGL((k_dkdv<T, DM, CS, true>), grid, dim3(256), 0, st, a, s);
+    else hipLaunchKernelGGL((k_dkdv<T, DM, CS, false>), grid, dim3(256), 0, st, a, s);
 }
 template <typename T> void by_width(const BwdArgs& a, const Shape& s, hipStream_t st) {
     if (s.D <= 40) go<T, 40>(a, s, st);                // (40 and the 8 extra channels are three K steps)
