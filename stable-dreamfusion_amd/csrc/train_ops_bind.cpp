@@ -1,7 +1,7 @@
 // train_ops_bind.cpp — the training operators as C++ autograd functions, bound to Python. The kernels stay behind the C ABI of
 // libsdfx_hip.so (include/sdfx.h); this file allocates, keeps what a backward pass needs and calls it on the current stream. It exists for
-// latency: a backward pass that runs Python code on autograd's thread costs 70 us more than its kernels (measured on GEGLU of
-// 128 x 10240: 116 us forward + backward from Python, see the figures in sdfx_nerf/groupnorm.py's users), which is most of a small call.
+// latency: a backward pass that runs Python code on autograd's thread costs 70 us more than its kernels, which is most of a small call (GEGLU
+// of 128 x 10240, forward and backward: 120 us from Python, 45 us from here).
 // The library's entry points arrive as addresses (bind()), so that the library that _sdfx.py opened is the one that runs.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
@@ -84,7 +84,7 @@ Strides strides(const Tensor& t) { return {{(uint64_t)t.stride(0), (uint64_t)t.s
 Tensor rows16(const Tensor& t) {          // as the kernels read it, or a copy
     const bool ok = t.stride(3) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && t.stride(2) % 8 == 0 && t.stride(2) < (1 << 24) &&
                     reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
-    return ok ? t : t.contiguous();
+    return ok ? t : at::empty(t.sizes(), t.options()).copy_(t);          // (contiguous() returns a dense tensor as it is, misaligned or with odd strides of its axes of one)
 }
 struct Attention : torch::autograd::Function<Attention> {
     static Tensor forward(AutogradContext* ctx, const Tensor& q0, const Tensor& k0, const Tensor& v0, const std::optional<Tensor>& mask0, bool causal,
@@ -168,14 +168,15 @@ struct Norm : torch::autograd::Function<Norm> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list g) {
         const variable_list s = ctx->get_saved_variables();
-        const Tensor &x = s[0], &pre = s[1], &w = s[2], &b = s[3], &stats = s[4];
-        const c10::DeviceGuard guard(x.device());
+        const Tensor &pre = s[1], &w = s[2], &b = s[3], &stats = s[4];
+        const c10::DeviceGuard guard(s[0].device());
         const auto shape = ctx->saved_data["shape"].toIntVector();
         const int64_t N = shape[0], C = shape[1], HW = shape[2] * shape[3], G = ctx->saved_data["G"].toInt(), flags = ctx->saved_data["flags"].toInt();
         Tensor dx, dpre, dw, db, scratch;
         {
             const at::AutoDispatchBelowADInplaceOrView below;
             const Tensor dy = dense16(g[0], at::MemoryFormat::ChannelsLast);
+            const Tensor x = (flags & 2) ? s[0] : dense16(s[0], at::MemoryFormat::ChannelsLast);      // (hooks on saved tensors may return another layout)
             const size_t e = pre.defined() ? 1 : 0;                 // (an absent `pre` has no edge)
             if (ctx->needs_input_grad(0)) dx = at::empty_like(dy);
             if (e && ctx->needs_input_grad(1)) dpre = at::empty_like(pre);
