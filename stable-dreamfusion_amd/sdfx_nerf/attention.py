@@ -98,7 +98,7 @@ def attention(q, k, v, key_mask=None, causal=False, scale=None):
     if not 0.0 < scale < 3e38:
         raise ValueError(f"attention: the scale must be positive and finite, got {scale}")
     if 0 in (B, H, Nq, d) or Nk == 0:
-        return (q.sum() + k.sum() + v.sum()) * 0 + torch.zeros(B, Nq, H * d, dtype=q.dtype, device=q.device)
+        return torch.zeros(B, Nq, H * d, dtype=q.dtype, device=q.device) + sum(t[:0].sum() for t in (q, k, v))    # (in the graph; no value is read)
     if not (q.is_cuda and q.dtype in (torch.float16, torch.bfloat16) and d % 8 == 0 and d <= 256):
         return _attention_plain(q, k, v, key_mask, causal, scale)
     return _sdfx.native().attention(q, k, v, key_mask, causal, scale)
