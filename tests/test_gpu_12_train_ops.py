@@ -166,6 +166,91 @@ def test_attention_on_another_stream_and_two_at_once(dev):
             assert all(torch.equal(a, b) for a, b in zip(r, want))
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("how", ["one_key", "mask", "first_row"])
+def test_attention_a_row_of_one_visible_key_has_no_gradient(dev, dtype, how):
+    """p = 1 whatever the score: dq and dk are zeros, not what dp - delta leaves, and dv is dy's sum over the rows."""
+    B, H, N, d = 2, 3, 70, 72
+    Nk = 1 if how == "one_key" else 90 if how == "mask" else N
+    q, dy = (_heads(dev, B, H, N, d, i, dtype, 3.0) for i in (1, 4))
+    k, v = (_heads(dev, B, H, Nk, d, i, dtype, 3.0) for i in (2, 3))
+    dy = dy.transpose(1, 2).reshape(B, N, H * d).contiguous()
+    m = None
+    if how == "mask":
+        m = torch.zeros(B, Nk, dtype=torch.bool, device=dev)
+        m[0, 41] = m[1, 89] = True
+    o, dq, dk, dv = got = _attend(q, k, v, dy, m, how == "first_row")
+    _compare(got, *ref.attention(q, k, v, dy, m, how == "first_row"))
+    if how == "first_row":
+        assert not dq[:, :, 0].any() and dq[:, :, 1:].any()
+        return
+    j = [0, 0] if how == "one_key" else [41, 89]
+    assert not dq.any() and not dk.any()
+    for b in range(B):
+        assert torch.equal(o[b], v[b, :, j[b]].reshape(1, -1).expand(N, -1))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("H,Hk,Nq,Nk,causal,spread", [(1, 1, 4, 100, False, 2.0), (2, 1, 40, 333, False, 1.0), (3, 3, 60, 60, True, 1.0),
+                                                      (2, 2, 700, 12, False, 0.5), (4, 4, 1010, 1010, True, 2.0)])
+def test_attention_short_sums_are_as_exact_as_their_type(dev, dtype, H, Hk, Nq, Nk, causal, spread):
+    """Few rows, few keys or rows that few keys carry: the error (2-norm) of each result stays within 1.25 times that of rounding the float64
+    result once (dv of many rows: 1.5). Left from p and ds are their second roundings, half steps of half steps: 2^-8 of a term, against
+    a cancellation of their terms of up to 2^5 at these scores, in quadrature under 1 %; the remainder of 1.25 is for o + o_lo's last bits in delta."""
+    d = 64
+    q, k, v, dy = (_heads(dev, 1, h, n, d, i, dtype, s) for i, (h, n, s) in enumerate([(H, Nq, spread), (Hk, Nk, spread), (Hk, Nk, 1.0), (H, Nq, 1.0)], 1))
+    dy = dy.transpose(1, 2).reshape(1, Nq, H * d).contiguous()
+    got, (want, _) = _attend(q, k, v, dy, None, causal), ref.attention(q, k, v, dy, None, causal)
+    short = Nq * (H // Hk) <= 512 or Nk <= 128
+    for n, g, w in zip(("o", "dq", "dk", "dv"), got, want):
+        own = float((w.to(dtype).double() - w).norm())
+        assert float((g.cpu().double() - w).norm()) <= (1.25 if short or n in ("dq", "dk") else 1.5) * own, n
+
+
+def test_attention_misaligned_and_odd_axes_of_one(dev):
+    """Dense tensors that start between two 16-byte addresses, an axis of one with an odd stride, a dy of stride 0, a mask that is a view."""
+    B, H, N, d = 1, 1, 37, 24
+    flat = _rn(dev, 3 * N * d + 3, seed=1)
+    q, k, v = (flat[i + 1 + i * N * d:][:N * d].view(B, H, N, d) for i in range(3))
+    odd = torch.as_strided(flat, (B, H, N, d), (7, 5, d, 1), 1)
+    m = _mask(dev, "holes", N, 2 * B).t()[:B]
+    for a in (q, odd):
+        leaf = [t.detach().requires_grad_(True) for t in (a, k, v)]
+        o = attention(*leaf, m)
+        got = [o.detach(), *torch.autograd.grad(o.sum(), leaf)]
+        _compare(got, *ref.attention(a, k, v, torch.ones(B, N, d, dtype=F16), m))
+
+
+def test_differentiated_twice_is_refused_and_saved_tensors_may_move(dev):
+    """create_graph gives first gradients whose own backward raises; a graph kept gives the same gradients again; tensors that hooks took to the
+    host and back (in another layout) give the same gradients; an input changed in place behind the forward is noticed."""
+    C = 64
+    x4 = _rn(dev, 2, C, 6, 7, seed=1).contiguous(memory_format=torch.channels_last)
+    w, b, pre = (_rn(dev, *s, seed=i, dtype=t) for i, (s, t) in enumerate([((C,), F32), ((C,), F32), ((2, C), F16)], 2))
+    q = _heads(dev, 2, 4, 33, 40, 5, F16)
+    cases = [((x4, w, b, pre), lambda x, w, b, p: group_norm_act(x, 8, w, b, pre=p)),
+             ((x4, w, b), lambda x, w, b: group_norm_act(x, 8, w, b, checkpoint="int8")),
+             ((q, q * 0.5, q + 1), lambda q, k, v: attention(q, k, v)),
+             ((x4.permute(0, 2, 3, 1).reshape(-1, C),), lambda x: geglu(x, "int8")), ((x4.permute(0, 2, 3, 1).reshape(-1, C),), lambda x: geglu(x, "full"))]
+    for args, f in cases:
+        leaves = [t.detach().requires_grad_(True) for t in args]
+        y = f(*leaves)
+        want = torch.autograd.grad(y, leaves, torch.ones_like(y), retain_graph=True)
+        again = torch.autograd.grad(y, leaves, torch.ones_like(y), create_graph=True)
+        assert all(torch.equal(a, c) for a, c in zip(want, again))
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            sum(t.float().sum() for t in again).backward()
+        with torch.autograd.graph.save_on_cpu():
+            y = f(*leaves)
+        assert all(torch.equal(a, c) for a, c in zip(want, torch.autograd.grad(y, leaves, torch.ones_like(y))))
+    x = x4.detach().clone(memory_format=torch.channels_last)
+    w.requires_grad_(True)
+    y = group_norm_act(x, 8, w, b)
+    x.add_(1)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.sum().backward()
+
+
 # ---- group norm -----------------------------------------------------------------------------------------------------------------
 def _norm(x, G, w, b, dy, **kw):
     leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]

@@ -47,6 +47,10 @@ def test_attention_lengths_of_zero(shapes):
     assert o.shape == (shapes[0][0], shapes[0][2], 32) and not o.any()
     o.sum().backward()
     assert q.grad.shape == q.shape and not q.grad.any() and not k.grad.any()
+    with torch.no_grad():                         # nor does any value reach the zeros
+        q.fill_(float("inf"))
+        k.fill_(float("nan"))
+        assert not attention(q, k, k).any()
 
 
 def test_attention_refuses():
