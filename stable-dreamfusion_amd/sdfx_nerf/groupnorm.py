@@ -173,7 +173,7 @@ def group_norm_act(x, groups, weight, bias, eps=1e-5, act=True, pre=None, checkp
     _check_checkpoint(checkpoint, C, "group_norm_act")
     if x.numel() == 0:
         return x + (weight.sum() + bias.sum()).to(x.dtype) * 0 + (0 if pre is None else pre[:, :, None, None] * 0)
-    if x.is_cuda and x.dtype in _KERNEL_TYPES and C % 8 == 0 and C <= 2560 and groups <= 64 and H * W < 2 ** 31:
+    if x.is_cuda and x.dtype in _KERNEL_TYPES and C % 8 == 0 and C <= 2560 and groups <= 64 and H * W < 2 ** 31 and N < 2 ** 23:
         return _S.native().group_norm(x, pre, weight, bias, groups, eps, act, checkpoint == "int8")
     keep = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or bias.requires_grad or (pre is not None and pre.requires_grad))
     return _GroupNormPlainFn.apply(x, pre, weight, bias, groups, eps, act, checkpoint == "int8", keep)

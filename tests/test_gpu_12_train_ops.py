@@ -341,6 +341,18 @@ def test_geglu_and_its_gradient(dev, dtype, lead, n, checkpoint):
         assert torch.equal(geglu(x, checkpoint), y)
 
 
+@pytest.mark.parametrize("checkpoint", ["full", "int8"])
+def test_no_rows_and_no_pixels(dev, checkpoint):
+    x = torch.zeros(3, 0, 128, dtype=F16, device=dev, requires_grad=True)
+    y = geglu(x, checkpoint)
+    y.sum().backward()
+    assert y.shape == (3, 0, 64) and x.grad.shape == x.shape
+    w = torch.ones(64, device=dev, requires_grad=True)
+    m = torch.zeros(2, 64, 0, 5, dtype=F16, device=dev, requires_grad=True)
+    group_norm_act(m, 8, w, w, checkpoint=checkpoint).sum().backward()
+    assert m.grad.shape == m.shape and not w.grad.any()
+
+
 def test_geglu_far_arguments_views_and_other_widths(dev):
     x = torch.tensor([[1.0, -1.0] * 8 + [0.0, -0.0, 40.0, -40.0, 6.0, -6.0, 300.0, -300.0] * 2], device=dev, dtype=F32)
     dy = torch.ones(1, 16, device=dev)
