@@ -207,6 +207,22 @@ def test_attention_short_sums_are_as_exact_as_their_type(dev, dtype, H, Hk, Nq, 
         assert float((g.cpu().double() - w).norm()) <= (1.25 if short or n in ("dq", "dk") else 1.5) * own, n
 
 
+def test_attention_a_cache_that_spans_more_than_32_bits(dev):
+    """Tokens 2^17 elements apart (one layer of a cache that holds many): 20 000 of them span 5.2 GB. The result of the dense copy, bit for bit."""
+    H, Nk, d, step = 2, 20000, 64, 2 ** 17
+    q, dy = _rn(dev, 1, 2 * H, 3, d, seed=1), _rn(dev, 1, 3, 2 * H * d, seed=2)
+    k, v = _heads(dev, 1, H, Nk, d, 3, F16), _heads(dev, 1, H, Nk, d, 4, F16)
+    cache = torch.empty(Nk * step, dtype=F16, device=dev)
+    far = [torch.as_strided(cache, (1, H, Nk, d), (Nk * step, d, step, 1), 2 * H * d * i) for i in range(2)]
+    for f, t in zip(far, (k, v)):
+        f.copy_(t)
+    m = torch.ones(1, Nk, dtype=torch.bool, device=dev)
+    m[:, 100:300] = False
+    want = _attend(q, k, v, dy, m, True)
+    assert all(torch.equal(a, c) for a, c in zip(_attend(q, *far, dy, m, True), want))
+    _compare(want, *ref.attention(q, k, v, dy, m, True))
+
+
 def test_attention_misaligned_and_odd_axes_of_one(dev):
     """Dense tensors that start between two 16-byte addresses, an axis of one with an odd stride, a dy of stride 0, a mask that is a view."""
     B, H, N, d = 1, 1, 37, 24
