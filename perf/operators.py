@@ -201,10 +201,10 @@ def _plain_attention(st):
 
 def _eight_bits(x):
     """What the 8-bit form of x [..., C] stands for: blocks of 32 channels share a step 2^(floor(log2 max|x|) - 6)."""
-    b = x.double().unflatten(-1, (-1, 32))
-    _, e = torch.frexp(b.abs().amax(-1, keepdim=True))                # the mantissa lies in [1/2, 1): floor(log2) = e - 1
-    step = ((e.to(torch.int64) - 7).clamp(min=-126) + 1023 << 52).view(torch.float64)       # a power of two from its bits: exact
-    return (torch.round(b / step).clamp(-127, 127) * step).flatten(-2).to(x.dtype)
+    b = x.unflatten(-1, (-1, 32))
+    _, e = torch.frexp(b.abs().amax(-1, keepdim=True))
+    e = (e - 7).clamp(min=-126)                                       # frexp's mantissa lies in [1/2, 1): floor(log2) = e - 1
+    return torch.ldexp(torch.round(torch.ldexp(b, -e)).clamp(-127, 127), e).flatten(-2)
 
 
 def _plain_group_norm(st):
