@@ -135,7 +135,7 @@ class Attention(nn.Module):
         d = C // self.heads
         frozen = not (self.q.weight.requires_grad or self.k.weight.requires_grad or self.v.weight.requires_grad
                       or self.o.weight.requires_grad or self.o.bias.requires_grad)
-        if (self.train_ops or ctx_mask is not None) and d <= 256:
+        if ctx_mask is not None or (self.train_ops and d <= 256):      # (only `attention` takes a mask; it takes heads of any width)
             split = lambda t: t.view(B, -1, self.heads, d).transpose(1, 2)
             out = self.o(attention(split(self.q(x)), split(self.k(ctx)), split(self.v(ctx)), key_mask=ctx_mask))
             return out if residual is None else out + residual
