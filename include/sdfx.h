@@ -613,7 +613,7 @@ int sdfx_attention_train_backward(const void* q, const void* k, const void* v, c
  *   infinity or a NaN and decodes as NaN). pre[N, C] may be NULL.
  * backward: x is the forward's x, or its saved8 with eight_bits != 0. dx / dpre / dgamma / dbeta may each be NULL. With the 8-bit input the
  *   derivative is evaluated at the decoded x with the forward's statistics.
- * scratch: sdfx_group_norm_train_scratch_bytes(N, HW, C, G) bytes, uninitialised (0: the shape is not taken).
+ * scratch: sdfx_group_norm_train_scratch_bytes(N, HW, C, G) bytes, 8-byte aligned, uninitialised (0: the shape is not taken).
  */
 uint64_t sdfx_group_norm_train_scratch_bytes(uint32_t N, uint32_t HW, uint32_t C, uint32_t G);
 int sdfx_group_norm_train_forward(const void* x, const void* pre, const void* gamma, const void* beta, uint32_t N, uint32_t HW, uint32_t C, uint32_t G,

@@ -5,8 +5,10 @@
 //   dz = dy silu'(z), dbeta = sum dz, dgamma = sum dz xh, g = dz gamma, dx = rstd (g - mean(g) - xh mean(g xh)), dpre = sum over pixels of dx
 // Memory bound: forward two reads and a write of the map (+ half a write of codes), backward two reads of x and dy and a write. With the
 // 8-bit input the backward's reads of x halve.
-//   forward   k_stats     per (sample, pixel slab): sums of d and d^2 per group, d = u - pivot, pivot = the group's first value: the
-//                         difference E[d^2] - E[d]^2 stays accurate for a map whose mean is far from zero
+//   forward   k_stats     per (sample, pixel slab): sums of d and d^2 per group, d = u - pivot, pivot = the group's first value, in double:
+//                         E[d^2] - E[d]^2 loses (mean of d / deviation)^2 of 2^-53. That ratio is 0 for a constant map wherever it lies, and
+//                         at most the root of the group's size where the first value is an outlier (whose own square is in the deviation).
+//                         In float32 such an outlier cost 3 to 5 digits of rstd; double's fma runs at float32's rate here
 //             k_finish    per (sample, group): slab partials combined in double -> mean, rstd. Up to kInlineSlabs slabs a sample every
 //                         workgroup of k_apply combines them itself (one launch less; at most 64 KB out of L2 each)
 //             k_apply     y, and the 8-bit form of x
@@ -74,9 +76,9 @@ struct GroupWalk {
     __device__ __forceinline__ GroupWalk(const Shape& s, uint32_t c) : g(c / s.cpg), r(c - g * s.cpg) {}
     __device__ __forceinline__ void next(const Shape& s) { if (++r == s.cpg) { r = 0; g++; } }
 };
-template <typename T> __device__ __forceinline__ float pivot_of(const T* x, const T* pre, const Shape& s, uint32_t n, uint32_t g) {
-    const float p = pre ? (float)pre[(size_t)n * s.C + g * s.cpg] : 0.f;
-    return (float)x[(size_t)n * s.HW * s.C + g * s.cpg] + p;
+template <typename T> __device__ __forceinline__ double pivot_of(const T* x, const T* pre, const Shape& s, uint32_t n, uint32_t g) {
+    const double p = pre ? (double)(float)pre[(size_t)n * s.C + g * s.cpg] : 0.0;
+    return (double)(float)x[(size_t)n * s.HW * s.C + g * s.cpg] + p;
 }
 __device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
@@ -89,14 +91,14 @@ struct Partials { uint32_t item, slab; };
 __host__ __device__ inline Partials partials_of(const Shape& s) { return s.inl ? Partials{1u, 2u * s.G} : Partials{s.slabs, 1u}; }
 
 // every workgroup's own combination: sums[2 G] in LDS (doubles), scr LDS doubles [threads]; the same order in every workgroup
-__device__ __forceinline__ void combine_inline(const Shape& s, const float* __restrict__ partial, double* scr, double* sums) {
+template <typename P> __device__ __forceinline__ void combine_inline(const Shape& s, const P* __restrict__ partial, double* scr, double* sums) {
     const uint32_t K = 2 * s.G, J = s.threads >= K ? s.threads / K : 1u;
     for (uint32_t k0 = 0; k0 < K; k0 += s.threads) {                      // (one round unless the workgroup has fewer threads than items)
         const uint32_t j = threadIdx.x / (K < s.threads ? K : s.threads), k = k0 + threadIdx.x - j * (K < s.threads ? K : s.threads);
         double a = 0.0;
         if (j < J && k < K) {
             for (uint32_t w = j; w < s.slabs; w += 8 * J) {                // eight partials a trip, loaded together
-                float v[8];
+                P v[8];
 #pragma unroll
                 for (uint32_t u = 0; u < 8; u++) v[u] = partial[(size_t)min(w + u * J, s.slabs - 1) * K + k];
 #pragma unroll
@@ -119,24 +121,26 @@ __device__ __forceinline__ void moments(const Shape& s, const T* x, const T* pre
     a /= cnt; b /= cnt;
     double var = b - a * a;
     var = var > 0.0 || var != var ? var : 0.0;                             // (a NaN stays one)
-    mean = (float)((double)pivot_of(x, pre, s, n, g) + a);
+    mean = (float)(pivot_of(x, pre, s, n, g) + a);
     rstd = (float)(1.0 / sqrt(var + (double)s.eps));
 }
 
 // ---- forward --------------------------------------------------------------------------------------------------------------------
 template <typename T>
-__global__ __launch_bounds__(kMaxThreads) void k_stats(const T* __restrict__ x, const T* __restrict__ pre, Shape s, float* __restrict__ partial) {
-    extern __shared__ float part[];          // [2][ppi][C], then [2][C]
+__global__ __launch_bounds__(kMaxThreads) void k_stats(const T* __restrict__ x, const T* __restrict__ pre, Shape s, double* __restrict__ partial) {
+    extern __shared__ double sums[];         // [2][ppi][C]; the sums over ppi end in the first of it
     const uint32_t n = blockIdx.x / s.slabs, slab = blockIdx.x - n * s.slabs;
     uint32_t pp, cv;
     if (my_place(s, pp, cv)) {
-        float e[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sum[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sq[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (pre) widen(load8(pre + (size_t)n * s.C + cv * 8), e);
+        float f0[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        double e[8], sum[8], sq[8];
+        if (pre) widen(load8(pre + (size_t)n * s.C + cv * 8), f0);
         GroupWalk w(s, cv * 8);
-        float pivot = pivot_of(x, pre, s, n, w.g);
+        double pivot = pivot_of(x, pre, s, n, w.g);
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            e[i] -= pivot;
+            sum[i] = sq[i] = 0.0;
+            e[i] = (double)f0[i] - pivot;
             const uint32_t g = w.g;
             w.next(s);
             if (i < 7 && w.g != g) pivot = pivot_of(x, pre, s, n, w.g);
@@ -153,47 +157,47 @@ __global__ __launch_bounds__(kMaxThreads) void k_stats(const T* __restrict__ x, 
                 float f[8];
                 widen(v[u], f);
 #pragma unroll
-                for (int i = 0; i < 8; i++) { const float d = f[i] + e[i]; sum[i] += d; sq[i] = __builtin_fmaf(d, d, sq[i]); }
+                for (int i = 0; i < 8; i++) { const double d = (double)f[i] + e[i]; sum[i] += d; sq[i] = __builtin_fma(d, d, sq[i]); }
             }
         }
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            part[(size_t)pp * s.C + cv * 8 + i] = sum[i];
-            part[(size_t)(s.ppi + pp) * s.C + cv * 8 + i] = sq[i];
+            sums[(size_t)pp * s.C + cv * 8 + i] = sum[i];
+            sums[(size_t)(s.ppi + pp) * s.C + cv * 8 + i] = sq[i];
         }
     }
     __syncthreads();
-    float* chan = part + 2 * s.ppi * s.C;
-    for (uint32_t k = threadIdx.x; k < 2 * s.C; k += s.threads) {
+    for (uint32_t k = threadIdx.x; k < 2 * s.C; k += s.threads) {           // (a thread reads and writes its own column)
         const uint32_t which = k >= s.C, c = k - which * s.C;
-        float a = 0.f;
-        for (uint32_t p = 0; p < s.ppi; p++) a += part[(size_t)(which * s.ppi + p) * s.C + c];
-        chan[k] = a;
+        double* col = sums + (size_t)which * s.ppi * s.C + c;
+        double a = 0.0;
+        for (uint32_t p = 0; p < s.ppi; p++) a += col[(size_t)p * s.C];
+        col[0] = a;
     }
     __syncthreads();
     const Partials lay = partials_of(s);
     for (uint32_t k = threadIdx.x; k < 2 * s.G; k += s.threads) {
         const uint32_t which = k & 1u, g = k >> 1;
-        float a = 0.f;
-        for (uint32_t c = 0; c < s.cpg; c++) a += chan[which * s.C + g * s.cpg + c];
+        double a = 0.0;
+        for (uint32_t c = 0; c < s.cpg; c++) a += sums[(size_t)which * s.ppi * s.C + g * s.cpg + c];
         partial[(size_t)n * 2 * s.G * s.slabs + (size_t)k * lay.item + (size_t)slab * lay.slab] = a;
     }
 }
 
 // one wave per (sample, group)
 template <typename T>
-__global__ __launch_bounds__(64) void k_finish(const T* __restrict__ x, const T* __restrict__ pre, const float* __restrict__ partial, Shape s,
+__global__ __launch_bounds__(64) void k_finish(const T* __restrict__ x, const T* __restrict__ pre, const double* __restrict__ partial, Shape s,
                                              float* __restrict__ mean_rstd) {
     const uint32_t n = blockIdx.x / s.G, g = blockIdx.x - n * s.G;
-    const float* p = partial + (size_t)blockIdx.x * 2 * s.slabs;
+    const double* p = partial + (size_t)blockIdx.x * 2 * s.slabs;
     double a = 0.0, b = 0.0;
-    for (uint32_t w = threadIdx.x; w < s.slabs; w += 64) { a += (double)p[w]; b += (double)p[s.slabs + w]; }
+    for (uint32_t w = threadIdx.x; w < s.slabs; w += 64) { a += p[w]; b += p[s.slabs + w]; }
     a = wave_sum(a); b = wave_sum(b);
     if (threadIdx.x == 0) moments(s, x, pre, n, g, a, b, mean_rstd[(size_t)blockIdx.x * 2], mean_rstd[(size_t)blockIdx.x * 2 + 1]);
 }
 
 template <typename T, bool ACT, bool Q8>
-__global__ __launch_bounds__(kMaxThreads) void k_apply(const T* __restrict__ x, const T* __restrict__ pre, Shape s, const float* __restrict__ partial,
+__global__ __launch_bounds__(kMaxThreads) void k_apply(const T* __restrict__ x, const T* __restrict__ pre, Shape s, const double* __restrict__ partial,
                                                         float* __restrict__ mean_rstd, const void* __restrict__ gamma, const void* __restrict__ beta,
                                                         T* __restrict__ y, u2n* __restrict__ codes, uint8_t* __restrict__ scales) {
     __shared__ double scr[kMaxThreads], sums[2 * kMaxGroups];
@@ -438,16 +442,17 @@ __global__ __launch_bounds__(kMaxThreads) void k_bwd_apply(const void* __restric
 }
 
 // ---- launches -------------------------------------------------------------------------------------------------------------------
-uint64_t group_floats(const Shape& s) { return (uint64_t)s.N * 2 * s.G * s.slabs; }
+uint64_t group_floats(const Shape& s) { return (uint64_t)s.N * 2 * s.G * s.slabs; }      // (the forward's are doubles: within the backward's total, since G <= C)
 uint64_t chan_floats(const Shape& s) { return (uint64_t)s.N * 3 * s.C * s.slabs; }
 
 template <typename T, bool ACT, bool Q8>
 void forward(const void* x_, const void* pre_, const void* gamma, const void* beta, const Shape& s, void* y, uint8_t* saved, float* mean_rstd,
              float* scratch, hipStream_t st) {
+    double* partial = reinterpret_cast<double*>(scratch);
     const T *x = static_cast<const T*>(x_), *pre = static_cast<const T*>(pre_);
-    hipLaunchKernelGGL(k_stats<T>, dim3(s.N * s.slabs), dim3(s.threads), (2 * s.ppi + 2) * s.C * 4, st, x, pre, s, scratch);
-    if (!s.inl) hipLaunchKernelGGL(k_finish<T>, dim3(s.N * s.G), dim3(64), 0, st, x, pre, scratch, s, mean_rstd);
-    hipLaunchKernelGGL((k_apply<T, ACT, Q8>), dim3(s.N * s.slabs), dim3(s.threads), 0, st, x, pre, s, scratch, mean_rstd, gamma, beta, static_cast<T*>(y),
+    hipLaunchKernelGGL(k_stats<T>, dim3(s.N * s.slabs), dim3(s.threads), 2 * s.ppi * s.C * 8, st, x, pre, s, partial);
+    if (!s.inl) hipLaunchKernelGGL(k_finish<T>, dim3(s.N * s.G), dim3(64), 0, st, x, pre, partial, s, mean_rstd);
+    hipLaunchKernelGGL((k_apply<T, ACT, Q8>), dim3(s.N * s.slabs), dim3(s.threads), 0, st, x, pre, s, partial, mean_rstd, gamma, beta, static_cast<T*>(y),
                        reinterpret_cast<u2n*>(saved), saved + (size_t)s.N * s.HW * s.C);
 }
 template <typename T, bool ACT, bool Q8, bool PRE>
@@ -513,7 +518,8 @@ int sdfx_group_norm_train_forward(const void* x, const void* pre, const void* ga
     SDFX_REQUIRE(make_shape(N, HW, C, G, s), "group_norm_train_forward: needs C %% 8 == 0, C %% G == 0, C <= %u, G <= %u and N < 2^23 (got N=%u HW=%u C=%u G=%u)",
                  kMaxThreads * 8, kMaxGroups, N, HW, C, G);
     SDFX_REQUIRE(!saved8 || C % 32 == 0, "group_norm_train_forward: the 8-bit form needs C %% 32 == 0 (got %u)", C);
-    SDFX_REQUIRE(aligned16(x) && aligned16(y) && aligned16(saved8) && aligned16(pre) && aligned16(gamma) && aligned16(beta), "group_norm_train_forward: misaligned pointer");
+    SDFX_REQUIRE(aligned16(x) && aligned16(y) && aligned16(saved8) && aligned16(pre) && aligned16(gamma) && aligned16(beta) &&
+                 reinterpret_cast<uintptr_t>(scratch) % 8 == 0, "group_norm_train_forward: misaligned pointer");
     SDFX_REQUIRE(eps >= 0.f, "group_norm_train_forward: negative eps");
     s.eps = eps; s.pf32 = params_f32 || dtype == 2;
     const bool eight = saved8 != nullptr;
