@@ -54,16 +54,19 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
     const bool seen = key < s.Nk && (!s.mask || s.mask[(size_t)b * s.Nk + kc] != 0);
     const bool wave_on = __ballot(seen) != 0;
     // fp16: ds g (g from grad_scale, |ds g| <= 1) times 2^15 is what the second product takes. g is put into v (`gv`, so that dp comes out with it)
-    // as long as the largest |v g| stays in 2^-6 .. 2^12, well inside fp16; beyond, what is left of it goes into the shift of p (large
-    // dy) or is left out (small dy: ds is then 2^-12 of its bound and more, still normal).
-    float gv = 1.f, shift = Half<T>::kShift, md = 1.f;
+    // where that is exact: not below 1, at which small values would leave fp16's normal numbers and dp no longer cancel against delta (dk of
+    // rows that one of two keys carries by 12 nats, dy of 64: 10 % off), and with the largest |v g| up to 2^12. What is left of g
+    // (`gr`) takes a multiplication a score. Only where |dy| |v| passes 2^28 is gv under 1: delta's parts end at 2^31, and such a v has no
+    // value that gv brings under 2^-33 of the row's largest.
+    constexpr float shift = Half<T>::kShift;
+    float gv = 1.f, gr = 1.f, md = 1.f;
     if (Half<T>::kScaled) {
         float vmax;
         const float g = grad_scale(a.rows2 + (size_t)bh * prep_blocks(s.rows), prep_blocks(s.rows), a.v2 + (size_t)bh * prep_blocks(s.Nk), prep_blocks(s.Nk), lane, vmax);
         const float v1 = __uint_as_float(__float_as_uint(fminf(fmaxf(vmax, 1e-30f), 1e30f)) & 0x7f800000u);       // a power of two, vmax in v1 .. 2 v1
-        gv = fminf(fmaxf(g, 0.015625f / v1), 4096.f / v1);
-        if (gv > g) shift = fmaxf(Half<T>::kShift - __builtin_amdgcn_logf(gv / g), 0.f);
-        md = 0.5f * gv / g;                                              // >= the largest |delta gv|
+        gv = fmaxf(fminf(g, 4096.f / v1), fminf(1.f, g * 0x1p29f));
+        gr = g / gv;
+        md = 0.5f / gr;                                                  // >= the largest |delta gv|
     }
     // weights of the parts: scores as (shift - lse) / c reaches 2^28 in fp16
     const float ws = Half<T>::kScaled ? 4096.f : 1.f, wd = Half<T>::kScaled ? fminf(fmaxf(md, 1.f / 8192.f), 32768.f) : 1.f;
@@ -195,6 +198,11 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
                     sc[st][r] = __builtin_amdgcn_exp2f(sc[st][r] * s.c);
                     dp[st][r] = sc[st][r] * dp[st][r];
                 }
+                if (Half<T>::kScaled && gr != 1.f) {
+                    keep_branch();
+#pragma unroll
+                    for (int r = 0; r < 16; r++) dp[st][r] *= gr;
+                }
                 if (EX && lone) {
                     keep_branch();
                     const uint32_t bits = (uint32_t)(lone >> (32 * st)) >> (4u * hi);
@@ -230,7 +238,7 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
         __syncthreads();
     }
     if (key >= s.Nk) return;
-    const float fv = __builtin_amdgcn_exp2f(-shift), fk = s.scale * fv / gv;
+    const float fv = __builtin_amdgcn_exp2f(-shift), fk = s.scale * fv / gv / gr;
     const size_t at = (size_t)bh * s.Nk + key, pa = ((size_t)split * s.B * s.Hk * s.Nk + at) * s.D;
     const size_t oa = (((size_t)b * s.Nk + key) * s.Hk + hk) * s.D;
 #pragma unroll

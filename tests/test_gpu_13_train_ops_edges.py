@@ -67,3 +67,57 @@ def test_group_norm_and_its_gradient_beside_an_outlier(dev, dtype, first, checkp
     got = dict(zip(("dx", "dweight", "dbias"), torch.autograd.grad(y, leaves, dy)), y=y.detach())
     for n, (want, bound) in ref.group_norm(x, 8, w, b, dy, eight=checkpoint == "int8").items():
         ref.check(n, got[n], want, bound)
+
+
+# ---- attention ------------------------------------------------------------------------------------------------------------------
+def _heads(dev, B, H, N, d, seed, dtype, scale=1.0):
+    return _rn(dev, B, N, H * d, seed=seed, dtype=dtype, scale=scale).view(B, N, H, d).transpose(1, 2)
+
+
+def _attend(q, k, v, dy, mask=None, causal=False, scale=None):
+    q, k, v = (t.detach().requires_grad_(True) for t in (q, k, v))
+    o = attention(q, k, v, mask, causal, scale)
+    return [o.detach(), *torch.autograd.grad(o, (q, k, v), dy)]
+
+
+def _compare(got, want, bound):
+    for n, g, w, b in zip(("o", "dq", "dk", "dv"), got, want, bound):
+        ref.check(n, g, w, b)
+
+
+@pytest.mark.parametrize("H,Hk,Nq,Nk,d,spread", [(4, 4, 300, 200, 64, 1.0), (4, 2, 40, 2, 40, 3.0), (2, 2, 600, 700, 128, 1.0), (2, 1, 90, 33, 160, 2.0)])
+def test_fp16_attention_gradients_follow_a_loss_scale(dev, H, Hk, Nq, Nk, d, spread):
+    """dy times a power of two gives the gradients times it where both are normal numbers: dv bit for bit (it knows no scale), dq and dk but for
+    what float32 rounds on the way, 2^-21 of a probability, which moves one in 2^10 of the half-precision roundings of ds by 2^-11: 2^-16 of
+    the 2-norm, allowed 2^-14."""
+    q, k = (_heads(dev, 1, h, n, d, i, F16, spread) for i, (h, n) in enumerate(((H, Nq), (Hk, Nk)), 1))
+    v, dy = _heads(dev, 1, Hk, Nk, d, 3, F16), _rn(dev, 1, Nq, H * d, seed=4)
+    dy = torch.where(dy.abs() < 2.0 ** -4, torch.zeros_like(dy), dy)            # (2^-8 of it is exact in fp16)
+    want = _attend(q, k, v, dy)[1:]
+    for e in (-8, -3, 5, 9):
+        for n, g, w in zip(("dq", "dk", "dv"), _attend(q, k, v, dy * 2.0 ** e)[1:], want):
+            a, b = g.double() * 2.0 ** -e, w.double()
+            both = (b.abs() * min(1.0, 2.0 ** e) >= 2.0 ** -14) & (b.abs() * max(1.0, 2.0 ** e) < 65504)
+            assert both.float().mean() > 0.02, (n, e)
+            assert torch.equal(a[both], b[both]) if n == "dv" else float((a - b)[both].norm() / b[both].norm()) <= 2.0 ** -14, (n, e)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("gap", [9.0, 12.0])
+def test_a_row_that_one_of_two_keys_nearly_carries_keeps_its_gradient(dev, dtype, gap):
+    """512 rows of two keys, one of which has a share of e^-gap: dq and dk are what that share leaves, found as p (dp - delta). dp and delta are
+    float32 sums of d = 64 products of size 1, each addition off by at most half a step of the running sum: with rms 0.29 steps at random, the
+    running sum of j products having a size of sqrt(j), 0.29 * 2^-23 * sqrt(64 * 64 / 2) = 1.6e-6 in dp and no more in delta: 2.2e-6 beside
+    share * |dp_1 - dp_2| = share * 11. At 14 nats (8e-7) that is a quarter of the dominant key's ds, half of which energy is in dq and dk: 0.18
+    of their 2-norm, allowed 0.25; at 12 and 9 nats 0.03 and 0.01 with the type's own rounding, allowed 0.05."""
+    B, H, d = 64, 8, 64
+    q = _rn(dev, B, H, 1, d, seed=1, dtype=F32)
+    q = q * (8 / q.norm(dim=-1, keepdim=True))
+    k = torch.cat([q * (gap / 8), torch.zeros_like(q)], dim=2).to(dtype)
+    k[:, :, 1] = _rn(dev, B, H, d, seed=2, dtype=dtype, scale=0.05)
+    q, v, dy = q.to(dtype), _rn(dev, B, H, 2, d, seed=3, dtype=dtype), _rn(dev, B, 1, H * d, seed=4, dtype=dtype)
+    dy = dy * 64                                                            # (fp16: results far above 2^-24)
+    got, (want, _) = _attend(q, k, v, dy), ref.attention(q, k, v, dy)
+    for n, g, w in list(zip(("o", "dq", "dk", "dv"), got, want))[1:3]:
+        err = float((g.cpu().double() - w).norm() / w.norm())
+        assert err <= (0.25 if gap == 14.0 else 0.05), (n, err)
