@@ -202,12 +202,13 @@ __host__ __device__ inline uint32_t prep_blocks(uint32_t n) { return (n + kPrepR
 struct BwdArgs {
     const void *q, *k, *v, *dy;
     const float *lse, *delta, *rows2, *v2;
+    const uint32_t* seen2;                 // [B][2]: the first two keys of a batch entry's mask that are seen, Nk where there is none (null: no mask)
     void *dq, *dk, *dv;                    // T [B, Nq, H, D], [B, Nk, Hk, D] (or null: not wanted)
     float *part, *part2;                   // splits > 1: float32 [splits][B Hk][rows or Nk][D] of dq, or of dk and dv
 };
 constexpr int kWidths[] = {48, 64, 80, 128, 160, 256};      // channels a kernel is built for; a head takes the next of them
 
-// attention_train_dq.hip, attention_train_dkdv.hip: launch (shape's tiles_x / splits / per_split set for `waves` a workgroup)
+// attention_train_dq.hip, attention_train_dkdv.hip: launch (shape's tiles_x / splits set for `waves` a workgroup)
 void launch_dq(const BwdArgs& a, const Shape& s, int bf16, int waves, hipStream_t st);
 void launch_dkdv(const BwdArgs& a, const Shape& s, int bf16, hipStream_t st);
 // rows of the tile each stages: keys (forward, dq) or queries (dk / dv). One wave alone takes 32 and needs one buffer: its next tile waits in
@@ -246,17 +247,22 @@ __device__ __forceinline__ uint32_t split_at(uint32_t n, uint32_t i, uint32_t sp
 //    Marking rows below 16 gains nothing that shows and costs dq 14 us at 4096 x 40, this 4.
 //  - at most 512 rows to a key head or at most 128 keys (`exact`: every row is marked, and dv takes the product too): sums of a
 //    few, or of probabilities that all lie at one place between two powers of two, are up to 2.5 times as far off.
-// A row that one key carries alone has no ds: dp and delta are the same number, and the few bits that differ would be all of the gradient
-// where no row has another. Its sum is 1 but for the exponent's rounding, half a unit of the maximum m's last place; other keys with as little
-// are taken for none (at m = 20 1.3e-6, about where dp - delta ends; beyond 64 the allowance grows no more).
-// The marks are the log-sum-exp's two lowest bits (2^-22 of it): the forward knows the sum, the backward only its logarithm.
+// The mark is the log-sum-exp's lowest bit (2^-23 of it): the forward knows the sum, the backward only its logarithm.
 __device__ __forceinline__ float mark_row(float m, float l, float few) {
     const float lse = m + __builtin_amdgcn_logf(l);
-    const uint32_t u = __float_as_uint(lse) & ~3u;
-    return lse < INFINITY ? __uint_as_float(__builtin_fabsf(l - 1.f) <= fminf(__builtin_fabsf(m), 64.f) * 0x1p-24f + 0x1p-23f ? u | 3u : l < few ? u | 1u : u) : lse;
+    const uint32_t u = __float_as_uint(lse) & ~1u;
+    return lse < INFINITY ? __uint_as_float(l < few ? u | 1u : u) : lse;
 }
 __device__ __forceinline__ bool marked(float lse) { return lse < INFINITY && (__float_as_uint(lse) & 1u); }
-__device__ __forceinline__ bool alone(float lse) { return lse < INFINITY && (__float_as_uint(lse) & 3u) == 3u; }
+
+// A row that sees one key has no ds: dp and delta are the same number, and the bits in which they differ would be all of the gradient where no
+// row has another. Which rows those are follows from the masks alone: with f1 < f2 the first two keys of the batch entry's mask, a row
+// whose last key is `lim` sees none if lim < f1, one (f1) if f1 <= lim < f2, more otherwise.
+struct TwoSeen { int f1, f2; };
+__device__ __forceinline__ TwoSeen two_seen(const BwdArgs& a, uint32_t b) {
+    if (!a.seen2) return {0, 1};
+    return {(int)a.seen2[2 * b], (int)a.seen2[2 * b + 1]};
+}
 // what rounding elements 8 e .. 8 e + 7 of a D fragment to `hi` left, as an operand
 template <typename T> __device__ __forceinline__ typename Half<T>::v8 left_over(const f32x16& p, int e, const typename Half<T>::v8& hi) {
     typename Half<T>::v8 v;

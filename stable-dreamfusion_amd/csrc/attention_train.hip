@@ -292,12 +292,44 @@ __global__ __launch_bounds__(256) void k_join_sum(JoinSums js, uint32_t B, uint3
 // ---- ahead of the gradient's kernels ---------------------------------------------------------------------------------------------
 // delta[b, h, i] = sum over channels of dy (o + o_lo): o_lo is what rounding o to 16 bits left, without which ds = p (dp - delta) of a
 // peaked row loses the digits the subtraction cancels (bf16, scores with a deviation of 4: dq 5.8e-3 off instead of 2.4e-3). Also the
-// block maxima of |dy row|^2 and |v row|^2 that grad_scale reads (fp16). LR lanes a row.
+// block maxima of |dy row|^2 and |v row|^2 that grad_scale reads (fp16), and with a mask each batch entry's first two keys (two_seen).
+// LR lanes a row.
+__device__ __forceinline__ void find_two(const uint8_t* __restrict__ mask, uint32_t Nk, uint32_t* lds, uint32_t* __restrict__ two) {
+    if (threadIdx.x < 2) lds[threadIdx.x] = Nk;
+    uint32_t f1 = Nk, f2 = Nk;                                    // of the keys this thread has looked at
+    for (uint32_t k0 = 0; k0 < Nk; k0 += 256 * 16) {              // sixteen a trip, loaded together; every thread leaves after the trip that found two
+        uint8_t m[16];
+#pragma unroll
+        for (uint32_t u = 0; u < 16; u++) m[u] = mask[min(k0 + u * 256 + threadIdx.x, Nk - 1u)];
+#pragma unroll
+        for (uint32_t u = 0; u < 16; u++) {
+            const uint32_t k = k0 + u * 256 + threadIdx.x;
+            if (k >= Nk || !m[u]) continue;
+            if (f1 == Nk) f1 = k;
+            else if (f2 == Nk) f2 = k;
+        }
+        if (__syncthreads_count(f1 < Nk) + __syncthreads_count(f2 < Nk) >= 2) break;
+    }
+    __syncthreads();
+    atomicMin(&lds[0], f1);
+    __syncthreads();
+    atomicMin(&lds[1], f1 == lds[0] ? f2 : f1);
+    __syncthreads();
+    if (threadIdx.x < 2) two[threadIdx.x] = lds[threadIdx.x];
+}
 template <typename T, int LR>
 __global__ __launch_bounds__(256) void k_prep(const T* __restrict__ v, const T* __restrict__ o, const T* __restrict__ o_lo, const T* __restrict__ dy,
-                                             const float* __restrict__ lse, Shape s, float* __restrict__ delta, float* __restrict__ rows2, float* __restrict__ v2) {
+                                             const float* __restrict__ lse, Shape s, float* __restrict__ delta, float* __restrict__ rows2, float* __restrict__ v2,
+                                             uint32_t* __restrict__ seen2) {
     __shared__ float red[256 / LR];
+    __shared__ uint32_t two[2];
     const uint32_t nr = prep_blocks(s.rows), nv = prep_blocks(s.Nk), bh_n = s.B * s.Hk;
+    const uint32_t masks = bh_n * (nr + (Half<T>::kScaled ? nv : 0));          // the workgroups from here on take a mask each
+    if (blockIdx.x >= masks) {
+        const uint32_t b = blockIdx.x - masks;
+        find_two(s.mask + (size_t)b * s.Nk, s.Nk, two, seen2 + 2 * b);
+        return;
+    }
     const bool of_v = blockIdx.x >= bh_n * nr;
     const uint32_t id = of_v ? blockIdx.x - bh_n * nr : blockIdx.x, per = of_v ? nv : nr;
     const uint32_t bh = id / per, blk = id - bh * per, b = bh / s.Hk, hk = bh - b * s.Hk;
@@ -385,13 +417,13 @@ template <typename T> void join_o(const float* part, const float* ml, const Shap
     hipLaunchKernelGGL(k_join_o<T>, dim3((uint32_t)((n + rows_here - 1) / rows_here)), dim3(256), 0, st, part, ml, s, parts, static_cast<T*>(o),
                        static_cast<T*>(o_lo), lse);
 }
-template <typename T> void prep(const void* v, const void* o, const void* o_lo, const void* dy, const float* lse, const Shape& s, float* delta, float* rows2, float* v2, hipStream_t st) {
+template <typename T> void prep(const void* v, const void* o, const void* o_lo, const void* dy, const float* lse, const Shape& s, float* delta, float* rows2, float* v2, uint32_t* seen2, hipStream_t st) {
     const uint32_t bh = s.B * s.Hk;
-    const dim3 grid(bh * (prep_blocks(s.rows) + (Half<T>::kScaled ? prep_blocks(s.Nk) : 0)));
+    const dim3 grid(bh * (prep_blocks(s.rows) + (Half<T>::kScaled ? prep_blocks(s.Nk) : 0)) + (s.mask ? s.B : 0));
     const T *vp = static_cast<const T*>(v), *op = static_cast<const T*>(o), *lp = static_cast<const T*>(o_lo), *yp = static_cast<const T*>(dy);
-    if (s.D <= 64) hipLaunchKernelGGL((k_prep<T, 8>), grid, dim3(256), 0, st, vp, op, lp, yp, lse, s, delta, rows2, v2);
-    else if (s.D <= 128) hipLaunchKernelGGL((k_prep<T, 16>), grid, dim3(256), 0, st, vp, op, lp, yp, lse, s, delta, rows2, v2);
-    else hipLaunchKernelGGL((k_prep<T, 32>), grid, dim3(256), 0, st, vp, op, lp, yp, lse, s, delta, rows2, v2);
+    if (s.D <= 64) hipLaunchKernelGGL((k_prep<T, 8>), grid, dim3(256), 0, st, vp, op, lp, yp, lse, s, delta, rows2, v2, seen2);
+    else if (s.D <= 128) hipLaunchKernelGGL((k_prep<T, 16>), grid, dim3(256), 0, st, vp, op, lp, yp, lse, s, delta, rows2, v2, seen2);
+    else hipLaunchKernelGGL((k_prep<T, 32>), grid, dim3(256), 0, st, vp, op, lp, yp, lse, s, delta, rows2, v2, seen2);
 }
 
 const char* shape_error(uint32_t B, uint32_t H, uint32_t Hk, uint32_t Nq, uint32_t Nk, uint32_t D) {
@@ -427,7 +459,7 @@ bool strides_ok(const uint64_t* a, const uint64_t* b, const uint64_t* c) {
     return all % 8 == 0 && token < (1ull << 24);
 }
 uint64_t up16(uint64_t floats) { return (floats + 3) / 4 * 4; }
-struct BwdLayout { uint64_t rows2, v2, pq, pk, pv, total; };   // float offsets behind delta
+struct BwdLayout { uint64_t rows2, v2, seen2, pq, pk, pv, total; };   // float offsets behind delta
 BwdLayout bwd_layout(const Shape& s0) {
     Shape a = s0, b = s0;
     int waves;
@@ -437,7 +469,8 @@ BwdLayout bwd_layout(const Shape& s0) {
     BwdLayout l;
     l.rows2 = up16(heads * s0.rows);
     l.v2 = l.rows2 + up16(heads * prep_blocks(s0.rows));
-    l.pq = l.v2 + up16(heads * prep_blocks(s0.Nk));
+    l.seen2 = l.v2 + up16(heads * prep_blocks(s0.Nk));
+    l.pq = l.seen2 + up16(2ull * s0.B);
     l.pk = l.pq + (a.splits > 1 ? a.splits * heads * s0.rows * s0.D : 0);
     const uint64_t one = b.splits > 1 ? b.splits * heads * s0.Nk * s0.D : 0;
     l.pv = l.pk + one;
@@ -510,8 +543,10 @@ int sdfx_attention_train_backward(const void* q, const void* k, const void* v, c
     a.q = q; a.k = k; a.v = v; a.dy = dy; a.lse = lse;
     a.delta = scratch; a.rows2 = scratch + l.rows2; a.v2 = scratch + l.v2;
     a.dq = dq; a.dk = dk; a.dv = dv;
-    if (bf16) prep<__bf16>(v, o, o_lo, dy, lse, s, scratch, scratch + l.rows2, scratch + l.v2, st);
-    else prep<_Float16>(v, o, o_lo, dy, lse, s, scratch, scratch + l.rows2, scratch + l.v2, st);
+    uint32_t* seen2 = reinterpret_cast<uint32_t*>(scratch + l.seen2);
+    a.seen2 = s.mask ? seen2 : nullptr;
+    if (bf16) prep<__bf16>(v, o, o_lo, dy, lse, s, scratch, scratch + l.rows2, scratch + l.v2, seen2, st);
+    else prep<_Float16>(v, o, o_lo, dy, lse, s, scratch, scratch + l.rows2, scratch + l.v2, seen2, st);
     JoinSums js;
     uint32_t joins = 0;
     uint64_t most = 0;

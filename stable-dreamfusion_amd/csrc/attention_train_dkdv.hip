@@ -135,16 +135,21 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
             qp += (uint64_t)QT * s.q_sn; yp += (uint64_t)QT * y_sn; stat_at += QT;
         }
     };
+    // Queries ahead of `lone_end` see one key at most (two_seen): staged as zeros with a log-sum-exp of 0 they have p = 1 there and, whatever
+    // ds comes to, add nothing to dk: no branch in the products' loop.
+    const TwoSeen two = two_seen(a, b);
+    const int lone_end = s.causal ? two.f2 - s.off : two.f2 >= (int)s.Nk ? 0x7fffffff : 0;
     bool few = false;                                                    // (some row of the tile)
-    uint64_t lone = 0;                                                   // the tile's rows that one key carries alone
     auto put = [&](uint32_t buf) {
         const uint32_t left = s.Nq - nq0;
         uint64_t live = left >= 64u ? ~0ull : (1ull << left) - 1ull;
         if (empties) live &= __ballot(r_lse != INFINITY);
         const bool whole = left >= (uint32_t)QT && !empties;
-        if (EX) lone = __ballot(alone(r_lse));
-        else few = __ballot(marked(r_lse)) != 0;
-        stq.put(ldsQ + buf * L::BYTES, rq, whole, live);
+        if (!EX) few = __ballot(marked(r_lse)) != 0;
+        const int lone = min(lone_end - (int)nq0, 64);                   // the tile's first so many rows
+        const uint64_t lone_rows = lone <= 0 ? 0ull : lone == 64 ? ~0ull : (1ull << lone) - 1ull;
+        if ((int)lane < lone && r_lse < INFINITY) r_lse = 0.f;           // (not a row that sees nothing, nor a NaN)
+        stq.put(ldsQ + buf * L::BYTES, rq, whole && lone <= 0, live & ~lone_rows);
         sty.put(ldsY + buf * L::BYTES, ry, whole, live);
         if (lane < (uint32_t)QT) {                                       // the rows' extra channels, one tensor's by each of two waves
             if (wave == 0) *reinterpret_cast<u4v*>(ldsQ + buf * L::BYTES + lane * L::PITCH + s.D * 2u) = split_parts<T>((shift - r_lse) * inv_c, ws);
@@ -202,13 +207,6 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
                     keep_branch();
 #pragma unroll
                     for (int r = 0; r < 16; r++) dp[st][r] *= gr;
-                }
-                if (EX && lone) {
-                    keep_branch();
-                    const uint32_t bits = (uint32_t)(lone >> (32 * st)) >> (4u * hi);
-#pragma unroll
-                    for (int r = 0; r < 16; r++)
-                        if (bits & (1u << ((r & 3) + 8 * (r >> 2)))) dp[st][r] = 0.f;
                 }
 #pragma unroll
                 for (int e = 0; e < 2; e++) {

@@ -33,8 +33,11 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_dq(BwdArgs a, Sha
     const bool few = __ballot(row.on && marked(lse)) != 0;             // (some row of the wave)
     float g = 1.f, vmax;
     if (Half<T>::kScaled) g = grad_scale(a.rows2 + (size_t)bh * prep_blocks(s.rows), prep_blocks(s.rows), a.v2 + (size_t)bh * prep_blocks(s.Nk), prep_blocks(s.Nk), lane, vmax);
+    const TwoSeen two = two_seen(a, b);
+    const int last = min(row.lim, (int)s.Nk - 1);
+    const bool alone = last >= two.f1 && last < two.f2;
     // ds = p (dp - delta) g: g joins the exponent (p is used for nothing else), -delta starts dp's sum on the matrix cores
-    const float nlse = alone(lse) ? -INFINITY : Half<T>::kShift + (Half<T>::kScaled ? __builtin_amdgcn_logf(g) : 0.f) - lse, ndelta = -a.delta[at];
+    const float nlse = alone ? -INFINITY : Half<T>::kShift + (Half<T>::kScaled ? __builtin_amdgcn_logf(g) : 0.f) - lse, ndelta = -a.delta[at];
     f32x16 dp0;
 #pragma unroll
     for (int r = 0; r < 16; r++) dp0[r] = ndelta;

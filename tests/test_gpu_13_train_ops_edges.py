@@ -103,7 +103,7 @@ def test_fp16_attention_gradients_follow_a_loss_scale(dev, H, Hk, Nq, Nk, d, spr
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
-@pytest.mark.parametrize("gap", [9.0, 12.0])
+@pytest.mark.parametrize("gap", [9.0, 12.0, 14.0])
 def test_a_row_that_one_of_two_keys_nearly_carries_keeps_its_gradient(dev, dtype, gap):
     """512 rows of two keys, one of which has a share of e^-gap: dq and dk are what that share leaves, found as p (dp - delta). dp and delta are
     float32 sums of d = 64 products of size 1, each addition off by at most half a step of the running sum: with rms 0.29 steps at random, the
@@ -121,3 +121,40 @@ def test_a_row_that_one_of_two_keys_nearly_carries_keeps_its_gradient(dev, dtype
     for n, g, w in list(zip(("o", "dq", "dk", "dv"), got, want))[1:3]:
         err = float((g.cpu().double() - w).norm() / w.norm())
         assert err <= (0.25 if gap == 14.0 else 0.05), (n, err)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("H,Hk,Nq,Nk,spread", [(2, 2, 1024, 300, 1.0), (4, 1, 700, 130, 3.0), (3, 3, 70, 90, 8.0), (2, 1, 5, 4000, 8.0), (1, 1, 9, 1, 12.0)])
+def test_a_mask_that_leaves_one_key_leaves_no_gradient_of_q_and_k(dev, dtype, H, Hk, Nq, Nk, spread):
+    """Exact zeros whatever the score (up to several hundred here) and the number of rows; a second batch entry sees two keys and has gradients."""
+    B, d = 2, 64
+    q, k = (_heads(dev, B, h, n, d, i, dtype, spread) for i, (h, n) in enumerate(((H, Nq), (Hk, Nk)), 1))
+    v, dy = _heads(dev, B, Hk, Nk, d, 3, dtype), _rn(dev, B, Nq, H * d, seed=4, dtype=dtype)
+    m = torch.zeros(B, Nk, dtype=torch.bool, device=dev)
+    m[:, Nk // 2] = m[1, Nk - 1] = True
+    o, dq, dk, dv = got = _attend(q, k, v, dy, m)
+    assert not dq[0].any() and not dk[0].any() and dv[0].any()
+    assert torch.equal(o[0], v[0, :, Nk // 2].repeat_interleave(H // Hk, 0).reshape(1, -1).expand(Nq, -1))
+    if Nk > 1:
+        assert dq[1].any() and dk[1].any()
+    if spread < 8:
+        _compare(got, *ref.attention(q, k, v, dy, m))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("H,Hk,Nq,Nk,first,second", [(2, 2, 1024, 1024, 100, 600), (4, 2, 300, 900, 640, 800), (1, 1, 700, 200, 0, 150), (2, 1, 90, 90, 33, 90),
+                                                     (1, 1, 900, 900, 0, 1)])
+def test_causal_rows_between_the_first_and_the_second_key_have_no_gradient_of_q_and_k(dev, dtype, H, Hk, Nq, Nk, first, second):
+    """Rows that see key `first` alone get dq = 0 and add nothing to its dk: with dy zero elsewhere dk is zero throughout."""
+    d, off = 40, Nk - Nq
+    q, k = (_heads(dev, 1, h, n, d, i, dtype, 3.0) for i, (h, n) in enumerate(((H, Nq), (Hk, Nk)), 1))
+    v, dy = _heads(dev, 1, Hk, Nk, d, 3, dtype), _rn(dev, 1, Nq, H * d, seed=4, dtype=dtype)
+    m = (torch.arange(Nk, device=dev)[None] == first) | (torch.arange(Nk, device=dev)[None] >= second)
+    last = torch.arange(Nq, device=dev) + off
+    lone = (last >= first) & (last < second)
+    got = _attend(q, k, v, dy, m, True)
+    assert not got[1][:, :, lone].any()
+    _compare(got, *ref.attention(q, k, v, dy, m, True))
+    only = dy * lone[None, :, None]
+    o, dq, dk, dv = _attend(q, k, v, only, m, True)
+    assert not dq.any() and not dk.any() and dv.any() == lone.any()
