@@ -586,7 +586,7 @@ int sdfx_geglu(const void* x, uint64_t rows, uint32_t n, void* out, sdfx_stream_
  * accumulation and statistics. H query heads share Hk key heads (H % Hk == 0): head h reads key head h / (H / Hk). D a multiple of 8 up to
  * 256. q[b, h, n, :] is read at q + b strides[0] + n strides[1] + h strides[2] (elements, multiples of 8, strides[1] below 2^24; unit channel
  * stride; 16-byte aligned), k / v likewise over Nk keys. key_mask[B, Nk] bytes (may be NULL): 0 = no query sees the key, whatever its k and v hold.
- * causal != 0: query i sees keys <= i + Nk - Nq. A row that sees no key: o = 0, lse = +inf, no gradient. scale > 0.
+ * causal != 0: query i sees keys <= i + Nk - Nq. A row that sees no key: o = 0, lse = +inf, no gradient. scale in 1e-30 .. 1e30.
  *   Nor has a row that sees one key a gradient for q and k.
  * forward: lse[B, H, Nq] (base-2 log-sum-exp of the scaled scores; its lowest bit marks rows that few keys carry) and o_lo (what rounding o to
  *   16 bits left, same type and layout) are what the backward needs; both NULL without one.

@@ -498,7 +498,7 @@ int sdfx_attention_train_forward(const void* q, const void* k, const void* v, co
     SDFX_REQUIRE(q && k && v && o && q_strides && k_strides && v_strides, "attention_train_forward: null pointer");
     const char* e = shape_error(B, H, Hk, Nq, Nk, D);
     SDFX_REQUIRE(!e, "attention_train_forward: %s (B=%u H=%u Hk=%u Nq=%u Nk=%u D=%u)", e, B, H, Hk, Nq, Nk, D);
-    SDFX_REQUIRE(scale > 0.f && scale < 3e38f, "attention_train_forward: the scale must be positive and finite");
+    SDFX_REQUIRE(scale >= 1e-30f && scale <= 1e30f, "attention_train_forward: the scale must lie in 1e-30 .. 1e30");
     SDFX_REQUIRE(strides_ok(q_strides, k_strides, v_strides) && ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) |
                  reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(o_lo) | reinterpret_cast<uintptr_t>(scratch)) % 16) == 0,
                  "attention_train_forward: rows must be 16-byte aligned, token strides below 2^24");
@@ -529,7 +529,7 @@ int sdfx_attention_train_backward(const void* q, const void* k, const void* v, c
     SDFX_REQUIRE(!dk == !dv, "attention_train_backward: dk and dv come together");
     const char* e = shape_error(B, H, Hk, Nq, Nk, D);
     SDFX_REQUIRE(!e, "attention_train_backward: %s (B=%u H=%u Hk=%u Nq=%u Nk=%u D=%u)", e, B, H, Hk, Nq, Nk, D);
-    SDFX_REQUIRE(scale > 0.f && scale < 3e38f, "attention_train_backward: the scale must be positive and finite");
+    SDFX_REQUIRE(scale >= 1e-30f && scale <= 1e30f, "attention_train_backward: the scale must lie in 1e-30 .. 1e30");
     SDFX_REQUIRE(strides_ok(q_strides, k_strides, v_strides) && ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) |
                  reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(o_lo) | reinterpret_cast<uintptr_t>(dy) |
                  reinterpret_cast<uintptr_t>(dq) | reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv) | reinterpret_cast<uintptr_t>(scratch)) % 16) == 0,

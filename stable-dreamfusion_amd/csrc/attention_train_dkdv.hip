@@ -6,7 +6,8 @@
 // as many cycles there as the operands (8 of 30 reads a block); instead they ride in the products: a row carries 8 extra channels, q's
 // with (shift - lse) / c and dy's with -delta as sums of 16-bit parts, k's and v's with the parts' weights, powers of two. s and dp come out
 // of the matrix cores complete. Three parts: 24 bits in bf16, in fp16 as many as the
-// weights' range allows, at least 22 (with two, ds of a row of 2 keys that one carries by 1e4 to 1 was 8e-4 off).
+// weights' range allows, at least 22 (with two, ds of a row of 2 keys that one carries by 1e4 to 1 was 8e-4 off). In fp16 the weights end
+// at 2^28: a tile with a row beyond (a small scale makes (shift - lse) / c large) leaves these channels zero and takes shift - lse from LDS.
 // Bound: as dq's (2 x 8 heads, 4096 x 4096 x 40, fp16: 154 us for four products, 558 TFLOP/s). A workgroup takes one key head's tile and
 // all the rows of its query heads, so that shared heads need no atomics; few key tiles split the rows and join in float32.
 #include "attention_train.h"
@@ -43,6 +44,7 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
     constexpr int QT = query_tile(DM), KS = DP / 16, DT = (DM + 31) / 32 / CS, NB = QT / 32;
     typedef Tile<DP, QT, 64 * NW> L;
     __shared__ __attribute__((aligned(16))) uint8_t lds[4 * L::BYTES + kTileSlack];
+    __shared__ float far_stat[2][QT];
     uint8_t* const ldsY = lds;
     uint8_t* const ldsQ = lds + 2 * L::BYTES;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), x = lane & 31u, hi = lane >> 5;
@@ -68,7 +70,7 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
         gr = g / gv;
         md = 0.5f / gr;                                                  // >= the largest |delta gv|
     }
-    // weights of the parts: scores as (shift - lse) / c reaches 2^28 in fp16
+    // weights of the parts: (shift - lse) / c reaches 2^28 in fp16
     const float ws = Half<T>::kScaled ? 4096.f : 1.f, wd = Half<T>::kScaled ? fminf(fmaxf(md, 1.f / 8192.f), 32768.f) : 1.f;
     const float inv_c = 1.f / s.c;
 
@@ -139,7 +141,7 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
     // ds comes to, add nothing to dk: no branch in the products' loop.
     const TwoSeen two = two_seen(a, b);
     const int lone_end = s.causal ? two.f2 - s.off : two.f2 >= (int)s.Nk ? 0x7fffffff : 0;
-    bool few = false;                                                    // (some row of the tile)
+    bool few = false, far = false;                                       // (some row of the tile)
     auto put = [&](uint32_t buf) {
         const uint32_t left = s.Nq - nq0;
         uint64_t live = left >= 64u ? ~0ull : (1ull << left) - 1ull;
@@ -149,10 +151,14 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
         const int lone = min(lone_end - (int)nq0, 64);                   // the tile's first so many rows
         const uint64_t lone_rows = lone <= 0 ? 0ull : lone == 64 ? ~0ull : (1ull << lone) - 1ull;
         if ((int)lane < lone && r_lse < INFINITY) r_lse = 0.f;           // (not a row that sees nothing, nor a NaN)
+        if (Half<T>::kScaled) far = __ballot(lane < (uint32_t)QT && r_lse != INFINITY && __builtin_fabsf((shift - r_lse) * inv_c) > 0x1p27f) != 0;
         stq.put(ldsQ + buf * L::BYTES, rq, whole && lone <= 0, live & ~lone_rows);
         sty.put(ldsY + buf * L::BYTES, ry, whole, live);
         if (lane < (uint32_t)QT) {                                       // the rows' extra channels, one tensor's by each of two waves
-            if (wave == 0) *reinterpret_cast<u4v*>(ldsQ + buf * L::BYTES + lane * L::PITCH + s.D * 2u) = split_parts<T>((shift - r_lse) * inv_c, ws);
+            if (wave == 0) {
+                *reinterpret_cast<u4v*>(ldsQ + buf * L::BYTES + lane * L::PITCH + s.D * 2u) = split_parts<T>(far ? 0.f : (shift - r_lse) * inv_c, ws);
+                if (far) far_stat[buf][lane] = shift - r_lse;
+            }
             if (wave == 1) *reinterpret_cast<u4v*>(ldsY + buf * L::BYTES + lane * L::PITCH + s.D * 2u) = split_parts<T>(r_lse == INFINITY ? 0.f : -r_delta * gv, wd);
         }
     };
@@ -164,6 +170,7 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
         const uint8_t* qt = ldsQ + buf * L::BYTES;
         const uint8_t* yt = ldsY + buf * L::BYTES;
         const int q0 = (int)nq0;
+        const float factor = far ? 1.f : s.c;
         if (todo > 1) { advance(); ask(); }
         if (wave_on && (!s.causal || q0 + QT - 1 + s.off >= (int)w0)) {
             const bool diagonal = s.causal && q0 + s.off < (int)w0 + 31;
@@ -191,6 +198,11 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
                         }
                     __builtin_amdgcn_sched_barrier(0);
                 }
+                if (Half<T>::kScaled && far) {
+                    keep_branch();
+#pragma unroll
+                    for (int r = 0; r < 16; r++) sc[st][r] = __builtin_fmaf(sc[st][r], s.c, far_stat[buf][32 * st + (r & 3) + 8 * (r >> 2) + 4 * (int)hi]);
+                }
                 if (diagonal) {                                          // query q0 + 32 st + 4 hi + i sees this key when it is not before it
                     keep_branch();
                     const int first = (int)key - s.off - q0 - 32 * st - 4 * (int)hi;
@@ -200,7 +212,7 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
                 }
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
-                    sc[st][r] = __builtin_amdgcn_exp2f(sc[st][r] * s.c);
+                    sc[st][r] = __builtin_amdgcn_exp2f(sc[st][r] * factor);
                     dp[st][r] = sc[st][r] * dp[st][r];
                 }
                 if (Half<T>::kScaled && gr != 1.f) {

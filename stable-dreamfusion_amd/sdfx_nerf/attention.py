@@ -82,7 +82,7 @@ def attention(q, k, v, key_mask=None, causal=False, scale=None):
     keys are seen by no query, whatever their k and v hold, and get zero gradients. `causal`: query i sees keys <= i + Nk - Nq. A row that
     sees no key gives zeros and has no gradient.
 
-    fp16 / bf16 CUDA tensors with d a multiple of 8 up to 256 run csrc/attention_train.hip: any batch / head / token strides (0 of an
+    fp16 / bf16 CUDA tensors with d a multiple of 8 up to 256 and a scale in 1e-30 .. 1e30 run csrc/attention_train.hip: any batch / head / token strides (0 of an
     expanded tensor included; other layouts are copied), float32 accumulation and statistics, probabilities and their gradients rounded to
     the inputs' type for the second products. Everything else runs the same formulas in PyTorch ops. One derivative only."""
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4 or not q.is_floating_point():
@@ -99,6 +99,6 @@ def attention(q, k, v, key_mask=None, causal=False, scale=None):
         raise ValueError(f"attention: the scale must be positive and finite, got {scale}")
     if 0 in (B, H, Nq, d) or Nk == 0:
         return torch.zeros(B, Nq, H * d, dtype=q.dtype, device=q.device) + sum(t[:0].sum() for t in (q, k, v))    # (in the graph; no value is read)
-    if not (q.is_cuda and q.dtype in (torch.float16, torch.bfloat16) and d % 8 == 0 and d <= 256):
+    if not (q.is_cuda and q.dtype in (torch.float16, torch.bfloat16) and d % 8 == 0 and d <= 256 and 1e-30 <= scale <= 1e30):
         return _attention_plain(q, k, v, key_mask, causal, scale)
     return _sdfx.native().attention(q, k, v, key_mask, causal, scale)

@@ -158,3 +158,18 @@ def test_causal_rows_between_the_first_and_the_second_key_have_no_gradient_of_q_
     only = dy * lone[None, :, None]
     o, dq, dk, dv = _attend(q, k, v, only, m, True)
     assert not dq.any() and not dk.any() and dv.any() == lone.any()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("H,Hk,Nq,Nk,causal", [(2, 2, 64, 64, False), (2, 1, 700, 1000, False), (1, 1, 600, 600, True)])
+@pytest.mark.parametrize("scale,size", [(1e-8, 1.0), (2e-7, 1.0), (1e-29, 1.0), (3e-8, 3000.0), (1e-40, 1.0)])
+def test_attention_scales_of_any_smallness(dev, dtype, H, Hk, Nq, Nk, causal, scale, size):
+    """Nearly equal probabilities, and large q and k whose product a small scale brings to scores of 17 (the key whose k is the query)."""
+    d = 64
+    k = _heads(dev, 1, Hk, Nk, d, 2, dtype, size)
+    at = torch.randint(0, min(Nq, Nk), (Nq,), generator=torch.Generator().manual_seed(1)).to(dev)
+    q = k.repeat_interleave(H // Hk, 1)[:, :, at].contiguous() if size > 1 else _heads(dev, 1, H, Nq, d, 1, dtype)
+    v, dy = _heads(dev, 1, Hk, Nk, d, 3, dtype, 4.0), _rn(dev, 1, Nq, H * d, seed=4, dtype=dtype, scale=32.0)
+    got = _attend(q, k, v, dy, None, causal, scale)
+    _compare(got, *ref.attention(q, k, v, dy, None, causal, scale))
+    assert got[3].any() and (size == 1.0 or (got[1].any() and got[2].any()))

@@ -25,3 +25,15 @@ def test_a_context_mask_hides_tokens_from_heads_of_any_width(dim, heads, trainin
     for c in (ctx, far):
         assert torch.allclose(block(x, c, mask), want, rtol=1e-10, atol=1e-12)
     assert not torch.allclose(block(x, ctx), want, rtol=1e-3)
+
+
+@pytest.mark.parametrize("scale,taken", [(1e-30, True), (9e-31, False), (1e30, True), (1.1e30, False)])
+def test_the_c_entries_refuse_scales_they_cannot_carry(scale, taken):
+    """A call that is refused for its scale says so; one whose scale is taken is refused for what is checked next (misaligned rows). No launch."""
+    import ctypes
+    import _sdfx as S
+    lib, P, odd, st = S.lib(), ctypes.c_void_p(4096), ctypes.c_void_p(4100), (ctypes.c_uint64 * 3)(8, 8, 8)
+    assert lib.sdfx_attention_train_forward(odd, P, P, None, 1, 1, 1, 3, 5, 16, st, st, st, scale, 0, 0, P, None, None, P, None) == -1
+    assert (b"scale" in lib.sdfx_last_error()) != taken
+    assert lib.sdfx_attention_train_backward(odd, P, P, None, P, P, P, P, 1, 1, 1, 3, 5, 16, st, st, st, scale, 0, 0, P, P, P, P, None) == -1
+    assert (b"scale" in lib.sdfx_last_error()) != taken
