@@ -588,8 +588,9 @@ int sdfx_geglu(const void* x, uint64_t rows, uint32_t n, void* out, sdfx_stream_
  * stride; 16-byte aligned), k / v likewise over Nk keys. key_mask[B, Nk] bytes (may be NULL): 0 = no query sees the key, whatever its k and v hold.
  * causal != 0: query i sees keys <= i + Nk - Nq. A row that sees no key: o = 0, lse = +inf, no gradient. scale in 1e-30 .. 1e30.
  *   Nor has a row that sees one key a gradient for q and k.
- * forward: lse[B, H, Nq] (base-2 log-sum-exp of the scaled scores; its lowest bit marks rows that few keys carry) and o_lo (what rounding o to
- *   16 bits left, same type and layout) are what the backward needs; both NULL without one.
+ * forward: lse[B, H, Nq] (base-2 log-sum-exp of the scaled scores) and o_lo (what rounding o to 16 bits left, 16-bit integers in o's layout, in
+ *   units of the float32's last place; the lowest bit of a row's first one marks a row that few keys carry) are what the backward needs; both
+ *   NULL without one.
  * backward: dy[B, Nq, H, D] contiguous -> dq[B, Nq, H, D] (may be NULL), dk / dv[B, Nk, Hk, D] (NULL together).
  * scratch: sdfx_attention_train_scratch_bytes(..., backward) bytes, 16-byte aligned, uninitialised (0: none needed). Results do not depend
  * on the order in which workgroups run.

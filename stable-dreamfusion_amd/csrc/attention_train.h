@@ -39,7 +39,7 @@ struct Shape {
     uint32_t tiles_x;                     // workgroups along rows (forward, dq) or keys (dk / dv)
     uint32_t splits;                      // workgroups along the other axis
     float few;                            // a row whose probabilities sum to less than this, of the largest, is one that few keys carry
-    int exact;                            // few sums: every rounding of p and ds is made good (below, at mark_row)
+    int exact;                            // few sums: every rounding of p and ds is made good (below, at marked)
 };
 
 template <typename T> struct Half;
@@ -247,13 +247,25 @@ __device__ __forceinline__ uint32_t split_at(uint32_t n, uint32_t i, uint32_t sp
 //    Marking rows below 16 gains nothing that shows and costs dq 14 us at 4096 x 40, this 4.
 //  - at most 512 rows to a key head or at most 128 keys (`exact`: every row is marked, and dv takes the product too): sums of a
 //    few, or of probabilities that all lie at one place between two powers of two, are up to 2.5 times as far off.
-// The mark is the log-sum-exp's lowest bit (2^-23 of it): the forward knows the sum, the backward only its logarithm.
-__device__ __forceinline__ float mark_row(float m, float l, float few) {
-    const float lse = m + __builtin_amdgcn_logf(l);
-    const uint32_t u = __float_as_uint(lse) & ~1u;
-    return lse < INFINITY ? __uint_as_float(l < few ? u | 1u : u) : lse;
+// The forward knows the sum, the backward only its logarithm, of which no bit can be spared (2^-22 of it were 2e-4 of a probability at 1000): the
+// mark is the lowest bit of o_rest's first channel, 2^-23 of that value, and from k_prep on delta's.
+__device__ __forceinline__ bool marked(float delta) { return __float_as_uint(delta) & 1u; }
+
+// What rounding o to 16 bits left, in units of the float32's last place: 16 bits again (13 in fp16), and with them o is known exactly. (As a
+// value of the inputs' type it was known to 17 bits in bf16.) Clamped below fp16's normal range, where o then is off by at most 2^-32.
+template <typename T> __device__ __forceinline__ int o_rest(float f, T rounded) {
+    const float r = (float)rounded;
+    const int d = (int)(__float_as_uint(f) - __float_as_uint(r));
+    return __builtin_fabsf(r) < INFINITY ? max(-32768, min(32767, d)) : 0;
 }
-__device__ __forceinline__ bool marked(float lse) { return lse < INFINITY && (__float_as_uint(lse) & 1u); }
+template <typename T> __device__ __forceinline__ float o_whole(T rounded, short rest) { return __uint_as_float(__float_as_uint((float)rounded) + (uint32_t)(int)rest); }
+template <typename T> __device__ __forceinline__ void store_rest4(short* p, const float (&f)[4], bool first, bool mark) {
+    int d[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) d[i] = o_rest<T>(f[i], (T)f[i]);
+    if (first) d[0] = (d[0] & ~1) | (mark ? 1 : 0);
+    *reinterpret_cast<s4*>(p) = s4{(short)d[0], (short)d[1], (short)d[2], (short)d[3]};
+}
 
 // A row that sees one key has no ds: dp and delta are the same number, and the bits in which they differ would be all of the gradient where no
 // row has another. Which rows those are follows from the masks alone: with f1 < f2 the first two keys of the batch entry's mask, a row

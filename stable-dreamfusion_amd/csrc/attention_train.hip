@@ -16,7 +16,7 @@ namespace {
 // fragments' reloads). One query by memory (4 x 16 heads on 4 x 4 caches of 16384 x 128: 27 us for 134 MB, 5.0 TB/s; a 2 GiB copy: 4.9).
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_fwd(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
-                                                   T* __restrict__ o, T* __restrict__ o_lo, float* __restrict__ lse, float* __restrict__ part,
+                                                   T* __restrict__ o, short* __restrict__ o_lo, float* __restrict__ lse, float* __restrict__ part,
                                                    float* __restrict__ part_ml, Shape s) {
     constexpr int KT = key_tile(DP, NW), NBUF = buffers(NW), KS = DP / 16, DT = (DP + 31) / 32, NB = KT / 32;
     typedef Tile<DP, KT, 64 * NW> L;
@@ -185,9 +185,10 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_fwd(const T* __re
     }
     // a row that sees nothing: zero, and a log-sum-exp of +inf, at which the backward's exp2(s - lse) is 0
     const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
-    if (lse && hi == 0) lse[at] = l > 0.f ? mark_row(m_run, l, s.few) : (l == l ? INFINITY : l);
+    if (lse && hi == 0) lse[at] = l > 0.f ? m_run + __builtin_amdgcn_logf(l) : (l == l ? INFINITY : l);
+    const bool mark = l > 0.f && l < s.few;
     T* op = o + (((size_t)b * s.Nq + row.qi) * s.H + row.head) * s.D;
-    T* lp = o_lo ? o_lo + (((size_t)b * s.Nq + row.qi) * s.H + row.head) * s.D : nullptr;
+    short* lp = o_lo ? o_lo + (((size_t)b * s.Nq + row.qi) * s.H + row.head) * s.D : nullptr;
 #pragma unroll
     for (int dt = 0; dt < DT; dt++)
 #pragma unroll
@@ -198,7 +199,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_fwd(const T* __re
 #pragma unroll
                 for (int i = 0; i < 4; i++) f[i] = acc[dt][4 * g + i] * inv;
                 store4(op + c0, f[0], f[1], f[2], f[3]);
-                if (lp) store4(lp + c0, f[0] - (float)(T)f[0], f[1] - (float)(T)f[1], f[2] - (float)(T)f[2], f[3] - (float)(T)f[3]);
+                if (lp) store_rest4<T>(lp + c0, f, c0 == 0, mark);
             }
         }
 }
@@ -206,7 +207,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_fwd(const T* __re
 // o of the splits of each row: D / 4 channel quads x `parts` ranges of the splits are the threads of a row, the ranges added in order through LDS
 template <typename T>
 __global__ __launch_bounds__(256) void k_join_o(const float* __restrict__ part, const float* __restrict__ ml, Shape s, uint32_t parts, T* __restrict__ o,
-                                               T* __restrict__ o_lo, float* __restrict__ lse) {
+                                               short* __restrict__ o_lo, float* __restrict__ lse) {
     __shared__ f4 red[256];
     __shared__ float redl[256], redm[256];
     const uint32_t quads = s.D / 4, per = quads * parts, rows_here = 256u / per;
@@ -257,10 +258,10 @@ __global__ __launch_bounds__(256) void k_join_o(const float* __restrict__ part, 
     const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
     const uint32_t bh = (uint32_t)(r / s.Nq), qi = (uint32_t)(r - (uint64_t)bh * s.Nq), b = bh / s.H, h = bh - b * s.H;
     const size_t at = (((size_t)b * s.Nq + qi) * s.H + h) * s.D + c0;
-    if (lse && c0 == 0) lse[r] = l > 0.f ? mark_row(m, l, s.few) : (l == l ? INFINITY : l);
-    a = a * inv;
-    store4(o + at, a[0], a[1], a[2], a[3]);
-    if (o_lo) store4(o_lo + at, a[0] - (float)(T)a[0], a[1] - (float)(T)a[1], a[2] - (float)(T)a[2], a[3] - (float)(T)a[3]);
+    if (lse && c0 == 0) lse[r] = l > 0.f ? m + __builtin_amdgcn_logf(l) : (l == l ? INFINITY : l);
+    const float f[4] = {a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv};
+    store4(o + at, f[0], f[1], f[2], f[3]);
+    if (o_lo) store_rest4<T>(o_lo + at, f, c0 == 0, l > 0.f && l < s.few);
 }
 
 // out[b, n, h, :] = sum over splits of part[split][b, h, n, :], in order, for each of the gradients that were split (blockIdx.y)
@@ -290,7 +291,7 @@ __global__ __launch_bounds__(256) void k_join_sum(JoinSums js, uint32_t B, uint3
 }
 
 // ---- ahead of the gradient's kernels ---------------------------------------------------------------------------------------------
-// delta[b, h, i] = sum over channels of dy (o + o_lo): o_lo is what rounding o to 16 bits left, without which ds = p (dp - delta) of a
+// delta[b, h, i] = sum over channels of dy o, o as the forward had it ahead of its rounding (o_rest), without which ds = p (dp - delta) of a
 // peaked row loses the digits the subtraction cancels (bf16, scores with a deviation of 4: dq 5.8e-3 off instead of 2.4e-3). Also the
 // block maxima of |dy row|^2 and |v row|^2 that grad_scale reads (fp16), and with a mask each batch entry's first two keys (two_seen).
 // LR lanes a row.
@@ -318,7 +319,7 @@ __device__ __forceinline__ void find_two(const uint8_t* __restrict__ mask, uint3
     if (threadIdx.x < 2) two[threadIdx.x] = lds[threadIdx.x];
 }
 template <typename T, int LR>
-__global__ __launch_bounds__(256) void k_prep(const T* __restrict__ v, const T* __restrict__ o, const T* __restrict__ o_lo, const T* __restrict__ dy,
+__global__ __launch_bounds__(256) void k_prep(const T* __restrict__ v, const T* __restrict__ o, const short* __restrict__ o_lo, const T* __restrict__ dy,
                                              const float* __restrict__ lse, Shape s, float* __restrict__ delta, float* __restrict__ rows2, float* __restrict__ v2,
                                              uint32_t* __restrict__ seen2) {
     __shared__ float red[256 / LR];
@@ -342,6 +343,7 @@ __global__ __launch_bounds__(256) void k_prep(const T* __restrict__ v, const T* 
         if (r >= end) continue;
         float d = 0.f, q = 0.f;
         size_t at = 0;
+        uint32_t mark = 0;
         if (of_v) {
             if ((!s.mask || s.mask[(size_t)b * s.Nk + r]) && c0 < s.D) {
                 const typename Half<T>::v8 a = *reinterpret_cast<const typename Half<T>::v8*>(v + (size_t)b * s.v_sb + (size_t)r * s.v_sn + (size_t)hk * s.v_sh + c0);
@@ -352,13 +354,14 @@ __global__ __launch_bounds__(256) void k_prep(const T* __restrict__ v, const T* 
             const uint32_t g = r / s.Nq, qi = r - g * s.Nq;
             at = (((size_t)b * s.Nq + qi) * s.H + hk * s.group + g) * s.D + c0;
             if (c0 < s.D) {
-                const typename Half<T>::v8 y = *reinterpret_cast<const typename Half<T>::v8*>(dy + at), a = *reinterpret_cast<const typename Half<T>::v8*>(o + at),
-                                           l = *reinterpret_cast<const typename Half<T>::v8*>(o_lo + at);
+                const typename Half<T>::v8 y = *reinterpret_cast<const typename Half<T>::v8*>(dy + at), a = *reinterpret_cast<const typename Half<T>::v8*>(o + at);
+                const s8 l = *reinterpret_cast<const s8*>(o_lo + at);
+                mark = (uint32_t)l[0] & 1u;                       // (the row's in the lane of its first channel)
                 const bool on = lse[(size_t)bh * s.rows + r] != INFINITY;          // (the dy of a row that sees nothing may be anything)
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     const float f = (float)y[i];
-                    d = __builtin_fmaf(f, (float)a[i] + (float)l[i], d);
+                    d = __builtin_fmaf(f, o_whole<T>(a[i], l[i]), d);
                     q = __builtin_fmaf(f, f, q);
                 }
                 if (!on) d = q = 0.f;
@@ -366,7 +369,7 @@ __global__ __launch_bounds__(256) void k_prep(const T* __restrict__ v, const T* 
         }
 #pragma unroll
         for (int w = LR / 2; w >= 1; w >>= 1) { d += __shfl_xor(d, w, 64); q += __shfl_xor(q, w, 64); }
-        if (!of_v && lr == 0) delta[(size_t)bh * s.rows + r] = d;
+        if (!of_v && lr == 0) delta[(size_t)bh * s.rows + r] = __uint_as_float((__float_as_uint(d) & ~1u) | mark);
         most = fmaxf(most, q);
     }
     if (!Half<T>::kScaled) return;
@@ -401,7 +404,7 @@ void plan_keys(Shape& s) { plan(s, s.Nk, s.group * div_up(s.Nq, query_tile((int)
 template <typename T, int DP, int NW>
 void launch_fwd(const void* q, const void* k, const void* v, void* o, void* o_lo, float* lse, float* part, float* ml, const Shape& s, hipStream_t st) {
     hipLaunchKernelGGL((k_fwd<T, DP, NW>), dim3(s.tiles_x * s.splits * s.B * s.Hk), dim3(64 * NW), 0, st, static_cast<const T*>(q), static_cast<const T*>(k),
-                       static_cast<const T*>(v), static_cast<T*>(o), static_cast<T*>(o_lo), lse, part, ml, s);
+                       static_cast<const T*>(v), static_cast<T*>(o), static_cast<short*>(o_lo), lse, part, ml, s);
 }
 // (one wave alone: head widths up to 160; see plan_rows)
 template <typename T, int DP, int NW>
@@ -415,12 +418,13 @@ template <typename T> void join_o(const float* part, const float* ml, const Shap
     const uint32_t rows_here = 256 / (quads * parts);
     const uint64_t n = (uint64_t)s.B * s.H * s.Nq;
     hipLaunchKernelGGL(k_join_o<T>, dim3((uint32_t)((n + rows_here - 1) / rows_here)), dim3(256), 0, st, part, ml, s, parts, static_cast<T*>(o),
-                       static_cast<T*>(o_lo), lse);
+                       static_cast<short*>(o_lo), lse);
 }
 template <typename T> void prep(const void* v, const void* o, const void* o_lo, const void* dy, const float* lse, const Shape& s, float* delta, float* rows2, float* v2, uint32_t* seen2, hipStream_t st) {
     const uint32_t bh = s.B * s.Hk;
     const dim3 grid(bh * (prep_blocks(s.rows) + (Half<T>::kScaled ? prep_blocks(s.Nk) : 0)) + (s.mask ? s.B : 0));
-    const T *vp = static_cast<const T*>(v), *op = static_cast<const T*>(o), *lp = static_cast<const T*>(o_lo), *yp = static_cast<const T*>(dy);
+    const T *vp = static_cast<const T*>(v), *op = static_cast<const T*>(o), *yp = static_cast<const T*>(dy);
+    const short* lp = static_cast<const short*>(o_lo);
     if (s.D <= 64) hipLaunchKernelGGL((k_prep<T, 8>), grid, dim3(256), 0, st, vp, op, lp, yp, lse, s, delta, rows2, v2, seen2);
     else if (s.D <= 128) hipLaunchKernelGGL((k_prep<T, 16>), grid, dim3(256), 0, st, vp, op, lp, yp, lse, s, delta, rows2, v2, seen2);
     else hipLaunchKernelGGL((k_prep<T, 32>), grid, dim3(256), 0, st, vp, op, lp, yp, lse, s, delta, rows2, v2, seen2);

@@ -6,8 +6,10 @@
 // as many cycles there as the operands (8 of 30 reads a block); instead they ride in the products: a row carries 8 extra channels, q's
 // with (shift - lse) / c and dy's with -delta as sums of 16-bit parts, k's and v's with the parts' weights, powers of two. s and dp come out
 // of the matrix cores complete. Three parts: 24 bits in bf16, in fp16 as many as the
-// weights' range allows, at least 22 (with two, ds of a row of 2 keys that one carries by 1e4 to 1 was 8e-4 off). In fp16 the weights end
-// at 2^28: a tile with a row beyond (a small scale makes (shift - lse) / c large) leaves these channels zero and takes shift - lse from LDS.
+// weights' range allows, at least 22 (with two, ds of a row of 2 keys that one carries by 1e4 to 1 was 8e-4 off). Two things end
+// this: fp16's weights at 2^28 (a small scale makes (shift - lse) / c large), and the products' sum, which keeps float32's bits of its largest
+// term: 2^-22 of the log-sum-exp, 1.7e-4 of every probability at 1443. A tile with a row beyond 2^27 or 128 leaves these channels zero and
+// takes shift - lse from LDS, added by an fma.
 // Bound: as dq's (2 x 8 heads, 4096 x 4096 x 40, fp16: 154 us for four products, 558 TFLOP/s). A workgroup takes one key head's tile and
 // all the rows of its query heads, so that shared heads need no atomics; few key tiles split the rows and join in float32.
 #include "attention_train.h"
@@ -37,7 +39,7 @@ template <typename T> __device__ __forceinline__ u4v part_weights(float w) {
 }
 
 // CS: workgroups that share a key tile's output channels (2 at 256 channels, where dk and dv of 32 keys and the operands would fill the register file)
-// EX: dv too takes the product with what the rounding of p left (mark_row, attention_train.h)
+// EX: dv too takes the product with what the rounding of p left (marked, attention_train.h)
 template <typename T, int DM, int CS, bool EX>
 __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape s) {
     constexpr int NW = 4, DP = (DM + 8 + 15) / 16 * 16;                  // channels with the extra ones, in whole K steps
@@ -147,17 +149,18 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
         uint64_t live = left >= 64u ? ~0ull : (1ull << left) - 1ull;
         if (empties) live &= __ballot(r_lse != INFINITY);
         const bool whole = left >= (uint32_t)QT && !empties;
-        if (!EX) few = __ballot(marked(r_lse)) != 0;
+        if (!EX) few = __ballot(marked(r_delta)) != 0;
         const int lone = min(lone_end - (int)nq0, 64);                   // the tile's first so many rows
         const uint64_t lone_rows = lone <= 0 ? 0ull : lone == 64 ? ~0ull : (1ull << lone) - 1ull;
         if ((int)lane < lone && r_lse < INFINITY) r_lse = 0.f;           // (not a row that sees nothing, nor a NaN)
-        if (Half<T>::kScaled) far = __ballot(lane < (uint32_t)QT && r_lse != INFINITY && __builtin_fabsf((shift - r_lse) * inv_c) > 0x1p27f) != 0;
+        const float stat = shift - r_lse;
+        far = __ballot(lane < (uint32_t)QT && r_lse != INFINITY && (__builtin_fabsf(stat) > 128.f || __builtin_fabsf(stat * inv_c) > 0x1p27f)) != 0;
         stq.put(ldsQ + buf * L::BYTES, rq, whole && lone <= 0, live & ~lone_rows);
         sty.put(ldsY + buf * L::BYTES, ry, whole, live);
         if (lane < (uint32_t)QT) {                                       // the rows' extra channels, one tensor's by each of two waves
             if (wave == 0) {
-                *reinterpret_cast<u4v*>(ldsQ + buf * L::BYTES + lane * L::PITCH + s.D * 2u) = split_parts<T>(far ? 0.f : (shift - r_lse) * inv_c, ws);
-                if (far) far_stat[buf][lane] = shift - r_lse;
+                *reinterpret_cast<u4v*>(ldsQ + buf * L::BYTES + lane * L::PITCH + s.D * 2u) = split_parts<T>(far ? 0.f : stat * inv_c, ws);
+                if (far) far_stat[buf][lane] = stat;
             }
             if (wave == 1) *reinterpret_cast<u4v*>(ldsY + buf * L::BYTES + lane * L::PITCH + s.D * 2u) = split_parts<T>(r_lse == INFINITY ? 0.f : -r_delta * gv, wd);
         }
@@ -198,7 +201,7 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
                         }
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                if (Half<T>::kScaled && far) {
+                if (far) {
                     keep_branch();
 #pragma unroll
                     for (int r = 0; r < 16; r++) sc[st][r] = __builtin_fmaf(sc[st][r], s.c, far_stat[buf][32 * st + (r & 3) + 8 * (r >> 2) + 4 * (int)hi]);

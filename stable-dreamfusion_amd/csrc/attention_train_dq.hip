@@ -29,15 +29,15 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_dq(BwdArgs a, Sha
     row_fragments<T, KS>(qf, static_cast<const T*>(a.q) + (size_t)b * s.q_sb + (size_t)row.qi * s.q_sn + (size_t)row.head * s.q_sh, s.D, hi);
     row_fragments<T, KS>(yf, static_cast<const T*>(a.dy) + (((size_t)b * s.Nq + row.qi) * s.H + row.head) * s.D, s.D, hi);
     const size_t at = (size_t)bh * s.rows + row.R;
-    const float lse = a.lse[at];
-    const bool few = __ballot(row.on && marked(lse)) != 0;             // (some row of the wave)
+    const float lse = a.lse[at], delta = a.delta[at];
+    const bool few = __ballot(row.on && marked(delta)) != 0;            // (some row of the wave)
     float g = 1.f, vmax;
     if (Half<T>::kScaled) g = grad_scale(a.rows2 + (size_t)bh * prep_blocks(s.rows), prep_blocks(s.rows), a.v2 + (size_t)bh * prep_blocks(s.Nk), prep_blocks(s.Nk), lane, vmax);
     const TwoSeen two = two_seen(a, b);
     const int last = min(row.lim, (int)s.Nk - 1);
     const bool alone = last >= two.f1 && last < two.f2;
     // ds = p (dp - delta) g: g joins the exponent (p is used for nothing else), -delta starts dp's sum on the matrix cores
-    const float nlse = alone ? -INFINITY : Half<T>::kShift + (Half<T>::kScaled ? __builtin_amdgcn_logf(g) : 0.f) - lse, ndelta = -a.delta[at];
+    const float nlse = alone ? -INFINITY : Half<T>::kShift + (Half<T>::kScaled ? __builtin_amdgcn_logf(g) : 0.f) - lse, ndelta = -delta;
     f32x16 dp0;
 #pragma unroll
     for (int r = 0; r < 16; r++) dp0[r] = ndelta;

@@ -95,7 +95,7 @@ struct Attention : torch::autograd::Function<Attention> {
         const Tensor o = at::empty({B, Nq, H * d}, q.options());
         Tensor lo, lse, scratch;
         if (keep) {
-            lo = at::empty_like(o);
+            lo = at::empty(o.sizes(), o.options().dtype(at::kShort));
             lse = at::empty({B, H, Nq}, q.options().dtype(at::kFloat));
         }
         float* sp = scratch_of(api.attention_scratch(u(B), u(H), u(Hk), u(Nq), u(Nk), u(d), 0), q, scratch);

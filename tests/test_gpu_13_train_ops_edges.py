@@ -1,5 +1,7 @@
 """Calls of the training operators (csrc/attention_train*.hip, groupnorm_train.hip, geglu_train.hip) at the edge of what their documentation
 allows, against float64."""
+import math
+
 import pytest
 import torch
 
@@ -173,3 +175,41 @@ def test_attention_scales_of_any_smallness(dev, dtype, H, Hk, Nq, Nk, causal, sc
     got = _attend(q, k, v, dy, None, causal, scale)
     _compare(got, *ref.attention(q, k, v, dy, None, causal, scale))
     assert got[3].any() and (size == 1.0 or (got[1].any() and got[2].any()))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_attention_recomputes_probabilities_that_sum_to_one(dev, dtype):
+    """Scores about 1000, spread by 1, one query a head, dy = 1: dv is p, whose sum over 4000 keys averages dv's roundings away. Each is off by at most
+    u = 2^-11 or 2^-8 of itself, rms 0.42 u (uniform within a step, mantissas between 1 and 2); weights e^N(0, 1) make 4000 keys worth 4000 / e
+    equal ones: 0.42 u / 38, and 3.5 times that over 256 heads, 2e-5 or 1.5e-4. The other part is float32's half step of the log-sum-exp, 6.1e-5 at
+    1443, times log(2): 4.2e-5. Together 6e-5 or 1.9e-4, allowed 1e-4 and 2e-4."""
+    B, H, Nk, d = 16, 16, 4000, 64
+    q, k = _heads(dev, B, H, 1, d, 1, dtype), _heads(dev, B, H, Nk, d, 2, dtype)
+    q[..., 0], k[..., 0] = 64.0, 125.0
+    v, dy = _heads(dev, B, H, Nk, d, 3, dtype), torch.ones(B, 1, H * d, device=dev, dtype=dtype)
+    dv = _attend(q, k, v, dy)[3]
+    assert float((dv[..., 0].double().sum(-1) - 1).abs().max()) <= (1e-4 if dtype == F16 else 2e-4)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_attention_saves_what_rounding_o_left_exactly(dev, dtype):
+    """o and o_lo give the float32 output again, the log-sum-exp is whole. Probabilities enter the product in two parts, 2^-17 of them off in bf16, less in
+    fp16, with float32's sums within 2^-15 of p |v|; rounding o alone is 2^-12 / 2^-9 of o off. Whole and split key axes."""
+    import _sdfx as S
+    import ctypes
+    for Nq, Nk in ((300, 200), (3, 5000)):
+        B, H, d = 1, 2, 40
+        q, k, v = (_rn(dev, B, H, n, d, seed=i, dtype=dtype) for i, n in enumerate((Nq, Nk, Nk), 1))
+        o = torch.empty(B, Nq, H, d, dtype=dtype, device=dev)
+        lo, lse = torch.empty(B, Nq, H, d, dtype=torch.int16, device=dev), torch.empty(B, H, Nq, device=dev)
+        scratch = torch.empty(max(1, S.lib().sdfx_attention_train_scratch_bytes(B, H, H, Nq, Nk, d, 0)), dtype=torch.uint8, device=dev)
+        st = lambda t: (ctypes.c_uint64 * 3)(t.stride(0), t.stride(2), t.stride(1))
+        S.call("sdfx_attention_train_forward", S.ptr(q), S.ptr(k), S.ptr(v), None, B, H, H, Nq, Nk, d, st(q), st(k), st(v), d ** -0.5, 0, int(dtype == BF16),
+               S.ptr(o), S.ptr(lo), S.ptr(lse), S.ptr(scratch), S.stream())
+        whole = ((o.float().view(torch.int32) + lo.int()).view(torch.float32)).cpu().double()
+        qd, kd, vd = (t.cpu().double() for t in (q, k, v))
+        s = qd @ kd.transpose(-1, -2) * d ** -0.5
+        p = torch.softmax(s, -1)
+        want, size = ((p @ t).transpose(1, 2) for t in (vd, vd.abs()))
+        assert float(((whole - want).abs() - 2.0 ** -15 * size).max()) <= 0
+        assert float((torch.logsumexp(s, -1) / math.log(2) - lse.cpu().double()).abs().max()) <= 1e-5
