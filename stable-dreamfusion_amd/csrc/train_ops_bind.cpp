@@ -65,6 +65,18 @@ Tensor dense16(const Tensor& t, at::MemoryFormat f) {
     const Tensor c = t.contiguous(f);
     return reinterpret_cast<uintptr_t>(c.const_data_ptr()) % 16 ? c.clone(f) : c;
 }
+// A saved tensor as it comes back: hooks on saved tensors may have moved it into another layout (copied), but its size, type and device are what
+// the kernels' addresses are formed from.
+void same(const Tensor& t, const char* what, at::IntArrayRef sizes, at::ScalarType type, const at::Device& device) {
+    TORCH_CHECK(t.defined() && t.sizes() == sizes && t.scalar_type() == type && t.device() == device, what, ": a hook on saved tensors returned ",
+                t.defined() ? t.toString() : std::string("nothing"), " ", t.defined() ? t.sizes() : at::IntArrayRef(), " where ", type, " ", sizes, " on ",
+                device, " was saved");
+}
+Tensor back(const Tensor& t, const char* what, at::IntArrayRef sizes, at::ScalarType type, const at::Device& device,
+            at::MemoryFormat f = at::MemoryFormat::Contiguous) {
+    same(t, what, sizes, type, device);
+    return dense16(t, f);
+}
 // gradients that raise when they are differentiated again
 variable_list once(variable_list v) {
     if (!at::GradMode::is_enabled()) return v;
@@ -104,6 +116,7 @@ struct Attention : torch::autograd::Function<Attention> {
                                     q.scalar_type() == at::kBFloat16, out(o), out(lo), static_cast<float*>(out(lse)), sp, stream_of(q)));
         if (keep) {
             ctx->save_for_backward({q, k, v, mask, o, lo, lse});
+            ctx->saved_data["dims"] = std::vector<int64_t>{B, H, Hk, Nq, Nk, d};
             ctx->saved_data["causal"] = causal;
             ctx->saved_data["scale"] = scale;
         }
@@ -111,12 +124,20 @@ struct Attention : torch::autograd::Function<Attention> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list g) {
         const variable_list s = ctx->get_saved_variables();
-        const Tensor &q = s[0], &k = s[1], &v = s[2];
-        const c10::DeviceGuard guard(q.device());
-        const int64_t B = q.size(0), H = q.size(1), Nq = q.size(2), d = q.size(3), Hk = k.size(1), Nk = k.size(2);
+        const at::Device dev = g[0].device();
+        const at::ScalarType type = g[0].scalar_type();
+        const c10::DeviceGuard guard(dev);
+        const auto dims = ctx->saved_data["dims"].toIntVector();
+        const int64_t B = dims[0], H = dims[1], Hk = dims[2], Nq = dims[3], Nk = dims[4], d = dims[5];
         Tensor dq, dk, dv, scratch;
         {
             const at::AutoDispatchBelowADInplaceOrView below;
+            same(s[0], "attention", {B, H, Nq, d}, type, dev);
+            same(s[1], "attention", {B, Hk, Nk, d}, type, dev);
+            same(s[2], "attention", {B, Hk, Nk, d}, type, dev);
+            const Tensor q = rows16(s[0]), k = rows16(s[1]), v = rows16(s[2]), o = back(s[4], "attention", {B, Nq, H * d}, type, dev),
+                         lo = back(s[5], "attention", {B, Nq, H * d}, at::kShort, dev), lse = back(s[6], "attention", {B, H, Nq}, at::kFloat, dev),
+                         mask = s[3].defined() ? back(s[3], "attention", {B, Nk}, at::kBool, dev) : Tensor();
             const Tensor dy = dense16(g[0], at::MemoryFormat::Contiguous);
             if (ctx->needs_input_grad(0)) dq = at::empty({B, Nq, H, d}, q.options());
             if (ctx->needs_input_grad(1) || ctx->needs_input_grad(2)) {
@@ -125,7 +146,7 @@ struct Attention : torch::autograd::Function<Attention> {
             }
             float* sp = scratch_of(api.attention_scratch(u(B), u(H), u(Hk), u(Nq), u(Nk), u(d), 1), q, scratch);
             const Strides qs = strides(q), ks = strides(k), vs = strides(v);
-            check(api.attention_backward(in(q), in(k), in(v), in(s[3]), in(s[4]), in(s[5]), static_cast<const float*>(in(s[6])), in(dy), u(B), u(H), u(Hk),
+            check(api.attention_backward(in(q), in(k), in(v), in(mask), in(o), in(lo), static_cast<const float*>(in(lse)), in(dy), u(B), u(H), u(Hk),
                                          u(Nq), u(Nk), u(d), qs.s, ks.s, vs.s, (float)ctx->saved_data["scale"].toDouble(),
                                          ctx->saved_data["causal"].toBool(), q.scalar_type() == at::kBFloat16, out(dq), out(dk), out(dv), sp,
                                          stream_of(q)));
@@ -162,21 +183,27 @@ struct Norm : torch::autograd::Function<Norm> {
             ctx->save_for_backward({saved.defined() ? saved : x, pre, w, b, stats});
             ctx->saved_data["shape"] = x.sizes();
             ctx->saved_data["G"] = G;
-            ctx->saved_data["flags"] = (int64_t)(act ? 1 : 0) | (saved.defined() ? 2 : 0);
+            ctx->saved_data["flags"] = (int64_t)(act ? 1 : 0) | (saved.defined() ? 2 : 0) | (w.scalar_type() == at::kFloat ? 4 : 0);
         }
         return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list g) {
         const variable_list s = ctx->get_saved_variables();
-        const Tensor &pre = s[1], &w = s[2], &b = s[3], &stats = s[4];
-        const c10::DeviceGuard guard(s[0].device());
+        const at::Device dev = g[0].device();
+        const at::ScalarType type = g[0].scalar_type();
+        const c10::DeviceGuard guard(dev);
         const auto shape = ctx->saved_data["shape"].toIntVector();
         const int64_t N = shape[0], C = shape[1], HW = shape[2] * shape[3], G = ctx->saved_data["G"].toInt(), flags = ctx->saved_data["flags"].toInt();
         Tensor dx, dpre, dw, db, scratch;
         {
             const at::AutoDispatchBelowADInplaceOrView below;
             const Tensor dy = dense16(g[0], at::MemoryFormat::ChannelsLast);
-            const Tensor x = (flags & 2) ? s[0] : dense16(s[0], at::MemoryFormat::ChannelsLast);      // (hooks on saved tensors may return another layout)
+            const int64_t n = N * HW * C;
+            const Tensor x = (flags & 2) ? back(s[0], "group_norm_act", {n + n / 32}, at::kByte, dev)
+                                         : back(s[0], "group_norm_act", shape, type, dev, at::MemoryFormat::ChannelsLast);
+            const Tensor w = back(s[2], "group_norm_act", {C}, (flags & 4) ? at::kFloat : type, dev), b = back(s[3], "group_norm_act", {C}, w.scalar_type(), dev),
+                         stats = back(s[4], "group_norm_act", {N, G, 2}, at::kFloat, dev),
+                         pre = s[1].defined() ? back(s[1], "group_norm_act", {N, C}, type, dev) : Tensor();
             const size_t e = pre.defined() ? 1 : 0;                 // (an absent `pre` has no edge)
             if (ctx->needs_input_grad(0)) dx = at::empty_like(dy);
             if (e && ctx->needs_input_grad(1)) dpre = at::empty_like(pre);
@@ -215,8 +242,10 @@ struct Geglu : torch::autograd::Function<Geglu> {
         return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list g) {
-        const Tensor x = ctx->get_saved_variables()[0];
-        const c10::DeviceGuard guard(x.device());
+        const variable_list s = ctx->get_saved_variables();
+        const at::Device dev = g[0].device();
+        const c10::DeviceGuard guard(dev);
+        const bool eight = ctx->saved_data["eight"].toBool();
         Tensor dx;
         {
             const at::AutoDispatchBelowADInplaceOrView below;
@@ -224,8 +253,10 @@ struct Geglu : torch::autograd::Function<Geglu> {
             const int64_t n = dy.size(-1);
             std::vector<int64_t> shape = dy.sizes().vec();
             shape.back() = 2 * n;
+            const int64_t all = 2 * dy.numel();
+            const Tensor x = eight ? back(s[0], "geglu", {all + all / 32}, at::kByte, dev) : back(s[0], "geglu", shape, dy.scalar_type(), dev);
             dx = at::empty(shape, dy.options());
-            check(api.geglu_backward(in(x), ctx->saved_data["eight"].toBool(), in(dy), (uint64_t)(dy.numel() / n), u(n), dtype_of(dy), out(dx), stream_of(dy)));
+            check(api.geglu_backward(in(x), eight, in(dy), (uint64_t)(dy.numel() / n), u(n), dtype_of(dy), out(dx), stream_of(dy)));
         }
         variable_list r = once({dx});
         r.resize(3);

@@ -213,3 +213,43 @@ def test_attention_saves_what_rounding_o_left_exactly(dev, dtype):
         want, size = ((p @ t).transpose(1, 2) for t in (vd, vd.abs()))
         assert float(((whole - want).abs() - 2.0 ** -15 * size).max()) <= 0
         assert float((torch.logsumexp(s, -1) / math.log(2) - lse.cpu().double()).abs().max()) <= 1e-5
+
+
+# ---- hooks on saved tensors -----------------------------------------------------------------------------------------------------
+def _saving_calls(dev):
+    C = 64
+    x = _rn(dev, 2, C, 6, 7, seed=1).contiguous(memory_format=torch.channels_last)
+    w, b, pre = (_rn(dev, *s, seed=i, dtype=t) for i, (s, t) in enumerate([((C,), F32), ((C,), F32), ((2, C), F16)], 2))
+    q, m = _heads(dev, 2, 4, 33, 40, 5, F16), torch.arange(33, device=dev)[None].expand(2, 33) < 30
+    rows = x.permute(0, 2, 3, 1).reshape(-1, C)
+    return [((x, w, b, pre), lambda x, w, b, p: group_norm_act(x, 8, w, b, pre=p)), ((x, w, b), lambda x, w, b: group_norm_act(x, 8, w, b, checkpoint="int8")),
+            ((q, q * 0.5, q + 1), lambda q, k, v: attention(q, k, v, m)), ((rows,), lambda x: geglu(x, "int8")), ((rows,), lambda x: geglu(x, "full"))]
+
+
+@pytest.mark.parametrize("how", ["apart", "reversed", "misaligned"])
+def test_saved_tensors_may_come_back_in_any_layout(dev, how):
+    def unpack(t):
+        if how == "apart":                                  # every second element of a wider tensor
+            return torch.stack([t, torch.zeros_like(t)], -1)[..., 0]
+        if how == "reversed":                               # axes in the opposite order in memory
+            return t.permute(*range(t.dim() - 1, -1, -1)).contiguous().permute(*range(t.dim() - 1, -1, -1))
+        return torch.cat([t.flatten()[:1], t.flatten()])[1:].view(t.shape)
+    for args, f in _saving_calls(dev):
+        leaves = [t.detach().requires_grad_(True) for t in args]
+        y = f(*leaves)
+        want = torch.autograd.grad(y, leaves, torch.ones_like(y))
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            y = f(*leaves)
+        for a, c in zip(torch.autograd.grad(y, leaves, torch.ones_like(y)), want):
+            assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("how", ["shorter", "wider type", "on the host"])
+def test_saved_tensors_that_come_back_as_others_are_refused(dev, how):
+    unpack = {"shorter": lambda t: t[..., :-1], "wider type": lambda t: t.double(), "on the host": lambda t: t.cpu()}[how]
+    for args, f in _saving_calls(dev):
+        leaves = [t.detach().requires_grad_(True) for t in args]
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            y = f(*leaves)
+        with pytest.raises(RuntimeError, match="hook on saved tensors"):
+            torch.autograd.grad(y, leaves, torch.ones_like(y))
