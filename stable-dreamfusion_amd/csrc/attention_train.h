@@ -42,6 +42,11 @@ struct Shape {
     int exact;                            // few sums: every rounding of p and ds is made good (below, at marked)
 };
 
+// A launch takes fewer than 2^32 threads along x: workgroups beyond 2^22 go along y (many short windows: 2^24 heads of a few tokens).
+constexpr uint32_t kGridXLog2 = 22;
+inline dim3 flat_grid(uint64_t n) { return n >> kGridXLog2 ? dim3(1u << kGridXLog2, (uint32_t)((n + (1u << kGridXLog2) - 1) >> kGridXLog2)) : dim3((uint32_t)n); }
+__device__ __forceinline__ uint32_t flat_block() { return (blockIdx.y << kGridXLog2) + blockIdx.x; }          // (to be checked against the launch's count)
+
 template <typename T> struct Half;
 template <> struct Half<_Float16> {
     typedef h8 v8; typedef h4 v4; typedef h2 v2;

@@ -25,7 +25,8 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_fwd(const T* __re
     uint8_t* const ldsV = lds + NBUF * L::BYTES;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), x = lane & 31u, hi = lane >> 5;
     const uint32_t per_bh = s.tiles_x * s.splits;
-    const uint32_t lid = xcd_contiguous(blockIdx.x, per_bh * s.B * s.Hk);
+    if (flat_block() >= per_bh * s.B * s.Hk) return;
+    const uint32_t lid = xcd_contiguous(flat_block(), per_bh * s.B * s.Hk);
     const uint32_t bh = lid / per_bh, rest = lid - bh * per_bh, split = rest / s.tiles_x, xt = rest - split * s.tiles_x;
     const uint32_t b = bh / s.Hk, hk = bh - b * s.Hk;
     const uint32_t r0 = xt * NW * 32u, w0 = r0 + wave * 32u;
@@ -326,13 +327,15 @@ __global__ __launch_bounds__(256) void k_prep(const T* __restrict__ v, const T* 
     __shared__ uint32_t two[2];
     const uint32_t nr = prep_blocks(s.rows), nv = prep_blocks(s.Nk), bh_n = s.B * s.Hk;
     const uint32_t masks = bh_n * (nr + (Half<T>::kScaled ? nv : 0));          // the workgroups from here on take a mask each
-    if (blockIdx.x >= masks) {
-        const uint32_t b = blockIdx.x - masks;
+    const uint32_t block = flat_block();
+    if (block >= masks) {
+        const uint32_t b = block - masks;
+        if (!s.mask || b >= s.B) return;
         find_two(s.mask + (size_t)b * s.Nk, s.Nk, two, seen2 + 2 * b);
         return;
     }
-    const bool of_v = blockIdx.x >= bh_n * nr;
-    const uint32_t id = of_v ? blockIdx.x - bh_n * nr : blockIdx.x, per = of_v ? nv : nr;
+    const bool of_v = block >= bh_n * nr;
+    const uint32_t id = of_v ? block - bh_n * nr : block, per = of_v ? nv : nr;
     const uint32_t bh = id / per, blk = id - bh * per, b = bh / s.Hk, hk = bh - b * s.Hk;
     const uint32_t lr = threadIdx.x % LR, c0 = lr * 8u;
     const uint32_t n = of_v ? s.Nk : s.rows, end = min((blk + 1) * kPrepRows, n);
@@ -403,7 +406,7 @@ void plan_keys(Shape& s) { plan(s, s.Nk, s.group * div_up(s.Nq, query_tile((int)
 
 template <typename T, int DP, int NW>
 void launch_fwd(const void* q, const void* k, const void* v, void* o, void* o_lo, float* lse, float* part, float* ml, const Shape& s, hipStream_t st) {
-    hipLaunchKernelGGL((k_fwd<T, DP, NW>), dim3(s.tiles_x * s.splits * s.B * s.Hk), dim3(64 * NW), 0, st, static_cast<const T*>(q), static_cast<const T*>(k),
+    hipLaunchKernelGGL((k_fwd<T, DP, NW>), flat_grid((uint64_t)s.tiles_x * s.splits * s.B * s.Hk), dim3(64 * NW), 0, st, static_cast<const T*>(q), static_cast<const T*>(k),
                        static_cast<const T*>(v), static_cast<T*>(o), static_cast<short*>(o_lo), lse, part, ml, s);
 }
 // (one wave alone: head widths up to 160; see plan_rows)
@@ -421,8 +424,7 @@ template <typename T> void join_o(const float* part, const float* ml, const Shap
                        static_cast<short*>(o_lo), lse);
 }
 template <typename T> void prep(const void* v, const void* o, const void* o_lo, const void* dy, const float* lse, const Shape& s, float* delta, float* rows2, float* v2, uint32_t* seen2, hipStream_t st) {
-    const uint32_t bh = s.B * s.Hk;
-    const dim3 grid(bh * (prep_blocks(s.rows) + (Half<T>::kScaled ? prep_blocks(s.Nk) : 0)) + (s.mask ? s.B : 0));
+    const dim3 grid = flat_grid((uint64_t)s.B * s.Hk * (prep_blocks(s.rows) + (Half<T>::kScaled ? prep_blocks(s.Nk) : 0)) + (s.mask ? s.B : 0));
     const T *vp = static_cast<const T*>(v), *op = static_cast<const T*>(o), *yp = static_cast<const T*>(dy);
     const short* lp = static_cast<const short*>(o_lo);
     if (s.D <= 64) hipLaunchKernelGGL((k_prep<T, 8>), grid, dim3(256), 0, st, vp, op, lp, yp, lse, s, delta, rows2, v2, seen2);

@@ -51,7 +51,8 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
     uint8_t* const ldsQ = lds + 2 * L::BYTES;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), x = lane & 31u, hi = lane >> 5;
     const uint32_t per_bh = s.tiles_x * s.splits;
-    const uint32_t all = xcd_contiguous(blockIdx.x, per_bh * s.B * s.Hk * CS), lid = all / CS, dt0 = (all - lid * CS) * DT;
+    if (flat_block() >= per_bh * s.B * s.Hk * CS) return;
+    const uint32_t all = xcd_contiguous(flat_block(), per_bh * s.B * s.Hk * CS), lid = all / CS, dt0 = (all - lid * CS) * DT;
     const uint32_t bh = lid / per_bh, rest = lid - bh * per_bh, split = rest / s.tiles_x, xt = rest - split * s.tiles_x;
     const uint32_t b = bh / s.Hk, hk = bh - b * s.Hk;
     const uint32_t wg_key = xt * NW * 32u, w0 = wg_key + wave * 32u, key = w0 + x, kc = min(key, s.Nk - 1u);
@@ -279,7 +280,7 @@ __global__ __launch_bounds__(256, DM <= 64 ? 2 : 1) void k_dkdv(BwdArgs a, Shape
 
 template <typename T, int DM> void go(const BwdArgs& a, const Shape& s, hipStream_t st) {
     constexpr int CS = DM == 256 ? 2 : 1;
-    const dim3 grid(s.tiles_x * s.splits * s.B * s.Hk * CS);
+    const dim3 grid = flat_grid((uint64_t)s.tiles_x * s.splits * s.B * s.Hk * CS);
     if (s.exact) hipLaunchKernelGGL((k_dkdv<T, DM, CS, true>), grid, dim3(256), 0, st, a, s);
     else hipLaunchKernelGGL((k_dkdv<T, DM, CS, false>), grid, dim3(256), 0, st, a, s);
 }

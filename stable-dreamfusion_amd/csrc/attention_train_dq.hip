@@ -17,7 +17,8 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_dq(BwdArgs a, Sha
     uint8_t* const ldsK = lds + NBUF * L::BYTES;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), x = lane & 31u, hi = lane >> 5;
     const uint32_t per_bh = s.tiles_x * s.splits;
-    const uint32_t lid = xcd_contiguous(blockIdx.x, per_bh * s.B * s.Hk);
+    if (flat_block() >= per_bh * s.B * s.Hk) return;
+    const uint32_t lid = xcd_contiguous(flat_block(), per_bh * s.B * s.Hk);
     const uint32_t bh = lid / per_bh, rest = lid - bh * per_bh, split = rest / s.tiles_x, xt = rest - split * s.tiles_x;
     const uint32_t b = bh / s.Hk, hk = bh - b * s.Hk;
     const uint32_t r0 = xt * NW * 32u, w0 = r0 + wave * 32u;
@@ -167,7 +168,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 80 ? 2 : 1) void k_dq(BwdArgs a, Sha
 }
 
 template <typename T, int DP, int NW> void go(const BwdArgs& a, const Shape& s, hipStream_t st) {
-    hipLaunchKernelGGL((k_dq<T, DP, NW>), dim3(s.tiles_x * s.splits * s.B * s.Hk), dim3(64 * NW), 0, st, a, s);
+    hipLaunchKernelGGL((k_dq<T, DP, NW>), flat_grid((uint64_t)s.tiles_x * s.splits * s.B * s.Hk), dim3(64 * NW), 0, st, a, s);
 }
 template <typename T, int DP, int NW> void go_one(const BwdArgs& a, const Shape& s, hipStream_t st) { go<T, DP < 160 ? DP : 160, NW>(a, s, st); }
 

@@ -253,3 +253,19 @@ def test_saved_tensors_that_come_back_as_others_are_refused(dev, how):
             y = f(*leaves)
         with pytest.raises(RuntimeError, match="hook on saved tensors"):
             torch.autograd.grad(y, leaves, torch.ones_like(y))
+
+
+# ---- many short rows ------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("B,H,N,masked", [(2 ** 21, 8, 4, False), (2 ** 23, 8, 1, True)])
+def test_attention_of_more_heads_than_a_launch_has_threads(dev, B, H, N, masked):
+    """2^24 heads of 4 tokens, 2^26 of one: the first, middle and last batch entries bit for bit as a call of their own gives them."""
+    d = 8
+    g = torch.Generator(device=dev).manual_seed(1)
+    q, k, v, dy = (torch.empty(B, N, H * d, dtype=F16, device=dev).normal_(generator=g) for _ in range(4))
+    heads = lambda t: t.view(-1, N, H, d).transpose(1, 2)
+    m = torch.rand(B, N, device=dev, generator=g) < 0.7 if masked else None
+    got = _attend(heads(q), heads(k), heads(v), dy, m)
+    for at in (0, B // 2 - 50, B - 100):
+        cut = slice(at, at + 100)
+        want = _attend(heads(q[cut]), heads(k[cut]), heads(v[cut]), dy[cut], None if m is None else m[cut])
+        assert all(torch.equal(a[cut], c) for a, c in zip(got, want))
