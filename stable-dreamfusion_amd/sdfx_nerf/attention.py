@@ -68,6 +68,7 @@ def _attention_plain(q, k, v, key_mask, causal, scale):
     if causal:
         see = see & torch.ones(Nq, Nk, dtype=torch.bool, device=q.device).tril(Nk - Nq)
     some = see.any(-1, keepdim=True)
+    qf = qf.masked_fill(~some, 0.0)                                                        # (nor what rows hold that see nothing)
     kf, vf = (t.repeat_interleave(H // Hk, dim=1) for t in (kf, vf))
     s = torch.matmul(qf, kf.transpose(-1, -2).contiguous()) * scale
     s = s.masked_fill(~see, -float("inf")).masked_fill(~some, 0.0)                         # (a row that sees nothing: zero, below)

@@ -269,3 +269,24 @@ def test_attention_of_more_heads_than_a_launch_has_threads(dev, B, H, N, masked)
         cut = slice(at, at + 100)
         want = _attend(heads(q[cut]), heads(k[cut]), heads(v[cut]), dy[cut], None if m is None else m[cut])
         assert all(torch.equal(a[cut], c) for a, c in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("Nq,Nk", [(700, 300), (20, 9), (300, 700)])
+def test_attention_rows_that_see_no_key_may_hold_anything(dev, dtype, Nq, Nk):
+    """As the tensor operations do (tests/test_train_ops_edges.py): NaN and infinities in the queries and dy of such rows reach nothing."""
+    H, Hk, d = 4, 2, 40
+    q, k, v = _heads(dev, 2, H, Nq, d, 1, dtype), _heads(dev, 2, Hk, Nk, d, 2, dtype), _heads(dev, 2, Hk, Nk, d, 3, dtype)
+    dy = _rn(dev, 2, Nq, H * d, seed=4, dtype=dtype)
+    m = torch.ones(2, Nk, dtype=torch.bool, device=dev)
+    m[0, :5] = m[1] = False
+    n = max(0, Nq - Nk + 5)
+    want = None
+    for bad in (0.0, float("nan"), float("inf")):
+        qb, dyb = q.clone(), dy.clone()
+        qb[0, :, :n] = qb[1] = bad
+        dyb[0, :n] = dyb[1] = bad
+        got = _attend(qb, k, v, dyb, m, True)
+        want = want or got
+        assert all(torch.isfinite(t).all() for t in got) and all(torch.equal(a, b) for a, b in zip(got, want))
+    _compare(got, *ref.attention(q, k, v, dy, m, True))

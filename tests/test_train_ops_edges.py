@@ -37,3 +37,20 @@ def test_the_c_entries_refuse_scales_they_cannot_carry(scale, taken):
     assert (b"scale" in lib.sdfx_last_error()) != taken
     assert lib.sdfx_attention_train_backward(odd, P, P, None, P, P, P, P, 1, 1, 1, 3, 5, 16, st, st, st, scale, 0, 0, P, P, P, P, None) == -1
     assert (b"scale" in lib.sdfx_last_error()) != taken
+
+
+def test_a_row_that_sees_no_key_may_hold_anything():
+    """NaN and infinities in the queries and dy of rows that see nothing reach no gradient; nor do those of masked keys (in tensor operations)."""
+    q, k, v, dy = _rn(2, 2, 6, 8, seed=1), _rn(2, 2, 4, 8, seed=2), _rn(2, 2, 4, 8, seed=3), _rn(2, 6, 16, seed=4)
+    m = torch.tensor([[True] * 4, [False] * 4])
+    want = None
+    for bad in (0.0, float("nan"), float("inf")):
+        qb, dyb = q.clone(), dy.clone()
+        qb[0, :, :2] = qb[1] = bad                                    # (six queries on four keys: the first two see none)
+        dyb[0, :2] = dyb[1] = bad
+        leaves = [t.clone().requires_grad_(True) for t in (qb, k, v)]
+        o = attention(*leaves, m, True)
+        got = [o.detach(), *torch.autograd.grad(o, leaves, dyb)]
+        want = want or got
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert not got[0][0, :2].any() and got[0][0, 2:].all() and got[2][0].any()
