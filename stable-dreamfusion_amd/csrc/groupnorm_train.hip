@@ -2,6 +2,8 @@
 // vector `pre` added ahead of the norm; fp16, bf16 and float32 activations; the backward's copy of the input as it is or in 8 bits
 // (act8.h). What a prior block needs when it trains; groupnorm.hip is the frozen fp16 form.
 //   u = x + pre, xh = (u - mean) rstd, z = xh gamma + beta, y = silu(z) or z
+// In float32 xh is (u - mean) rstd, an operation at a time; in 16 bits, whose own step hides it, an affine map of x (an operation less each way:
+// mean rstd and the products with gamma round apart from x's).
 //   dz = dy silu'(z), dbeta = sum dz, dgamma = sum dz xh, g = dz gamma, dx = rstd (g - mean(g) - xh mean(g xh)), dpre = sum over pixels of dx
 // Memory bound: forward two reads and a write of the map (+ half a write of codes), backward two reads of x and dy and a write. With the
 // 8-bit input the backward's reads of x halve.
@@ -214,15 +216,20 @@ __global__ __launch_bounds__(kMaxThreads) void k_apply(const T* __restrict__ x, 
     __syncthreads();
     uint32_t pp, cv;
     if (!my_place(s, pp, cv)) return;
-    float a[8], b[8], e[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    constexpr bool kWhole = sizeof(T) == 4;
+    float a[8], b[8], e[8] = {0, 0, 0, 0, 0, 0, 0, 0}, r[8];
     load_params<T>(gamma, cv * 8, s.pf32, a);
     load_params<T>(beta, cv * 8, s.pf32, b);
     if (pre) widen(load8(pre + (size_t)n * s.C + cv * 8), e);
     GroupWalk w(s, cv * 8);
 #pragma unroll
     for (int i = 0; i < 8; i++, w.next(s)) {
-        a[i] *= mom[2 * w.g + 1];
-        b[i] = __builtin_fmaf(e[i] - mom[2 * w.g], a[i], b[i]);           // (x + e - mean) a + beta = x a + b
+        e[i] -= mom[2 * w.g];
+        r[i] = mom[2 * w.g + 1];
+        if (!kWhole) {                                                    // (x + e) r a + beta = x (a r) + b
+            a[i] *= r[i];
+            b[i] = __builtin_fmaf(e[i], a[i], b[i]);
+        }
     }
     const uint32_t p1 = min((slab + 1) * s.P, s.HW);
     const size_t at0 = (size_t)n * s.HW * s.cvs + cv;
@@ -243,8 +250,8 @@ __global__ __launch_bounds__(kMaxThreads) void k_apply(const T* __restrict__ x, 
             }
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float z = __builtin_fmaf(f[i], a[i], b[i]);
-                f[i] = ACT ? z * fast_sigmoid(z) : z;
+                const float z = __builtin_fmaf(kWhole ? (f[i] + e[i]) * r[i] : f[i], a[i], b[i]);
+                f[i] = ACT ? z * sigmoid_of<T>(z) : z;
             }
             store8(y + at * 8, f);
         }
@@ -252,13 +259,16 @@ __global__ __launch_bounds__(kMaxThreads) void k_apply(const T* __restrict__ x, 
 }
 
 // ---- backward -------------------------------------------------------------------------------------------------------------------
-template <bool ACT> __device__ __forceinline__ float dz_of(float xh, float dy, float gamma, float beta) {
+template <typename T, bool ACT> __device__ __forceinline__ float dz_of(float xh, float dy, float gamma, float beta) {
     if (!ACT) return dy;
-    const float z = __builtin_fmaf(xh, gamma, beta), sg = fast_sigmoid(z);
+    const float z = __builtin_fmaf(xh, gamma, beta), sg = sigmoid_of<T>(z);
     return dy * sg * __builtin_fmaf(z, 1.0f - sg, 1.0f);
 }
-// what a backward thread keeps of its 8 channels: xh = x r + m
+// what a backward thread keeps of its 8 channels: xh = (x + m) r in float32, x r + m in 16 bits
 struct Chan8 { float r[8], m[8], ga[8], be[8]; };
+template <typename T> __device__ __forceinline__ float xh_of(const Chan8& k, int i, float x) {
+    return sizeof(T) == 4 ? (x + k.m[i]) * k.r[i] : __builtin_fmaf(x, k.r[i], k.m[i]);
+}
 template <typename T>
 __device__ __forceinline__ void load_chan(Chan8& k, const Shape& s, uint32_t n, uint32_t cv, const float* mean_rstd, const T* pre, const void* gamma, const void* beta) {
     float e[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -270,7 +280,7 @@ __device__ __forceinline__ void load_chan(Chan8& k, const Shape& s, uint32_t n, 
     for (int i = 0; i < 8; i++, w.next(s)) {
         const float* mr = mean_rstd + ((size_t)n * s.G + w.g) * 2;
         k.r[i] = mr[1];
-        k.m[i] = (e[i] - mr[0]) * mr[1];
+        k.m[i] = sizeof(T) == 4 ? e[i] - mr[0] : (e[i] - mr[0]) * mr[1];
     }
 }
 
@@ -307,7 +317,7 @@ __global__ __launch_bounds__(kMaxThreads) void k_bwd_stats(const void* __restric
                 widen(vd[u], fd);
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const float xh = __builtin_fmaf(fx[i], k.r[i], k.m[i]), dz = dz_of<ACT>(xh, fd[i], k.ga[i], k.be[i]);
+                    const float xh = xh_of<T>(k, i, fx[i]), dz = dz_of<T, ACT>(xh, fd[i], k.ga[i], k.be[i]);
                     s1[i] += dz;
                     s2[i] = __builtin_fmaf(dz, xh, s2[i]);
                     if (PRE) s3[i] += xh;
@@ -397,7 +407,7 @@ __global__ __launch_bounds__(kMaxThreads) void k_bwd_apply(const void* __restric
                 widen(vd[u], fd);
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const float xh = __builtin_fmaf(fx[i], k.r[i], k.m[i]), dz = dz_of<ACT>(xh, fd[i], k.ga[i], k.be[i]);
+                    const float xh = xh_of<T>(k, i, fx[i]), dz = dz_of<T, ACT>(xh, fd[i], k.ga[i], k.be[i]);
                     fx[i] = k.r[i] * (__builtin_fmaf(dz, k.ga[i], -m1[i]) - xh * m2[i]);
                 }
                 store8(dx + (at0 + (size_t)(p + u * s.ppi) * s.cvs) * 8, fx);

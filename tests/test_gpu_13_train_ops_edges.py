@@ -290,3 +290,34 @@ def test_attention_rows_that_see_no_key_may_hold_anything(dev, dtype, Nq, Nk):
         want = want or got
         assert all(torch.isfinite(t).all() for t in got) and all(torch.equal(a, b) for a, b in zip(got, want))
     _compare(got, *ref.attention(q, k, v, dy, m, True))
+
+
+@pytest.mark.parametrize("act", [True, False])
+@pytest.mark.parametrize("shift,spread", [(0.0, 1.0), (3.0, 1.5), (-40.0, 1.0)])
+def test_float32_group_norm_is_as_exact_as_its_formulas(dev, act, shift, spread):
+    """The 2-norm of each error within 1.5 times that of the same formulas in float32, operation by operation, with mean and rstd rounded to float32
+    (1.5: their sums run in another order)."""
+    N, C, H, W, G = 2, 96, 37, 29, 8
+    x = (_rn(dev, N, C, H, W, seed=1, dtype=F32) * spread + shift).contiguous(memory_format=torch.channels_last)
+    w, b, dy = _rn(dev, C, seed=2, dtype=F32), _rn(dev, C, seed=3, dtype=F32) * 4, _rn(dev, N, C, H, W, seed=4, dtype=F32)
+    leaf = x.detach().requires_grad_(True)
+    y = group_norm_act(leaf, G, w, b, act=act)
+    got = {"y": y.detach(), "dx": torch.autograd.grad(y, leaf, dy)[0]}
+
+    def formulas(t):
+        per = lambda u: u.reshape(N, G, -1)
+        full = lambda u: u.expand(N, G, C // G * H * W).reshape(N, C, H, W)
+        xc, wc, bc, d = (u.cpu().to(t) for u in (x, w[None, :, None, None], b[None, :, None, None], dy))
+        mean = per(x.cpu().double()).mean(-1, keepdim=True)
+        rstd = ((per(x.cpu().double()) - mean).square().mean(-1, keepdim=True) + 1e-5).rsqrt().to(t)
+        xh = (xc - full(mean.to(t))) * full(rstd)
+        z = xh * wc + bc
+        sg = 1 / (1 + torch.exp(-z))
+        dz = d * sg * (1 + z * (1 - sg)) if act else d
+        g = dz * wc
+        avg = lambda u: full(per(u.double()).mean(-1, keepdim=True).to(t))
+        return {"y": z * sg if act else z, "dx": full(rstd) * (g - avg(g) - xh * avg(g * xh))}
+    want, plain = formulas(torch.float64), formulas(F32)
+    for n in want:
+        own, base = (float((t[n].cpu().double() - want[n]).norm()) for t in (got, plain))
+        assert own <= 1.5 * base, (n, own, base)
