@@ -196,13 +196,14 @@ class TransformerBlock(nn.Module):
         return x + self.proj_out(h.transpose(1, 2).reshape(B, C, H, W))
 
 
-def use_training_ops(module, checkpoint="int8"):
+def use_training_ops(module, checkpoint="full"):
     """Switches the group norms, attentions and feed-forwards inside `module` (a UNetSD15, a VAEEncoderSD15, or one of their blocks) to the
     forms with gradient kernels — for fine-tuning them, an adapter on them, or a gradient through them — and returns it. `checkpoint`:
-    "int8" keeps the norms' and GEGLUs' inputs for the backward in 8 bits (half the memory of half precision; channel counts that are
-    no multiple of 32 as they are), "full" as they are, None switches back. Parameters and state_dict are untouched; convolutions
-    and projections stay PyTorch's when a gradient is wanted. Heads wider than 256 (the VAE's one) keep their matrix products. A backward pass captured into a graph needs, as any of PyTorch's,
-    leaves that no live eager graph holds: autograd would make their stream wait for the captured one."""
+    "full" keeps the norms' and GEGLUs' inputs for the backward as they are, "int8" in 8 bits (half the memory of half precision, each off by
+    up to 2^-6 of the largest of its 32 channels; channel counts that are no multiple of 32 as they are), None switches back. Parameters
+    and state_dict are untouched; convolutions and projections stay PyTorch's when a gradient is wanted. Heads wider than 256 (the
+    VAE's one) keep their matrix products. A backward pass captured into a graph needs, as any of PyTorch's, leaves that no live eager graph
+    holds: autograd would make their stream wait for the captured one."""
     if checkpoint not in (None, "full", "int8"):
         raise ValueError(f'use_training_ops: checkpoint must be "int8", "full" or None, got {checkpoint!r}')
     for m in module.modules():

@@ -54,3 +54,14 @@ def test_a_row_that_sees_no_key_may_hold_anything():
         want = want or got
         assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert not got[0][0, :2].any() and got[0][0, 2:].all() and got[2][0].any()
+
+
+def test_training_ops_keep_inputs_whole_unless_8_bits_are_asked_for():
+    from sdfx_nerf.sd15_arch import ResBlock, TransformerBlock, use_training_ops
+    for block, x, more in ((ResBlock(32, 64, 16), _rn(2, 32, 4, 4, seed=1), (_rn(2, 16, seed=2),)),
+                           (TransformerBlock(32, 24, heads=2), _rn(2, 32, 4, 4, seed=1), (_rn(2, 5, 24, seed=2),))):
+        grads = {}
+        for how in ((), ("full",), ("int8",)):
+            y = use_training_ops(block, *how)(x, *more)
+            grads[how] = torch.cat([g.flatten() for g in torch.autograd.grad(y, list(block.parameters()), torch.ones_like(y))])
+        assert torch.equal(grads[()], grads[("full",)]) and not torch.equal(grads[()], grads[("int8",)])
