@@ -185,7 +185,7 @@ class TransformerBlock(nn.Module):
         else:
             h = self.proj_in(self.norm(x)).flatten(2).transpose(1, 2)
         h = self.attn1(self.n1(h), None, h)                    # (+ h: in the output projection)
-        h = self.attn2(self.n2(h), ctx, h, ctx_mask)
+        h = self.attn2(self.n2(h), ctx, h, *(() if ctx_mask is None else (ctx_mask,)))
         u = self.ff_in(self.n3(h))
         act = geglu(u) if self.checkpoint is None else geglu(u, checkpoint=self.checkpoint if u.shape[-1] % 64 == 0 else "full")
         h = linear_auto(act, self.ff_out.weight, self.ff_out.bias, h)
@@ -253,24 +253,24 @@ class UNetSD15(nn.Module):
     def forward(self, x, t, encoder_hidden_states, context_mask=None):
         """`context_mask` [B, tokens] bool (optional): which tokens of `encoder_hidden_states` are seen."""
         emb = F.silu(self.time(self.time_embedding(t).to(x.dtype)))   # every ResNet block takes SiLU(emb): applied once here
-        ctx = encoder_hidden_states.to(x.dtype)
+        ctx = (encoder_hidden_states.to(x.dtype),) + (() if context_mask is None else (context_mask,))     # (blocks that take no mask are given none)
         h = self.conv_in(x)
         hs = [h]
         for first, attn in self.down:
             if isinstance(first, ResBlock):
                 h = first(h, emb)
                 if attn is not None:
-                    h = attn(h, ctx, context_mask)
+                    h = attn(h, *ctx)
             else:
                 h = conv3x3(h, first.weight, first.bias, None, 2)   # stride-2 downsample
             hs.append(h)
         h = self.mid[0](h, emb)
-        h = self.mid[1](h, ctx, context_mask)
+        h = self.mid[1](h, *ctx)
         h = self.mid[2](h, emb)
         for res, attn, upconv in self.up:
             h = res(torch.cat([h, hs.pop()], dim=1), emb)
             if attn is not None:
-                h = attn(h, ctx, context_mask)
+                h = attn(h, *ctx)
             if upconv is not None:                           # nearest 2 x upsample + convolution (the kernel reads through the upsample)
                 h = conv3x3(h, upconv.weight, upconv.bias, None, 1, upsample=True)
         return self.conv_out(self.norm_out(h))

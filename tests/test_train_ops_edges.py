@@ -65,3 +65,24 @@ def test_training_ops_keep_inputs_whole_unless_8_bits_are_asked_for():
             y = use_training_ops(block, *how)(x, *more)
             grads[how] = torch.cat([g.flatten() for g in torch.autograd.grad(y, list(block.parameters()), torch.ones_like(y))])
         assert torch.equal(grads[()], grads[("full",)]) and not torch.equal(grads[()], grads[("int8",)])
+
+
+def test_blocks_that_take_no_mask_still_stand_in():
+    """A module put in the place of a cross-attention or of a transformer block with their older arguments is called with those."""
+    from sdfx_nerf.sd15_arch import TransformerBlock, UNetSD15
+
+    class Cross(torch.nn.Module):
+        def forward(self, x, ctx, residual):
+            return residual + ctx.mean()
+
+    class Block(torch.nn.Module):
+        def forward(self, x, ctx):
+            return x + ctx.mean()
+    torch.manual_seed(0)
+    net = UNetSD15(in_ch=4, out_ch=4, base=32, mult=(1, 2), ctx_dim=24, heads=4, res_per_level=1)
+    x, t, ctx = _rn(2, 4, 8, 8, seed=1), torch.tensor([3, 500]), _rn(2, 7, 24, seed=2)
+    net.mid[1] = Block()
+    for m in net.modules():
+        if isinstance(m, TransformerBlock):
+            m.attn2 = Cross()
+    assert net(x, t, ctx).shape == x.shape
