@@ -321,3 +321,20 @@ def test_float32_group_norm_is_as_exact_as_its_formulas(dev, act, shift, spread)
     for n in want:
         own, base = (float((t[n].cpu().double() - want[n]).norm()) for t in (got, plain))
         assert own <= 1.5 * base, (n, own, base)
+
+
+@pytest.mark.parametrize("Nq,Nk", [(300, 48), (40, 2048), (700, 900)])
+@pytest.mark.parametrize("big", ["k", "q"])
+def test_fp16_attention_keeps_the_digits_of_a_tiny_dy(dev, Nq, Nk, big):
+    """dy of 2^-17 (fp16's subnormal numbers), v of 2^6, and k (or q) so large that dq (or dk) is a normal number all the same. p and ds are rounded once
+    and the result once, sqrt(2) half steps at most in the 2-norm, and the sums: 3 allowed."""
+    H, d = 2, 64
+    size = {"q": 2.0 ** -10, "k": 2.0 ** 13} if big == "k" else {"q": 2.0 ** 13, "k": 2.0 ** -10}
+    q, k, v = (_heads(dev, 1, H, n, d, i, F16, s) for i, (n, s) in enumerate(((Nq, size["q"]), (Nk, size["k"]), (Nk, 64.0)), 1))
+    dy = _rn(dev, 1, Nq, H * d, seed=4, dtype=F32, scale=2.0 ** -17).to(F16)
+    got, (want, _) = _attend(q, k, v, dy, scale=2.0 ** -6), ref.attention(q, k, v, dy, scale=2.0 ** -6)
+    i = 1 if big == "k" else 2
+    normal = want[i].abs() > 2.0 ** -13
+    assert normal.float().mean() > 0.3
+    err = float((got[i].cpu().double() - want[i])[normal].norm() / want[i][normal].norm())
+    assert err <= 3 * ref.half_step(F16), err
