@@ -338,3 +338,34 @@ def test_fp16_attention_keeps_the_digits_of_a_tiny_dy(dev, Nq, Nk, big):
     assert normal.float().mean() > 0.3
     err = float((got[i].cpu().double() - want[i])[normal].norm() / want[i][normal].norm())
     assert err <= 3 * ref.half_step(F16), err
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("d", [8, 24, 40, 64, 72, 80, 104, 128, 160, 200, 256])
+@pytest.mark.parametrize("Nq,Nk,causal,way", [(300, 200, False, "scale"), (600, 600, True, "scale"), (530, 700, True, "offset"), (33, 40, False, "offset")])
+def test_attention_of_every_width_with_statistics_beyond_their_channels(dev, dtype, d, Nq, Nk, causal, way):
+    """A scale of 1e-9, or scores of 140 +- 1 (202 in base 2: float32 rounds such scores, and so p, by 2e-5): dk and dv take the log-sum-exp from LDS."""
+    H, Hk = 4, 2
+    q, k, v = (_heads(dev, 2, h, n, d, i, dtype) for i, (h, n) in enumerate(((H, Nq), (Hk, Nk), (Hk, Nk)), 1))
+    dy, m = _rn(dev, 2, Nq, H * d, seed=4, dtype=dtype), torch.rand(2, Nk, generator=torch.Generator().manual_seed(5)) < 0.8
+    scale = 1e-9
+    if way == "offset":
+        q[..., 0], k[..., 0], scale = 16.0, 70.0, 0.125
+    m = m.to(dev)
+    _compare(_attend(q, k, v, dy, m, causal, scale), *ref.attention(q, k, v, dy, m, causal, scale))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("seen", [(), (8500,), (4095, 4096), (0, 8999), (255, 4111), (8998, 8999)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_of_few_seen_keys_anywhere_in_a_long_mask(dev, dtype, seen, causal):
+    H, Nq, Nk, d = 2, 40, 9000, 40
+    q, k, v = (_heads(dev, 2, H, n, d, i, dtype) for i, n in enumerate((Nq, Nk, Nk), 1))
+    dy, m = _rn(dev, 2, Nq, H * d, seed=4, dtype=dtype), torch.zeros(2, Nk, dtype=torch.bool, device=dev)
+    m[0, list(seen)] = True
+    m[1, 5:9] = True
+    got = _attend(q, k, v, dy, m, causal)
+    _compare(got, *ref.attention(q, k, v, dy, m, causal))
+    last = torch.arange(Nq) + Nk - Nq if causal else torch.full((Nq,), Nk - 1)
+    sees = sum((last >= j).long() for j in seen) if seen else torch.zeros(Nq).long()
+    assert torch.equal(got[1][0].cpu().float().abs().amax((0, 2)) > 0, sees > 1)
