@@ -89,9 +89,10 @@ def build(force: bool = False, verbose: bool = False, devtools: bool = False) ->
     sources = [s for s in SOURCES if os.path.exists(os.path.join(CSRC, s))]
     lib = DEV_LIB if devtools else LIB
     with cf.ThreadPoolExecutor(max_workers=min(len(sources), os.cpu_count() or 1)) as ex:
-        bind = ex.submit(_build_bind, force, verbose)
+        bind = None if devtools else ex.submit(_build_bind, force, verbose)          # (one for both libraries)
         objs = list(ex.map(lambda s: _compile(s, force, verbose, devtools), sources))
-    bind.result()
+    if bind is not None:
+        bind.result()
     if force or not os.path.exists(lib) or os.path.getmtime(lib) < max(os.path.getmtime(o) for o in objs):
         cmd = [hipcc(), "--offload-arch=" + ARCH, "-shared", "-fPIC", "-o", lib] + objs
         if verbose:
