@@ -326,14 +326,13 @@ __global__ __launch_bounds__(256) void k_prep(const T* __restrict__ v, const T* 
     __shared__ float red[256 / LR];
     __shared__ uint32_t two[2];
     const uint32_t nr = prep_blocks(s.rows), nv = prep_blocks(s.Nk), bh_n = s.B * s.Hk;
-    const uint32_t masks = bh_n * (nr + (Half<T>::kScaled ? nv : 0));          // the workgroups from here on take a mask each
-    const uint32_t block = flat_block();
-    if (block >= masks) {
-        const uint32_t b = block - masks;
-        if (!s.mask || b >= s.B) return;
-        find_two(s.mask + (size_t)b * s.Nk, s.Nk, two, seen2 + 2 * b);
+    const uint32_t masks = s.mask ? s.B : 0u;          // the first workgroups take a mask each (a chain of latencies: last, it cost 4 us)
+    if (flat_block() < masks) {
+        find_two(s.mask + (size_t)flat_block() * s.Nk, s.Nk, two, seen2 + 2 * flat_block());
         return;
     }
+    const uint32_t block = flat_block() - masks;
+    if (block >= bh_n * (nr + (Half<T>::kScaled ? nv : 0))) return;
     const bool of_v = block >= bh_n * nr;
     const uint32_t id = of_v ? block - bh_n * nr : block, per = of_v ? nv : nr;
     const uint32_t bh = id / per, blk = id - bh * per, b = bh / s.Hk, hk = bh - b * s.Hk;
