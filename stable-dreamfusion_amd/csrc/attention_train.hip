@@ -10,7 +10,7 @@ namespace {
 // A wave owns 32 rows (of the query heads that share a key head), a workgroup of NW waves shares the key / value tiles, double-buffered
 // in LDS with the loads of tile j + 1 in flight while tile j is used. splits > 1 (few rows, a long key axis): a workgroup takes a range of
 // the tiles and leaves its unnormalised output, maximum and sum for k_join_o.
-// Bound: narrow heads by a wave's own instructions (2 x 8 heads, 4096 x 4096 x 40, fp16: 106 us, 405 TFLOP/s. A score has 160 operations of
+// Bound: narrow heads by a wave's own instructions (2 x 8 heads, 4096 x 4096 x 40, fp16: 107 us, 401 TFLOP/s; matrix units busy 29 % of the cycles, vector units 61 %. A score has 160 operations of
 // products and an exponential, a maximum, a sum and a conversion; vector and matrix cycles of a wave add up to its time, two waves a SIMD
 // overlap little of them: prodding the compiler's order towards that (scheduling groups, priorities) gained nothing, more waves lost to their
 // fragments' reloads). One query by memory (4 x 16 heads on 4 x 4 caches of 16384 x 128: 27 us for 134 MB, 5.0 TB/s; a 2 GiB copy: 4.9).

@@ -24,7 +24,7 @@
 //     two-levels-per-XCD split (275 vs 133 lines) becomes 8 equal shares: 335 -> 287 us. Without a hint every level
 //     costs the same and the split is the even one.
 //   * VALU off the critical path: level constants in scalar registers from one 32-byte record, hash / stride terms shared
-//     by the x-pair, packed half arithmetic (v_mul_f32, v_cvt_pk_f16_f32, v_pk_add_f16: bit-identical to at::Half's
+//     by the x-pair, half arithmetic in pairs (two v_mul_f32, v_cvt_pk_f16_f32, v_pk_add_f16: bit-identical to at::Half's
 //     round-after-every-operation, see Acc2), and all gathers of a lane issued before the first result is touched
 //     (more points per thread were measured slower: 2 -> -2 %, 4 -> -10 %).
 #include "grid_point.h"

@@ -20,9 +20,9 @@
 //             k_bwd_apply dx; then its waves take channels in turn: the sums over slabs and samples, in double -> dgamma, dbeta, and dpre
 //                         from the same sums: sum over pixels of dx = rstd (gamma S_dz - n m1 - m2 S_xh)
 // No atomics: partials are combined in a fixed order, results are bit-reproducible.
-// Measured, 512 x 512 x 128 fp16 with 8-bit input: k_stats 16 us (4.2 TB/s), k_apply 29 (5.9), k_bwd_stats 29 (3.5: it decodes and takes two
-// transcendentals a value), k_bwd_apply 33 (5.1); each finish 7. Maps of the UNet's lower levels end at launches: 64 x 64 x 320, four
-// kernels, 41 us in all (the engine and the host take 84).
+// Measured, 512 x 512 x 128 fp16 with 8-bit input: k_stats 17 us (3.8 TB/s; float32 sums took 16), k_apply 29 (5.9), k_bwd_stats 29 (3.5: it decodes and
+// takes two transcendentals a value), k_bwd_apply 32 (5.2); each finish 7. Maps of the UNet's lower levels end at launches: 64 x 64 x 320,
+// four kernels, 42 us in all, beside 81 us of host time for both ways.
 #include "act8.h"
 
 using namespace sdfx;

@@ -85,7 +85,8 @@ def attention(q, k, v, key_mask=None, causal=False, scale=None):
 
     fp16 / bf16 CUDA tensors with d a multiple of 8 up to 256 and a scale in 1e-30 .. 1e30 run csrc/attention_train.hip: any batch / head / token strides (0 of an
     expanded tensor included; other layouts are copied), float32 accumulation and statistics, probabilities and their gradients rounded to
-    the inputs' type for the second products. Everything else runs the same formulas in PyTorch ops. One derivative only."""
+    the inputs' type for the second products. Scores are float32: a probability is off by 2^-24 of the largest scaled score beside those roundings
+    (in the gradient, where it is found again from the log-sum-exp, as a factor of its row), so scaled scores should stay below some 10^4. Everything else runs the same formulas in PyTorch ops. One derivative only."""
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4 or not q.is_floating_point():
         raise ValueError("attention: q, k and v must be floating-point [B, H, N, d] tensors")
     (B, H, Nq, d), (Bk, Hk, Nk, dk) = q.shape, k.shape

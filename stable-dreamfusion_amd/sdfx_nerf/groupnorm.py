@@ -10,7 +10,7 @@ SDFX_GROUPNORM=0 forces the PyTorch ops everywhere (A/B switch).
 For blocks that train: `group_norm_act(...)` is the same norm with every gradient (input, gamma, beta, `pre`) in fp16, bf16 and float32
 (csrc/groupnorm_train.hip), `geglu(x, checkpoint=...)` GEGLU with its gradient (csrc/geglu_train.hip). `checkpoint` says how the input
 is kept for the backward: "full" as it is, "int8" in 8 bits (csrc/act8.h: a shared power-of-two step per 32 channels, 33 bytes instead
-of 64 in half precision). Set on a module (`GroupNormAct.checkpoint`, sd15_arch.enable_training) it selects these forms there."""
+of 64 in half precision). Set on a module (`GroupNormAct.checkpoint`, sd15_arch.use_training_ops) it selects these forms there."""
 from __future__ import annotations
 
 import torch
@@ -147,7 +147,7 @@ class _GroupNormPlainFn(torch.autograd.Function):
 
 def group_norm_act(x, groups, weight, bias, eps=1e-5, act=True, pre=None, checkpoint="full"):
     """`silu(group_norm(x + pre[:, :, None, None], groups, weight, bias, eps))` (the norm alone with `act` False) with gradients for x, `pre`,
-    weight and bias. x [N, C, H, W] in fp16, bf16 or float32, channels-last (another layout is copied into it), the result channels-last;
+    weight and bias. x [N, C, H, W] in fp16, bf16 or float32, channels-last (the kernels copy another layout into it and give a channels-last result);
     `pre` [N, C] (or None) in x's type; weight / bias [C] in x's type or float32. Statistics and sums are float32 or wider.
 
     `checkpoint`: "full" keeps x for the backward; "int8" keeps its 8-bit form (`eight_bits`; C % 32 == 0) and evaluates the
